@@ -147,6 +147,7 @@ def prepare(case, seed):
         # accumulated weight: a few heavy tokens, many light ones
         s["weights"] = torch.randn((B, hkv, cap), generator=g, device=dev).mul_(2.0).exp_()
         s["weights_out"] = torch.zeros((B, hkv, cap), device=dev)
+        s["new_len"] = torch.empty(B, dtype=torch.int32, device=dev)
         return s
     dt, hq = TYPES[c["type"]], hkv * c["group"]
     rows = lambda h: torch.randn((T, h, D), generator=g, device=dev).to(dt)  # noqa: E731
@@ -309,7 +310,7 @@ def run_own(s):
                                        out=s["acc_out"])}
     if c["op"] == "evict":
         kept, w, kv_len = m.paged_evict(cache, s["weights"], c["budget"], n_sink=c["sink"], n_recent=c["recent"],
-                                        weights_out=s["weights_out"])
+                                        weights_out=s["weights_out"], kv_len_out=s["new_len"])
         return {"k": s["k"], "v": s["v"], "kept": kept, "weights": w, "kv_len": kv_len}
     m.paged_store(cache, s["k_new"], s["v_new"], q=s["q"], q_out=s["q_out"], positions=s["positions"],
                   sections=s["sections"], n_rot=c["rot"], pairs=c["pairs"], freq_base=s["base"])
