@@ -66,6 +66,7 @@ enum mlzc_type {
 /* Kernel error bits reported by mlzc_device_errors(). */
 #define MLZC_DEVERR_WAIT_TIMEOUT 0x1u  /* a bounded mbarrier / flag wait gave up */
 #define MLZC_DEVERR_BAD_SHAPE 0x2u     /* a kernel saw a shape its launch did not promise */
+#define MLZC_DEVERR_BAD_INDEX 0x4u     /* a block table, length or row start pointed outside its tensor */
 
 /* ---------------------------------------------------------------- runtime */
 
@@ -202,6 +203,148 @@ int mlzc_flash_attn_dev(const mlzc_fa_desc* desc, void* workspace, size_t worksp
  * whose bounded wait gave up reports MLZC_DEVERR_WAIT_TIMEOUT in a device word that
  * mlzc_device_errors reads and clears (without allocating). */
 int mlzc_flash_attn_dev_noalloc(const mlzc_fa_desc* desc, void* stream);
+
+/* ------------------------------------------------------------ paged KV cache
+ *
+ * A cache shared by many sequences: K and V live in pools of pages of page_size rows, and
+ * row b of block_table names the pages of sequence b in order, so slot j of a sequence is
+ * row j % page_size of page block_table[b][j / page_size].  Four calls work on it:
+ *   mlzc_paged_store_dev    rotary positions of new tokens; their K and V into the pages,
+ *   mlzc_paged_attn_dev     attention of the new tokens over their sequences' slots,
+ *   mlzc_paged_weights_dev  the attention weight each slot received, accumulated,
+ *   mlzc_paged_evict_dev    each sequence cut down to its heaviest slots.
+ * No counterpart in the reference, whose attention reads one contiguous cache
+ * (src/simd/flash_attention.h:65-114).
+ *
+ * The new tokens of a call are rows of packed tensors: sequence b owns rows q_start[b] ..
+ * q_start[b + 1] - 1 (none, one or many), and its token i has slot
+ *   kv_len[b] - (q_start[b + 1] - q_start[b]) + i,
+ * so kv_len counts the new tokens.  A token whose slot would be negative has no slot: it is
+ * not stored and sees nothing.  Rows of the packed tensors from q_start[batch_size] on
+ * belong to no sequence and are neither read nor written.
+ *
+ * All pointers are device pointers of the current device.  block_table, kv_len and q_start
+ * are read by the kernels, so they may change between replays of a captured graph.  What
+ * they get wrong is not followed: lengths are cut to max_pages * page_size, row starts to
+ * 0 .. n_tokens, a page outside 0 .. n_pages - 1 reads as zeros and is not written; each
+ * sets MLZC_DEVERR_BAD_INDEX in the device error word.  Entries of block_table past the
+ * pages that kv_len needs are not read, and rows of a page past kv_len may hold anything. */
+typedef struct {
+    int32_t kv_type;             /* MLZC_TYPE_F16 */
+    int32_t page_size;           /* rows of a page: a multiple of 8 */
+    int64_t n_pages, head_dim;   /* head_dim 64, 128 or 256 */
+    int64_t n_head_kv, batch_size;
+    int64_t max_pages;           /* entries of a block_table row */
+    int64_t n_tokens;            /* rows of the packed tensors */
+    void* k;
+    void* v;
+    size_t k_nb[4], v_nb[4];     /* byte strides: element (2), row of a page, head, page;
+                                    pools 16-byte aligned, strides multiples of 16 */
+    const int32_t* block_table;  /* [batch_size][max_pages] */
+    size_t block_table_nb;       /* bytes between its rows */
+    const int32_t* kv_len;       /* [batch_size] */
+    const int32_t* q_start;      /* [batch_size + 1], ascending from 0 */
+} mlzc_paged_cache;
+
+/* How the dims of a rotated pair lie: (2j, 2j + 1), or (j, j + n_rot / 2). */
+#define MLZC_ROPE_ADJACENT 0
+#define MLZC_ROPE_HALVES 1
+
+/* The packed new rows of mlzc_paged_store_dev.  Rotation of pair j < n_rot / 2 of a q or k
+ * row: by the angle positions[axis(j)][token] * freq_scale * freq_base^(-2j / n_rot), where
+ * axis(j) is the position axis (one to four: text has one, pictures and video add height and
+ * width) in whose section j lies -- the first sections[0] pairs follow axis 0, the next
+ * sections[1] axis 1, and so on; the sections add up to n_rot / 2.  Dims from n_rot on are
+ * not rotated; n_rot 0: no rotation, positions not read. */
+typedef struct {
+    int32_t type;                /* of q, k, v and q_dst: MLZC_TYPE_F32 or MLZC_TYPE_F16 */
+    int32_t pairs;               /* MLZC_ROPE_ADJACENT or MLZC_ROPE_HALVES */
+    int32_t n_rot;               /* a multiple of 8, at most head_dim */
+    int32_t n_axes;
+    int32_t sections[4];
+    float freq_base, freq_scale;
+    const int32_t* positions;    /* [n_axes][n_tokens], axis stride positions_nb */
+    size_t positions_nb;
+    int64_t n_head_q;            /* heads of q; 0: no q */
+    const void* q;               /* rows [token][head][head_dim]: q_nb = element, head, token */
+    const void* k;
+    const void* v;
+    void* q_dst;                 /* rotated q; may be q itself */
+    size_t q_nb[3], k_nb[3], v_nb[3], q_dst_nb[3];   /* heads and tokens on 16-byte boundaries */
+} mlzc_paged_store_desc;
+
+/* Writes the new tokens' rotated k and their v into the cache (rounded to f16 once) and the
+ * rotated q to q_dst, on `stream`.  Angles are exact to a 2^-32 of a turn at any position.
+ * Two tokens with one slot, or sequences sharing a page that is written, race. */
+int mlzc_paged_store_dev(const mlzc_paged_cache* cache, const mlzc_paged_store_desc* desc, void* stream);
+
+/* The query side of mlzc_paged_attn_dev and mlzc_paged_weights_dev. */
+typedef struct {
+    int32_t type;                /* of q and dst: MLZC_TYPE_F32 or MLZC_TYPE_F16 */
+    uint32_t mode;               /* 0 or MLZC_FA_MODE_SOFTCAP (slots are no positions after an
+                                    eviction, so ALiBi is not taken) */
+    int64_t n_head_q;            /* a multiple of n_head_kv, at most 128 times it */
+    float scale, logit_softcap;  /* scale > 0 */
+    const void* q;               /* [token][head][head_dim], q_nb = element, head, token */
+    void* dst;                   /* the same shape */
+    size_t q_nb[3], dst_nb[3];   /* heads and tokens on 16-byte boundaries */
+    float* lse;                  /* [token][head] ln of the sum of exp(score): written by the
+                                    attention (NULL: not wanted), read by the weights */
+    size_t lse_nb[2];            /* head (4), token */
+} mlzc_paged_attn_desc;
+
+/* Workspace (device bytes, 16-byte aligned) that mlzc_paged_attn_dev needs; it depends on
+ * the current device. */
+int mlzc_paged_attn_workspace_bytes(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, size_t* out_bytes);
+
+/* Attention of every new token over the slots of its sequence up to its own (so a chunk is
+ * causal within itself and sees all that was cached before it): score s = scale * <q, k>,
+ * softcap * tanh(s / softcap) in SOFTCAP mode; KV head of query head h: h * n_head_kv /
+ * n_head_q.  A token that sees nothing gets zeros and lse = -inf.
+ * type F32: q, the weights and the sums keep f32 precision (q and the softmax weights go
+ * through the tensor cores as f16 hi + lo pairs); type F16: q is f16 as given, the softmax
+ * weights are rounded to f16 once, sums are f32, dst is rounded once.
+ * K and V of the slots below kv_len are finite. */
+int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+int mlzc_paged_weights_workspace_bytes(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc,
+                                       size_t* out_bytes);
+
+/* out[b][kv head][slot] = acc[b][kv head][slot] + the sum of exp(s - lse) over the new
+ * tokens that see the slot and the query heads of the kv head, for the slots below kv_len;
+ * acc NULL starts from 0, acc == out accumulates in place (with the same strides).  f32,
+ * byte strides nb = slot (4), head, sequence.  desc: q, scale, mode, softcap and lse as given
+ * to and returned by mlzc_paged_attn_dev; dst is not used.  A token with lse = -inf adds
+ * nothing.  The result repeats bit for bit. */
+int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, const float* acc,
+                           const size_t acc_nb[3], float* out, const size_t out_nb[3], void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Cuts every sequence with kv_len > budget down to `budget` slots a head, in place.
+ * n_sink + n_recent <= budget. */
+typedef struct {
+    int64_t budget, n_sink, n_recent;
+    const float* weights;        /* [b][kv head][slot] */
+    float* weights_out;          /* the same; may be `weights` itself (with the same strides) */
+    size_t weights_nb[3], weights_out_nb[3];   /* slot (4), head, sequence */
+    int32_t* kept;               /* [b][kv head][budget]: the slot that now lies in each slot */
+    size_t kept_nb[3];
+    int32_t* kv_len_out;         /* [b] = min(kv_len, budget); may be kv_len itself */
+} mlzc_paged_evict_desc;
+
+int mlzc_paged_evict_workspace_bytes(const mlzc_paged_cache* cache, const mlzc_paged_evict_desc* desc, size_t* out_bytes);
+
+/* Each (sequence, kv head) keeps its first n_sink and last n_recent slots, and of the others
+ * those of the largest weight (of equal weights the lowest slot; -0 equals 0, NaN comes
+ * last).  Kept rows of K and V at slots >= budget move, in order, into the freed slots below
+ * it, in order; no other row moves.  So the slots of a head are not its positions any more
+ * (and differ from head to head): rotate k before it is stored.  kept: the former slot of
+ * each slot, -1 past the new length.  weights_out: the kept slots' weights, 0 in the freed
+ * slots new length .. kv_len - 1.  q_start is not read.  A sequence whose pages are shared
+ * with another must not be cut. */
+int mlzc_paged_evict_dev(const mlzc_paged_cache* cache, const mlzc_paged_evict_desc* desc, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------ host-pointer (hook) level */
 

@@ -12,6 +12,8 @@ from ._lib import (EXPORTS, FA_MODE_ALIBI, FA_MODE_GQA_BATCH, FA_MODE_SOFTCAP, L
                    TYPE_Q4_K, TYPE_Q5_0, TYPE_Q5_1, TYPE_Q6_K, TYPE_Q8_0,
                    UNIQUE_ID_BYTES, FaDesc, MlzcError, TensorView, check, get_launch_overlap,
                    last_error, launch_count, lib, set_launch_overlap)
+from ._lib import DEVERR_BAD_INDEX, ROPE_ADJACENT, ROPE_HALVES
+from .paged import PagedCache, paged_attn, paged_attn_workspace_bytes, paged_evict, paged_store, paged_weights
 from .ops import (Comm, Weight, device_errors, flash_attn_dispatch, flash_attn_dispatch_quant,
                   flash_attn_workspace_bytes,
                   ggml_simd_try_flash_attn, ggml_simd_try_mul_mat, init, make_fa_desc, mul_mat,
@@ -26,5 +28,6 @@ __all__ = [
     "last_error", "launch_count", "lib", "Comm", "Weight", "device_errors", "flash_attn_dispatch", "flash_attn_dispatch_quant",
     "flash_attn_workspace_bytes", "ggml_simd_try_flash_attn", "ggml_simd_try_mul_mat", "init",
     "make_fa_desc", "mul_mat", "mul_mat_workspace_bytes", "quantize_q8k", "selftest_wait_timeout", "shutdown", "tensor_view",
-    "weight_type_of",
+    "weight_type_of", "PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store",
+    "paged_weights", "DEVERR_BAD_INDEX", "ROPE_ADJACENT", "ROPE_HALVES",
 ]

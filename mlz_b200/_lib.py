@@ -22,6 +22,8 @@ TYPE_Q4_1, TYPE_Q5_0, TYPE_Q5_1, TYPE_IQ4_NL = 3, 6, 7, 20   # quantised KV-cach
 FA_MODE_GQA_BATCH, FA_MODE_ALIBI, FA_MODE_SOFTCAP = 0x04, 0x08, 0x10
 OVERLAP_OFF, OVERLAP_SAFE, OVERLAP_WEIGHTS = 0, 1, 2
 UNIQUE_ID_BYTES = 128
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+DEVERR_WAIT_TIMEOUT, DEVERR_BAD_SHAPE, DEVERR_BAD_INDEX = 0x1, 0x2, 0x4
 
 # every symbol include/mlzc.h declares (checked by the CPU test suite)
 EXPORTS = (
@@ -30,6 +32,9 @@ EXPORTS = (
     "mlzc_set_launch_overlap", "mlzc_get_launch_overlap",
     "mlzc_mul_mat_workspace_bytes", "mlzc_mul_mat_dev", "mlzc_quantize_q8k_dev",
     "mlzc_flash_attn_workspace_bytes", "mlzc_flash_attn_dev", "mlzc_flash_attn_dev_noalloc",
+    "mlzc_paged_store_dev", "mlzc_paged_attn_workspace_bytes", "mlzc_paged_attn_dev",
+    "mlzc_paged_weights_workspace_bytes", "mlzc_paged_weights_dev",
+    "mlzc_paged_evict_workspace_bytes", "mlzc_paged_evict_dev",
     "mlzc_try_mul_mat", "mlzc_try_flash_attn",
     "mlzc_weight_upload", "mlzc_weight_free", "mlzc_mul_mat", "mlzc_weight_cache_clear",
     "mlzc_host_register", "mlzc_host_unregister",
@@ -58,6 +63,46 @@ class FaDesc(C.Structure):
         ("mask_nb", C.c_size_t * 4), ("dst_nb", C.c_size_t * 4),
         ("k_type", C.c_int32), ("v_type", C.c_int32),
         ("kv_len", C.c_void_p),
+    ]
+
+
+class PagedCacheDesc(C.Structure):
+    """Mirror of mlzc_paged_cache."""
+    _fields_ = [
+        ("kv_type", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int64), ("head_dim", C.c_int64),
+        ("n_head_kv", C.c_int64), ("batch_size", C.c_int64), ("max_pages", C.c_int64), ("n_tokens", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_nb", C.c_size_t * 4), ("v_nb", C.c_size_t * 4),
+        ("block_table", C.c_void_p), ("block_table_nb", C.c_size_t), ("kv_len", C.c_void_p), ("q_start", C.c_void_p),
+    ]
+
+
+class PagedStoreDesc(C.Structure):
+    """Mirror of mlzc_paged_store_desc."""
+    _fields_ = [
+        ("type", C.c_int32), ("pairs", C.c_int32), ("n_rot", C.c_int32), ("n_axes", C.c_int32),
+        ("sections", C.c_int32 * 4), ("freq_base", C.c_float), ("freq_scale", C.c_float),
+        ("positions", C.c_void_p), ("positions_nb", C.c_size_t), ("n_head_q", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_dst", C.c_void_p),
+        ("q_nb", C.c_size_t * 3), ("k_nb", C.c_size_t * 3), ("v_nb", C.c_size_t * 3), ("q_dst_nb", C.c_size_t * 3),
+    ]
+
+
+class PagedAttnDesc(C.Structure):
+    """Mirror of mlzc_paged_attn_desc."""
+    _fields_ = [
+        ("type", C.c_int32), ("mode", C.c_uint32), ("n_head_q", C.c_int64), ("scale", C.c_float),
+        ("logit_softcap", C.c_float), ("q", C.c_void_p), ("dst", C.c_void_p),
+        ("q_nb", C.c_size_t * 3), ("dst_nb", C.c_size_t * 3), ("lse", C.c_void_p), ("lse_nb", C.c_size_t * 2),
+    ]
+
+
+class PagedEvictDesc(C.Structure):
+    """Mirror of mlzc_paged_evict_desc."""
+    _fields_ = [
+        ("budget", C.c_int64), ("n_sink", C.c_int64), ("n_recent", C.c_int64),
+        ("weights", C.c_void_p), ("weights_out", C.c_void_p),
+        ("weights_nb", C.c_size_t * 3), ("weights_out_nb", C.c_size_t * 3),
+        ("kept", C.c_void_p), ("kept_nb", C.c_size_t * 3), ("kv_len_out", C.c_void_p),
     ]
 
 
@@ -101,6 +146,15 @@ def _declare(L: C.CDLL) -> None:
     L.mlzc_flash_attn_workspace_bytes.argtypes = [C.POINTER(FaDesc), psz]
     L.mlzc_flash_attn_dev.argtypes = [C.POINTER(FaDesc), vp, sz, vp]
     L.mlzc_flash_attn_dev_noalloc.argtypes = [C.POINTER(FaDesc), vp]
+    pc, pa = C.POINTER(PagedCacheDesc), C.POINTER(PagedAttnDesc)
+    pe, nb3 = C.POINTER(PagedEvictDesc), C.POINTER(C.c_size_t)
+    L.mlzc_paged_store_dev.argtypes = [pc, C.POINTER(PagedStoreDesc), vp]
+    L.mlzc_paged_attn_workspace_bytes.argtypes = [pc, pa, psz]
+    L.mlzc_paged_attn_dev.argtypes = [pc, pa, vp, sz, vp]
+    L.mlzc_paged_weights_workspace_bytes.argtypes = [pc, pa, psz]
+    L.mlzc_paged_weights_dev.argtypes = [pc, pa, vp, nb3, vp, nb3, vp, sz, vp]
+    L.mlzc_paged_evict_workspace_bytes.argtypes = [pc, pe, psz]
+    L.mlzc_paged_evict_dev.argtypes = [pc, pe, vp, sz, vp]
     L.mlzc_try_mul_mat.argtypes = [C.POINTER(TensorView)] * 3 + [i32, i32]
     L.mlzc_try_flash_attn.argtypes = [C.POINTER(FaDesc), i32, i32]
     L.mlzc_weight_upload.argtypes = [i32, i32, vp, sz, i64, i64, C.POINTER(vp)]

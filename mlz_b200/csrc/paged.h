@@ -1,0 +1,73 @@
+// paged.h -- the paged KV cache as its kernels see it (paged_*.cu): device view, length rules
+// and the host-side argument checks.
+#pragma once
+
+#include "internal.h"
+
+namespace mlzc {
+namespace paged {
+
+// Pools, block table and lengths of one call.  Strides in bytes.
+struct View {
+    char* k;
+    char* v;
+    size_t k_row, k_head, k_page, v_row, v_head, v_page;
+    const int* table;
+    size_t table_nb;
+    const int* kv_len;
+    const int* q_start;
+    int page, max_pages, n_pages, n_head_kv, batch, n_tokens, cap;   // cap = max_pages * page
+    unsigned int* err;
+};
+
+// A sequence's share of the call: `rows` new tokens from packed row `row0`, `kv` slots.  New
+// token i has slot kv - rows + i (negative: none).
+struct Seq {
+    int row0, rows, kv;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int ld_int(const int* p) {
+    int v;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
+// Reads a sequence's lengths and cuts them to the tensors (see mlzc_paged_cache).
+__device__ __forceinline__ Seq load_seq(const View& c, int b, bool with_rows = true) {
+    Seq s;
+    const int kv = ld_int(c.kv_len + b);
+    s.kv = min(max(kv, 0), c.cap);
+    bool bad = s.kv != kv;
+    s.row0 = s.rows = 0;
+    if (with_rows) {
+        const int q0 = ld_int(c.q_start + b), q1 = ld_int(c.q_start + b + 1);
+        s.row0 = min(max(q0, 0), c.n_tokens);
+        const int end = min(max(q1, s.row0), c.n_tokens);
+        s.rows = end - s.row0;
+        bad |= s.row0 != q0 || end != q1;
+    }
+    if (bad) atomicOr(c.err, MLZC_DEVERR_BAD_INDEX);
+    return s;
+}
+
+// Page of index `i` of sequence b, or -1 (and the error bit) where it is outside the pools.
+__device__ __forceinline__ int load_page(const View& c, int b, int i) {
+    const int p = ld_int(reinterpret_cast<const int*>(reinterpret_cast<const char*>(c.table) + (size_t)b * c.table_nb) + i);
+    if ((unsigned)p < (unsigned)c.n_pages) return p;
+    atomicOr(c.err, MLZC_DEVERR_BAD_INDEX);
+    return -1;
+}
+#endif
+
+// Fills `out` from `cache` after checking it; `rows`: the call reads q_start and n_tokens.
+int make_view(const mlzc_paged_cache* cache, bool rows, const DeviceCtx* c, View* out);
+int check_cache(const mlzc_paged_cache* cache, bool rows);
+// q / dst / lse of the attention and weights calls.
+int check_attn(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, bool weights);
+// A packed [token][head][head_dim] tensor on 16-byte boundaries.
+int check_rows(const char* what, const void* p, const size_t* nb, int64_t heads, int64_t tokens, size_t row_bytes,
+               size_t elem);
+
+}  // namespace paged
+}  // namespace mlzc
