@@ -65,6 +65,13 @@ int make_view(const mlzc_paged_cache* cache, bool rows, const DeviceCtx* c, View
 int check_cache(const mlzc_paged_cache* cache, bool rows);
 // q / dst / lse of the attention and weights calls.
 int check_attn(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, bool weights);
+// Tensor map of a pool (K or V): dims head_dim, row, head, page; boxes of 64 values x box_rows
+// rows in the 128-byte swizzle.
+int encode_pool(CUtensorMap* map, const mlzc_paged_cache* cache, bool v, int box_rows);
+// Tensor map of packed f16 rows [token][head][D]: dims D, head, token; boxes of 64 values x
+// `heads` heads x `tokens` tokens in the 128-byte swizzle.
+int encode_rows(CUtensorMap* map, const void* p, int64_t D, int64_t n_heads, int64_t n_tokens, size_t head_nb,
+                size_t token_nb, int heads, int tokens);
 // A packed [token][head][head_dim] tensor on 16-byte boundaries.
 int check_rows(const char* what, const void* p, const size_t* nb, int64_t heads, int64_t tokens, size_t row_bytes,
                size_t elem);

@@ -1,88 +1,765 @@
-// paged_attn.cu -- attention of new tokens over a paged KV cache (mlzc_paged_attn_dev).
+// paged_attn.cu -- attention of new tokens over a paged KV cache (mlzc_paged_attn_dev) on the
+// 5th-generation tensor cores.
 //
-// One warp a query row: online softmax over the slots the row sees, the head's dims spread over
-// the lanes.
+// One pass over a sequence's slots with the softmax's running maximum and sum:
+//   S = Q K^T,  m' = max(m, row max S),  P = 2^(c (S - m')),  l' = a l + row sum P,
+//   O' = a O + P V,  a = 2^(c (m - m')),  c = scale * log2 e;  out = O / l, lse = m scale + ln l.
+// The query rows of a sequence that share a KV head (its new tokens x the head's G query heads)
+// are packed into tiles of up to 128 rows, so K and V are read once for G heads: rows of a
+// tile are (token, head in group), tokens outermost.
+//
+// A CTA walks BN-slot tiles of K and V:
+//   loader warp    K and V tiles by TMA into a ring, one box per page piece (box height
+//                  gcd(page, BN), so a box never crosses a page); each lane looks up its own
+//                  box's page in the block table and issues its own copies;
+//   Q warp         the next piece's Q tile (f16: TMA; f32: split into f16 hi + lo);
+//   MMA warp       S = Q K^T (operands in shared memory) and O += P V (P in TMEM, V as an
+//                  N-contiguous B operand) with tcgen05.mma, accumulators in TMEM;
+//   softmax warps  one thread a row: S from TMEM, P back over it.  O is rescaled only when
+//                  the maximum has risen by more than 8 in the exponent (P then stays below 2^8
+//                  times its offset), so in the steady state no thread touches O.
+// NS = 2: two query tiles with a softmax warpgroup each share every K and V tile, and the
+// tensor cores work on one while the other is in the softmax; for calls with more than 128
+// query rows a sequence.  NS = 1: one tile and two S buffers; for decode (the time is that of
+// reading K and V) and for head_dim 256 (whose O takes half of TMEM).
+//
+// f32 calls keep f32 precision: Q = Qhi + Qlo and P = Phi + Plo (f16 each, 22 bits), twice the
+// products, all summed in f32.  f16 calls round P to f16 once: P V then carries the rounding
+// that the output's type has anyway.
+//
+// All (sequence, KV head, query tile, slot tile) of a call form one list, of which every CTA
+// takes an equal contiguous share (few rows over a long cache and many rows over a short one
+// balance alike).  A query tile that a share boundary cuts leaves partial (O, m, l) records in
+// the workspace, merged in slot order by the combine launch: results repeat bit for bit.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <numeric>
 
 #include "paged.h"
 #include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace mlzc {
 namespace {
 
 using paged::Seq;
 using paged::View;
+using ptx::mbar_arrive;
+using ptx::mbar_expect_tx;
+using ptx::mbar_init;
+using ptx::mbar_wait;
+using ptx::smem_u32;
+using namespace tc05;
+
+constexpr int kSmemMax = 232448;
+constexpr int kBarBytes = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// P carries a factor 2^6: f16 then holds weights down to 2^-20 of the largest at full
+// precision, and with the rescaling threshold 2^8 the largest P is 2^14 (f16 ends at 2^16).
+constexpr float kPOffset = 6.0f;
+constexpr float kRescale = 8.0f;
 
 struct AttnArgs {
     View c;
+    CUtensorMap mk, mv, mq;
     const char* q;
     char* dst;
-    size_t q_head, q_tok, d_head, d_tok, lse_head, lse_tok;
     char* lse;
-    int n_head_q, f32;
-    float scale, softcap;
+    size_t q_head, q_tok, d_head, d_tok, lse_head, lse_tok;
+    int G, tq;                 // query heads a KV head; tokens a tile (tq * G <= 128)
+    int box;                   // rows of a K / V box
+    float scale, softcap;      // softcap 0: none
+    int n_ctas, rec_rows;
+    float* rec;                // [cta][2][rec_rows][D]: 0 continues a cut tile, 1 begins one
+    float2* ml;                // [cta][2][rec_rows]: exponent of the record's scale, sum
+    int4* head;                // [cta]: sequence (-1: none), kv head, query tile, last CTA of the tile begun in record 1
 };
 
-constexpr int kWarps = 8;
+template <int D_, int NS_, bool HL_>
+struct Cfg {
+    static constexpr int D = D_, NS = NS_;
+    static constexpr bool HL = HL_;
+    static constexpr int BN = D == 256 ? 64 : 128;
+    static constexpr int SUBS = D / 64;
+    static constexpr uint32_t kQSub = 128 * 128;          // bytes of a 64-value block of a Q tile
+    static constexpr uint32_t kQTile = kQSub * SUBS;
+    static constexpr uint32_t kQBytes = kQTile * NS * (HL ? 2 : 1);   // [tile][hi, lo]
+    static constexpr uint32_t kSub = BN * 128;            // bytes of a 64-value block of a K / V tile
+    static constexpr uint32_t kSlot = kSub * SUBS;
+    static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - (int)kQBytes) / (int)kSlot;
+    static constexpr int ST = kFit > 8 ? 8 : kFit;
+    static constexpr size_t kSmem = 1024 + kBarBytes + kQBytes + (size_t)ST * kSlot;
+    static constexpr int kSoftWarps = 4 * NS;
+    static constexpr int kThreads = (kSoftWarps + 4) * 32;
+    static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
+    static constexpr uint32_t kOCol = 2 * BN;             // O of tile i at + i * D
+    static_assert(2 * BN + NS * D <= 512, "TMEM");
+    static_assert(ST >= 3, "ring");
+};
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32) attn_kernel(const __grid_constant__ AttnArgs a) {
-    constexpr int E = D / 32;
+// Barriers in shared memory.
+struct Bars {
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_step, o_done[2], o_empty[2];
+    uint32_t tmem;
+    int abort;
+    long long first, count, total;   // this CTA's share of the list; its start's place
+    int b, h, t, tile;
+    long long scan[12];
+};
+static_assert(sizeof(Bars) <= kBarBytes, "barriers");
+
+// Slots that query tile t of a sequence sees, and its slot tiles (one at least, so that rows
+// which see nothing are written too).
+template <int BN>
+__device__ __forceinline__ int visible(const Seq& s, int t, int tokens) {
+    const int64_t e = (int64_t)(t + 1) * tokens;
+    return max(0, s.kv - s.rows + (int)(e < s.rows ? e : s.rows));
+}
+template <int BN>
+__device__ __forceinline__ int tiles_of(const Seq& s, int t, int tokens) {
+    return max(1, (visible<BN>(s, t, tokens) + BN - 1) / BN);
+}
+
+// A walk over this CTA's share: piece after piece (the tiles of one query tile).
+template <class C>
+struct Walk {
+    int b, h, t, tile, n;      // the piece: slot tiles [tile, tile + n)
+    long long left;
+    Seq s;
+    bool first;
+    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(B->tile), n(0), left(B->count), first(true) {}
+    // Moves to the next piece; false at the end.
+    __device__ bool next(const AttnArgs& a) {
+        if (left <= 0) return false;
+        const int tokens = a.tq * C::NS;
+        if (first) {
+            s = paged::load_seq(a.c, b);
+            first = false;
+        } else {
+            tile = 0;
+            if ((int64_t)(++t) * tokens >= s.rows) {
+                t = 0;
+                if (++h == a.c.n_head_kv) {
+                    h = 0;
+                    do {
+                        s = paged::load_seq(a.c, ++b);
+                    } while (s.rows == 0);   // the list ends at a sequence with rows
+                }
+            }
+        }
+        const int all = tiles_of<C::BN>(s, t, tokens) - tile;
+        n = (int)min((long long)all, left);
+        left -= n;
+        return true;
+    }
+    __device__ int tok0(const AttnArgs& a) const { return t * a.tq * C::NS; }
+    __device__ int tiles(const AttnArgs& a) const { return C::NS == 2 && tok0(a) + a.tq < s.rows ? 2 : 1; }
+    __device__ bool ends(const AttnArgs& a) const { return tile + n == tiles_of<C::BN>(s, t, a.tq * C::NS); }
+};
+
+// Finds this CTA's share.  Threads own runs of sequences: their tile counts are summed over the
+// block, then the owner of the share's first tile walks to it.
+template <class C>
+__device__ void plan(const AttnArgs& a, Bars* B) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.c.batch + C::kThreads - 1) / C::kThreads;
+    const int b0 = tid * per, b1 = min(b0 + per, a.c.batch);
+    const int tokens = a.tq * C::NS;
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Seq s = paged::load_seq(a.c, b);
+        long long one = 0;
+        for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of<C::BN>(s, t, tokens);
+        mine += one * a.c.n_head_kv;
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) B->scan[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < C::kThreads / 32; ++w) {
+        if (w < warp) upto += B->scan[w];
+        total += B->scan[w];
+    }
+    const long long n = min((long long)a.n_ctas, total), c = blockIdx.x;
+    const long long lo = c < n ? total * c / n : 0, hi = c < n ? total * (c + 1) / n : 0;
+    if (tid == 0) { B->first = lo; B->count = hi - lo; B->total = total; }
+    if (hi > lo && lo >= upto - mine && lo < upto) {
+        long long r = lo - (upto - mine);
+        for (int b = b0; b < b1; ++b) {
+            const Seq s = paged::load_seq(a.c, b);
+            long long one = 0;
+            for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of<C::BN>(s, t, tokens);
+            if (r >= one * a.c.n_head_kv) { r -= one * a.c.n_head_kv; continue; }
+            B->b = b;
+            B->h = (int)(r / one);
+            r %= one;
+            int t = 0;
+            while (r >= tiles_of<C::BN>(s, t, tokens)) r -= tiles_of<C::BN>(s, t++, tokens);
+            B->t = t;
+            B->tile = (int)r;
+            break;
+        }
+    }
+    __syncthreads();
+}
+
+// 32 accumulator columns to a dst row (f16 or f32) or a record row.
+__device__ __forceinline__ void put32(float* p, const float (&x)[32]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+}
+__device__ __forceinline__ void put32(__half* p, const float (&x)[32]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(ptx::pack_h2(x[8 * i], x[8 * i + 1]), ptx::pack_h2(x[8 * i + 2], x[8 * i + 3]),
+                                                    ptx::pack_h2(x[8 * i + 4], x[8 * i + 5]), ptx::pack_h2(x[8 * i + 6], x[8 * i + 7]));
+}
+
+template <class C>
+__device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_t tmem, int warp, int lane) {
+    constexpr int BN = C::BN, D = C::D;
+    using Out = typename std::conditional<C::HL, float, __half>::type;
+    const int slot = C::NS == 2 ? warp >> 2 : 0;         // query tile of this warpgroup
+    const int row = (warp & 3) * 32 + lane;
+    const int tok_of = row / a.G, head_of = row % a.G;   // this row's token and head in its tile
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_col = lanes + C::kOCol + slot * D;
+    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
+    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float rise = kRescale / c2;
+    volatile int* abort = &B->abort;
+    uint32_t g = 0, piece = 0;
+    Walk<C> w(B);
+    while (w.next(a)) {
+        if (slot >= w.tiles(a)) continue;
+        const int tok = w.tok0(a) + slot * a.tq + tok_of;
+        const bool real = row < a.tq * a.G && tok < w.s.rows;
+        const bool busy = __any_sync(~0u, real);
+        const int own = w.s.kv - w.s.rows + tok;         // last slot this row sees
+        float m = -INFINITY, l = 0.0f;
+        for (int it = 0; it < w.n; ++it, ++g) {
+            const int buf = C::NS == 2 ? slot : (int)(g & 1);
+            const uint32_t par = C::NS == 2 ? g & 1 : (g >> 1) & 1;
+            if (!mbar_wait(smem_u32(&B->s_full[buf]), par, abort, a.c.err)) return;
+            tc_fence_after();
+            if (busy) {
+                const uint32_t s_col = lanes + C::kSCol + buf * BN;
+                float x[BN];
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i)
+                    tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
+                tmem_ld_wait();
+                if (a.softcap > 0.0f) {
+                    // cap * tanh(s scale / cap) = cap (1 - e) / (1 + e), e = exp(-2 |s| scale / cap)
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) {
+                        const float e = ex2(fabsf(x[i]) * cap_in);
+                        x[i] = copysignf(__fdividef(1.0f - e, 1.0f + e) * a.softcap, x[i]);
+                    }
+                }
+                const int limit = own - (w.tile + it) * BN;
+                if (__any_sync(~0u, limit < BN - 1)) {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) x[i] = i > limit ? -INFINITY : x[i];
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < BN; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (it == 0) {
+                    m = top;
+                } else if (__any_sync(~0u, top > m + rise)) {
+                    const float to = top > m + rise ? top : m;
+                    const float al = m == -INFINITY ? 0.0f : ex2((m - to) * c2);
+                    m = to;
+                    l *= al;
+                    // every product up to tile g - 1 is in O: with NS = 2 this S came after it, with
+                    // NS = 1 it came after that of tile g - 2
+                    if (C::NS == 1 && !mbar_wait(smem_u32(&B->o_step), (g - 1) & 1, abort, a.c.err)) return;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int i = 0; i < D; i += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_col + i, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
+                        tmem_st16(o_col + i, o);
+                    }
+                }
+                const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) {
+                    uint32_t hi[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float& p0 = x[i * 32 + 2 * j];
+                        float& p1 = x[i * 32 + 2 * j + 1];
+                        p0 = ex2(fmaf(p0, c2, off));
+                        p1 = ex2(fmaf(p1, c2, off));
+                        sum[j & 1] += p0;
+                        sum[2 + (j & 1)] += p1;
+                        hi[j] = ptx::pack_h2(p0, p1);
+                        if (C::HL) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
+                            p0 -= f.x;
+                            p1 -= f.y;
+                        }
+                    }
+                    tmem_st16(s_col + i * 16, hi);
+                    if (C::HL) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) hi[j] = ptx::pack_h2(x[i * 32 + 2 * j], x[i * 32 + 2 * j + 1]);
+                        tmem_st16(s_col + BN / 2 + i * 16, hi);
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&B->p_full[buf]));
+        }
+        // the piece's O
+        if (!mbar_wait(smem_u32(&B->o_done[slot]), piece & 1, abort, a.c.err)) return;
+        tc_fence_after();
+        const bool begins = w.tile == 0, ends = w.ends(a);
+        if (busy) {
+            const float e2 = m == -INFINITY ? -INFINITY : m * c2 - kPOffset;   // sum of 2^(...) = 2^e2 * l
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const int t = w.s.row0 + tok, h = w.h * a.G + head_of;
+            const size_t r = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * a.rec_rows + slot * 128 + row;
+            if (real) {
+                if (begins && ends) {
+                    if (a.lse)
+                        *reinterpret_cast<float*>(a.lse + (size_t)t * a.lse_tok + (size_t)h * a.lse_head) =
+                            l > 0.0f ? (e2 + log2f(l)) * kLn2 : -INFINITY;
+                } else {
+                    a.ml[r] = make_float2(e2, l);
+                }
+            }
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+                float o[32];
+                tmem_ld32(o_col + i, *reinterpret_cast<uint32_t(*)[32]>(o));
+                tmem_ld_wait();
+                if (!real) continue;
+                if (begins && ends) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] *= inv;
+                    put32(reinterpret_cast<Out*>(a.dst + (size_t)t * a.d_tok + (size_t)h * a.d_head) + i, o);
+                } else {
+                    put32(a.rec + r * D + i, o);
+                }
+            }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&B->o_empty[slot]));
+        ++piece;
+    }
+}
+
+// Slots of tile `i` that some row of the piece sees.
+template <class C>
+__device__ __forceinline__ int tile_rows(const AttnArgs& a, const Walk<C>& w, int i) {
+    return min(C::BN, max(0, visible<C::BN>(w.s, w.t, a.tq * C::NS) - i * C::BN));
+}
+
+template <class C>
+__device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t ring, int lane) {
+    volatile int* abort = &B->abort;
+    const int boxes = C::BN / a.box;          // <= 16
+    uint32_t at = 0;
+    bool ok = true;
+    // the page of box `lane` of slot tile i
+    auto page_of = [&](const Walk<C>& w, int i) {
+        const int j = i * C::BN + lane * a.box;
+        return lane < boxes && lane * a.box < tile_rows(a, w, i) ? paged::load_page(a.c, w.b, j / a.c.page) : -1;
+    };
+    auto load = [&](const Walk<C>& w, int i, int page, const CUtensorMap* map) {
+        const uint32_t st = at % C::ST;
+        if (!mbar_wait(smem_u32(&B->empty[st]), ((at / C::ST) & 1) ^ 1, abort, a.c.err)) return false;
+        const int n = (tile_rows(a, w, i) + a.box - 1) / a.box;
+        const uint32_t bar = smem_u32(&B->full[st]);
+        if (lane == 0) {
+            if (n) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
+            else mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (lane < n) {
+            const int j = i * C::BN + lane * a.box;
+            // a page outside the pools is a coordinate outside the map, which reads as zeros
+            const int pg = page < 0 ? a.c.n_pages : page;
+#pragma unroll
+            for (int u = 0; u < C::SUBS; ++u)
+                tma_load_4d(ring + st * C::kSlot + u * C::kSub + lane * a.box * 128, map, bar, u * 64, j % a.c.page, w.h, pg);
+        }
+        ++at;
+        return true;
+    };
+    Walk<C> w(B);
+    while (ok && w.next(a)) {
+        int cur = page_of(w, w.tile), nxt = -1;
+        ok = load(w, w.tile, cur, &a.mk);
+        for (int it = 0; ok && it < w.n; ++it) {
+            const int i = w.tile + it;
+            const bool more = it + 1 < w.n;
+            if (more) nxt = page_of(w, i + 1);
+            // the order in which the MMA warp takes them
+            if (C::NS == 1 && more) ok = load(w, i + 1, nxt, &a.mk);
+            if (ok) ok = load(w, i, cur, &a.mv);
+            if (C::NS == 2 && more && ok) ok = load(w, i + 1, nxt, &a.mk);
+            cur = nxt;
+        }
+    }
+    if (!ok) {
+        // the copies already issued land before this CTA's shared memory goes away
+        for (uint32_t j = at > (uint32_t)C::ST ? at - C::ST : 0; j < at; ++j) {
+            const uint64_t t0 = ptx::global_ns();
+            while (!ptx::mbar_try_wait(smem_u32(&B->full[j % C::ST]), (j / C::ST) & 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+            }
+        }
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, int lane) {
+    volatile int* abort = &B->abort;
+    uint32_t piece = 0;
+    bool ok = true;
+    Walk<C> w(B);
+    while (w.next(a)) {
+        if (!(ok = mbar_wait(smem_u32(&B->q_empty), (piece & 1) ^ 1, abort, a.c.err))) break;
+        const uint32_t bar = smem_u32(&B->q_full);
+        const int nt = w.tiles(a);
+        if constexpr (!C::HL) {
+            if (lane == 0) {
+                mbar_expect_tx(bar, (uint32_t)nt * a.tq * a.G * 128 * C::SUBS);
+                for (int i = 0; i < nt; ++i)
+#pragma unroll
+                    for (int u = 0; u < C::SUBS; ++u)
+                        tma_load_3d(qs + i * C::kQTile + u * C::kQSub, &a.mq, bar, u * 64, w.h * a.G, w.s.row0 + w.tok0(a) + i * a.tq);
+            }
+        } else {
+            constexpr int kCh = C::D / 8;     // 8 values: 32 bytes of q, 16 of each half
+            for (int i = 0; i < nt; ++i) {
+                const int t0 = w.tok0(a) + i * a.tq;
+                const int items = min(a.tq, w.s.rows - t0) * a.G * kCh;
+                const uint32_t base = qs + i * 2 * C::kQTile;
+#pragma unroll 4
+                for (int x = lane; x < items; x += 32) {
+                    const int r = x / kCh, ch = x % kCh;
+                    const char* p = a.q + (size_t)(w.s.row0 + t0 + r / a.G) * a.q_tok + (size_t)(w.h * a.G + r % a.G) * a.q_head + ch * 32;
+                    const float4 v0 = ptx::ld_act(reinterpret_cast<const float4*>(p));
+                    const float4 v1 = ptx::ld_act(reinterpret_cast<const float4*>(p + 16));
+                    uint4 hi, lo;
+                    ptx::split_h2(v0.x, v0.y, hi.x, lo.x);
+                    ptx::split_h2(v0.z, v0.w, hi.y, lo.y);
+                    ptx::split_h2(v1.x, v1.y, hi.z, lo.z);
+                    ptx::split_h2(v1.z, v1.w, hi.w, lo.w);
+                    const uint32_t to = base + (ch >> 3) * C::kQSub + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::kQTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        }
+        __syncwarp();
+        ++piece;
+    }
+    if (!C::HL && !ok && piece > 0 && lane == 0) {
+        const uint64_t t0 = ptx::global_ns();
+        while (!ptx::mbar_try_wait(smem_u32(&B->q_full), (piece - 1) & 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+        }
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs, uint32_t ring, uint32_t tmem, int lane) {
+    constexpr int BN = C::BN, D = C::D, NS = C::NS;
+    constexpr uint32_t idesc_s = umma_idesc_f16(128, BN);
+    constexpr uint32_t idesc_o = umma_idesc_f16(128, D) | kIdescBMnMajor;
+    volatile int* abort = &B->abort;
+    uint32_t at = 0, seg = 0, g[2] = {0, 0}, piece[2] = {0, 0};
+    uint32_t last_bar = 0, last_par = 0;     // of the latest commit to a ring barrier
+    // waits for the ring's next slot and takes it
+    auto take = [&](uint32_t& st) {
+        st = at % C::ST;
+        if (!mbar_wait(smem_u32(&B->full[st]), (at / C::ST) & 1, abort, a.c.err)) return false;
+        tc_fence_after();
+        ++at;
+        return true;
+    };
+    auto release = [&](uint32_t st, uint32_t index) {
+        if (lane == 0) umma_commit(smem_u32(&B->empty[st]));
+        last_bar = smem_u32(&B->empty[st]);
+        last_par = (index / C::ST) & 1;
+    };
+    auto scores = [&](int tile, int buf, uint32_t st) {
+        if (lane == 0) {
+            const uint64_t k = umma_desc_sw128(ring + st * C::kSlot);
+#pragma unroll
+            for (int half = 0; half < (C::HL ? 2 : 1); ++half) {
+                const uint64_t q = umma_desc_sw128(qs + (tile * (C::HL ? 2 : 1) + half) * C::kQTile);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    umma_f16(tmem + C::kSCol + buf * BN, q + (((i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
+                             k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s, half + i > 0 ? 1u : 0u);
+            }
+            umma_commit(smem_u32(&B->s_full[buf]));
+        }
+    };
+    auto values = [&](int tile, int buf, uint32_t st, bool add) {
+        if (lane == 0) {
+            const uint64_t v = umma_desc_mn_sw128(ring + st * C::kSlot, C::kSub);
+#pragma unroll
+            for (int half = 0; half < (C::HL ? 2 : 1); ++half)
+#pragma unroll
+                for (int i = 0; i < BN / 16; ++i)
+                    umma_f16_ta(tmem + C::kOCol + tile * D, tmem + C::kSCol + buf * BN + half * (BN / 2) + i * 8, v + ((i * 2048) >> 4),
+                                idesc_o, add || half + i > 0 ? 1u : 0u);
+        }
+    };
+    // V rows that no row of the piece sees may hold anything (a page's unused rows) or have not
+    // been copied: P is 0 there, and 0 * NaN would be NaN
+    auto blank = [&](const Walk<C>& w, int i, uint32_t st) {
+        const int n = tile_rows(a, w, i);
+        if (n == BN) return;
+        for (int x = n * 8 + lane; x < BN * 8; x += 32)
+#pragma unroll
+            for (int u = 0; u < C::SUBS; ++u)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * C::kSlot + u * C::kSub + x * 16), "r"(0) : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+    };
+    bool ok = true;
+    Walk<C> w(B);
+    while (ok && w.next(a)) {
+        const int nt = w.tiles(a);
+        uint32_t ks = 0, vs = 0;
+        ok = mbar_wait(smem_u32(&B->q_full), seg & 1, abort, a.c.err) && take(ks);
+        if (!ok) break;
+        ++seg;
+        tc_fence_after();
+        if constexpr (NS == 2) {
+            for (int i = 0; i < nt; ++i) scores(i, i, ks);
+        } else {
+            scores(0, g[0] & 1, ks);
+        }
+        release(ks, at - 1);
+        if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
+        for (int it = 0; ok && it < w.n; ++it) {
+            const bool more = it + 1 < w.n;
+            if constexpr (NS == 1) {
+                if (more) {
+                    if (!(ok = take(ks))) break;
+                    scores(0, (g[0] + 1) & 1, ks);
+                    release(ks, at - 1);
+                    if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
+                }
+            }
+            if (!(ok = take(vs))) break;
+            const uint32_t v_at = at - 1;
+            blank(w, w.tile + it, vs);
+            for (int i = 0; ok && i < nt; ++i) {
+                const int buf = NS == 2 ? i : (int)(g[0] & 1);
+                ok = mbar_wait(smem_u32(&B->p_full[buf]), NS == 2 ? g[i] & 1 : (g[0] >> 1) & 1, abort, a.c.err);
+                if (ok && it == 0) ok = mbar_wait(smem_u32(&B->o_empty[i]), (piece[i] & 1) ^ 1, abort, a.c.err);
+                if (!ok) break;
+                tc_fence_after();
+                values(i, buf, vs, it > 0);
+                if (NS == 1 && lane == 0) umma_commit(smem_u32(&B->o_step));
+                if (!more && lane == 0) umma_commit(smem_u32(&B->o_done[i]));
+                if constexpr (NS == 2) {
+                    if (more) {
+                        if (i == 0 && !(ok = take(ks))) break;
+                        scores(i, i, ks);
+                    }
+                }
+                ++g[i];
+            }
+            if (!ok) break;
+            release(vs, v_at);
+            if constexpr (NS == 2) {
+                if (more) {
+                    release(ks, at - 1);
+                    if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
+                }
+            }
+        }
+        for (int i = 0; i < nt; ++i) ++piece[i];
+    }
+    if (!ok && last_bar && lane == 0) {
+        // the products already issued end before TMEM is released
+        umma_commit(last_bar);
+        const uint64_t t0 = ptx::global_ns();
+        while (!ptx::mbar_try_wait(last_bar, last_par) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+        }
+    }
+}
+
+// Notes for the merge launch the query tile that begins in this CTA's share and ends in a later one.
+template <class C>
+__device__ __forceinline__ void head_role(const AttnArgs& a, Bars* B) {
+    int4 hd = make_int4(-1, 0, 0, 0);
+    long long at = B->first;
+    Walk<C> w(B);
+    while (w.next(a)) {
+        if (w.tile == 0 && !w.ends(a)) {
+            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of<C::BN>(w.s, w.t, a.tq * C::NS);
+            hd = make_int4(w.b, w.h, w.t, (int)((end * n - 1) / B->total));
+        }
+        at += w.n;
+    }
+    a.head[blockIdx.x] = hd;
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_constant__ AttnArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t qs = smem_u32(smem), ring = qs + C::kQBytes;
+    Bars* B = reinterpret_cast<Bars*>(smem + C::kQBytes + (size_t)C::ST * C::kSlot);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::ST; ++i) {
+            mbar_init(smem_u32(&B->full[i]), 1);
+            mbar_init(smem_u32(&B->empty[i]), 1);
+        }
+        mbar_init(smem_u32(&B->q_full), 1);
+        mbar_init(smem_u32(&B->q_empty), 1);
+        mbar_init(smem_u32(&B->o_step), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&B->s_full[i]), 1);
+            mbar_init(smem_u32(&B->p_full[i]), 4);
+            mbar_init(smem_u32(&B->o_done[i]), 1);
+            mbar_init(smem_u32(&B->o_empty[i]), 4);
+        }
+        B->abort = 0;
+        ptx::mbar_init_fence();
+        tma_prefetch_desc(&a.mk);
+        tma_prefetch_desc(&a.mv);
+        if (!C::HL) tma_prefetch_desc(&a.mq);
+    }
+    if (warp == C::kSoftWarps + 1) tmem_alloc(smem_u32(&B->tmem), 512);
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
-    const View& c = a.c;
-    const int lane = threadIdx.x & 31;
-    const int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int t = (int)(r / a.n_head_q), h = (int)(r % a.n_head_q);
-    if (t >= c.n_tokens) return;
-    int lo = 0, hi = c.batch;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (paged::ld_int(c.q_start + mid + 1) > t) hi = mid;
-        else lo = mid + 1;
+    plan<C>(a, B);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = B->tmem;
+    if (warp < C::kSoftWarps) softmax_role<C>(a, B, tmem, warp, lane);
+    else if (warp == C::kSoftWarps) load_role<C>(a, B, ring, lane);
+    else if (warp == C::kSoftWarps + 1) mma_role<C>(a, B, qs, ring, tmem, lane);
+    else if (warp == C::kSoftWarps + 2) q_role<C>(a, B, qs, lane);
+    else if (lane == 0) head_role<C>(a, B);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::kSoftWarps + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
     }
-    if (lo >= c.batch || paged::ld_int(c.q_start + lo) > t) return;
-    const Seq s = paged::load_seq(c, lo);
-    const int hk = h / (a.n_head_q / c.n_head_kv);
-    float q[E], o[E];
-    const char* qr = a.q + (size_t)t * a.q_tok + (size_t)h * a.q_head;
+}
+
+// Merges the records of each cut query tile: block (c, y) the tile begun by CTA c, 8 rows.
+constexpr int kMergeRows = 8;
+template <int D, typename Out>
+__global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_constant__ AttnArgs a, int tiles) {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    const int c = blockIdx.x, lane = threadIdx.x & 31;
+    const int hb = paged::ld_int(&a.head[c].x);
+    if (hb < 0) return;
+    const int h = paged::ld_int(&a.head[c].y), t = paged::ld_int(&a.head[c].z), last = paged::ld_int(&a.head[c].w);
+    const int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5);
+    const Seq s = paged::load_seq(a.c, hb);
+    const int in = row % 128, slot = row / 128;
+    const int tok = (t * tiles + slot) * a.tq + in / a.G;
+    if (row >= a.rec_rows || in >= a.tq * a.G || tok >= s.rows) return;
+    auto rec = [&](int i) { return ((size_t)i * 2 + (i == c ? 1 : 0)) * a.rec_rows + row; };
+    // lanes share the records' scales out, then every lane owns dims
+    float top = -INFINITY;
+    for (int i = c + lane; i <= last; i += 32) top = fmaxf(top, ptx::ld_act(&a.ml[rec(i)].x));
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        q[e] = a.f32 ? reinterpret_cast<const float*>(qr)[d] : __half2float(reinterpret_cast<const __half*>(qr)[d]);
-        o[e] = 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    const int seen = s.kv - s.rows + (t - s.row0) + 1;
-    for (int j = 0; j < seen; ++j) {
-        const int page = paged::load_page(c, lo, j / c.page);
-        const __half* kr = reinterpret_cast<const __half*>(c.k + (size_t)page * c.k_page + (size_t)hk * c.k_head + (size_t)(j % c.page) * c.k_row);
-        const __half* vr = reinterpret_cast<const __half*>(c.v + (size_t)page * c.v_page + (size_t)hk * c.v_head + (size_t)(j % c.page) * c.v_row);
-        float x = 0.0f;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    float l = 0.0f, acc[D / 32] = {};
+    if (top != -INFINITY) {
+#pragma unroll 4
+        for (int i = c; i <= last; ++i) {
+            const size_t r = rec(i);
+            const float f = ex2(ptx::ld_act(&a.ml[r].x) - top);
+            l += f * ptx::ld_act(&a.ml[r].y);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x += page < 0 ? 0.0f : q[e] * __half2float(kr[lane * E + e]);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-        x *= a.scale;
-        if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-        const float mn = fmaxf(m, x), al = expf(m - mn), p = expf(x - mn);
-        l = l * al + p;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * al + (page < 0 ? 0.0f : p * __half2float(vr[lane * E + e]));
-        m = mn;
+            for (int e = 0; e < D / 64; ++e) {
+                const uint2 v = ptx::ld_act(reinterpret_cast<const uint2*>(a.rec + r * D + e * 64 + lane * 2));
+                acc[2 * e] += f * __uint_as_float(v.x);
+                acc[2 * e + 1] += f * __uint_as_float(v.y);
+            }
+        }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    char* dr = a.dst + (size_t)t * a.d_tok + (size_t)h * a.d_head;
+    const int q = s.row0 + tok, head = h * a.G + in % a.G;
+    char* dst = a.dst + (size_t)q * a.d_tok + (size_t)head * a.d_head;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        if (a.f32) reinterpret_cast<float*>(dr)[d] = o[e] * inv;
-        else reinterpret_cast<__half*>(dr)[d] = __float2half_rn(o[e] * inv);
+    for (int e = 0; e < D / 64; ++e) {
+        if constexpr (sizeof(Out) == 4)
+            reinterpret_cast<float2*>(dst)[e * 32 + lane] = make_float2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        else
+            reinterpret_cast<uint32_t*>(dst)[e * 32 + lane] = ptx::pack_h2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
     }
     if (a.lse && lane == 0)
-        *reinterpret_cast<float*>(a.lse + (size_t)t * a.lse_tok + (size_t)h * a.lse_head) = l > 0.0f ? m + logf(l) : -INFINITY;
+        *reinterpret_cast<float*>(a.lse + (size_t)q * a.lse_tok + (size_t)head * a.lse_head) =
+            l > 0.0f ? (top + log2f(l)) * kLn2 : -INFINITY;
+}
+
+struct Plan {
+    int ns, bn, rec_rows;
+    size_t rec, ml, total;
+};
+
+Plan make_plan(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, int ctas) {
+    Plan p{};
+    const int64_t G = d->n_head_q / cache->n_head_kv, rows = cache->n_tokens * G;
+    // two query tiles a CTA when the sequences fill more than one on average
+    p.ns = cache->head_dim < 256 && rows > 128 * cache->batch_size ? 2 : 1;
+    p.bn = cache->head_dim == 256 ? 64 : 128;
+    p.rec_rows = (int)std::min<int64_t>(128 * p.ns, (rows + 3) / 4 * 4);
+    p.rec = (size_t)ctas * 2 * p.rec_rows * cache->head_dim * 4;
+    p.ml = (size_t)ctas * 2 * p.rec_rows * 8;
+    p.total = p.rec + p.ml + (size_t)ctas * 16;
+    return p;
+}
+
+template <class C>
+int launch(const AttnArgs& a, const DeviceCtx* c, cudaStream_t s) {
+    static bool set[64] = {};
+    const int dev = c->device < 64 ? c->device : 63;
+    if (!set[dev] || c->device >= 64) {
+        MLZC_CUDA_TRY(cudaFuncSetAttribute(attn_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+        set[dev] = true;
+    }
+    MLZC_CUDA_TRY(launch_pdl(attn_kernel<C>, dim3(a.n_ctas), dim3(C::kThreads), C::kSmem, s, a));
+    MLZC_CUDA_TRY(cudaGetLastError());
+    using Out = typename std::conditional<C::HL, float, __half>::type;
+    const dim3 g(a.n_ctas, (a.rec_rows + kMergeRows - 1) / kMergeRows);
+    MLZC_CUDA_TRY(launch_pdl(merge_kernel<C::D, Out>, g, dim3(kMergeRows * 32), 0, s, a, C::NS));
+    MLZC_CUDA_TRY(cudaGetLastError());
+    count_launch(2);
+    return MLZC_OK;
 }
 
 }  // namespace
@@ -94,7 +771,12 @@ extern "C" int mlzc_paged_attn_workspace_bytes(const mlzc_paged_cache* cache, co
                                                size_t* out_bytes) {
     if (!out_bytes) return fail(MLZC_ERR_INVALID, "paged attention: null out_bytes");
     *out_bytes = 0;
-    return paged::check_attn(cache, d, false);
+    const int st = paged::check_attn(cache, d, false);
+    if (st != MLZC_OK || cache->n_tokens == 0) return st;
+    DeviceCtx* c = current_ctx();
+    if (!c) return MLZC_ERR_CUDA;
+    *out_bytes = make_plan(cache, d, c->sm_count).total;
+    return MLZC_OK;
 }
 
 extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, void* workspace,
@@ -106,22 +788,38 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     AttnArgs a{};
     st = paged::make_view(cache, true, c, &a.c);
     if (st != MLZC_OK) return st;
+    const Plan p = make_plan(cache, d, c->sm_count);
+    if (!workspace || workspace_bytes < p.total)
+        return fail(MLZC_ERR_NOMEM, "paged attention: workspace of %zu bytes needed, %zu given", p.total, workspace_bytes);
+    if ((uintptr_t)workspace % 16) return fail(MLZC_ERR_INVALID, "paged attention: workspace not 16-byte aligned");
+    const bool f32 = d->type == MLZC_TYPE_F32;
+    a.G = (int)(d->n_head_q / cache->n_head_kv);
+    a.tq = 128 / a.G;
+    a.box = std::gcd(cache->page_size, p.bn);
+    if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
+    if ((st = paged::encode_pool(&a.mv, cache, true, a.box)) != MLZC_OK) return st;
+    if (!f32 && (st = paged::encode_rows(&a.mq, d->q, cache->head_dim, d->n_head_q, cache->n_tokens, d->q_nb[1], d->q_nb[2],
+                                         a.G, a.tq)) != MLZC_OK)
+        return st;
     a.q = static_cast<const char*>(d->q);
     a.dst = static_cast<char*>(d->dst);
     a.q_head = d->q_nb[1]; a.q_tok = d->q_nb[2];
     a.d_head = d->dst_nb[1]; a.d_tok = d->dst_nb[2];
     a.lse = reinterpret_cast<char*>(d->lse);
     a.lse_head = d->lse_nb[0]; a.lse_tok = d->lse_nb[1];
-    a.n_head_q = (int)d->n_head_q;
-    a.f32 = d->type == MLZC_TYPE_F32;
     a.scale = d->scale;
     a.softcap = (d->mode & MLZC_FA_MODE_SOFTCAP) ? d->logit_softcap : 0.0f;
-    const int64_t rows = cache->n_tokens * d->n_head_q;
-    const int D = (int)cache->head_dim;
-    MLZC_CUDA_TRY(launch_pdl(D == 64 ? attn_kernel<64> : (D == 128 ? attn_kernel<128> : attn_kernel<256>),
-                             dim3((unsigned)((rows + kWarps - 1) / kWarps)), dim3(kWarps * 32), 0,
-                             static_cast<cudaStream_t>(stream), a));
-    MLZC_CUDA_TRY(cudaGetLastError());
-    count_launch();
-    return MLZC_OK;
+    a.n_ctas = c->sm_count;
+    a.rec_rows = p.rec_rows;
+    a.rec = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.rec);
+    a.head = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.rec + p.ml);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch ((int)cache->head_dim * 10 + p.ns) {
+        case 641: return f32 ? launch<Cfg<64, 1, true>>(a, c, s) : launch<Cfg<64, 1, false>>(a, c, s);
+        case 642: return f32 ? launch<Cfg<64, 2, true>>(a, c, s) : launch<Cfg<64, 2, false>>(a, c, s);
+        case 1281: return f32 ? launch<Cfg<128, 1, true>>(a, c, s) : launch<Cfg<128, 1, false>>(a, c, s);
+        case 1282: return f32 ? launch<Cfg<128, 2, true>>(a, c, s) : launch<Cfg<128, 2, false>>(a, c, s);
+        default: return f32 ? launch<Cfg<256, 1, true>>(a, c, s) : launch<Cfg<256, 1, false>>(a, c, s);
+    }
 }

@@ -81,6 +81,37 @@ int make_view(const mlzc_paged_cache* cache, bool rows, const DeviceCtx* ctx, Vi
     return MLZC_OK;
 }
 
+namespace {
+int encode(CUtensorMap* map, const void* p, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return fail(MLZC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(p), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MLZC_ERR_UNSUPPORTED, "paged cache: strides not expressible as a tensor map (%d)", (int)r);
+    return MLZC_OK;
+}
+}  // namespace
+
+int encode_pool(CUtensorMap* map, const mlzc_paged_cache* c, bool v, int box_rows) {
+    const size_t* nb = v ? c->v_nb : c->k_nb;
+    const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->n_head_kv, (cuuint64_t)c->n_pages};
+    // the stride of a dimension of extent 1 is never stepped: any legal one
+    const cuuint64_t strides[3] = {nb[1], c->n_head_kv > 1 ? nb[2] : nb[1], c->n_pages > 1 ? nb[3] : nb[1]};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    return encode(map, v ? c->v : c->k, 4, dims, strides, box);
+}
+
+int encode_rows(CUtensorMap* map, const void* p, int64_t D, int64_t n_heads, int64_t n_tokens, size_t head_nb,
+                size_t token_nb, int heads, int tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)n_heads, (cuuint64_t)n_tokens};
+    const cuuint64_t row = (cuuint64_t)D * 2;
+    const cuuint64_t strides[2] = {n_heads > 1 ? (cuuint64_t)head_nb : row, n_tokens > 1 ? (cuuint64_t)token_nb : row};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens};
+    return encode(map, p, 3, dims, strides, box);
+}
+
 int check_attn(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, bool weights) {
     const int st = check_cache(cache, true);
     if (st != MLZC_OK) return st;
