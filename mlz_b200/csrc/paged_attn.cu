@@ -15,17 +15,20 @@
 //   Q warp         the next piece's Q tile (f16: TMA; f32: split into f16 hi + lo);
 //   MMA warp       S = Q K^T (operands in shared memory) and O += P V (P in TMEM, V as an
 //                  N-contiguous B operand) with tcgen05.mma, accumulators in TMEM;
-//   softmax warps  one thread a row: S from TMEM, P back over it.  O is rescaled only when
-//                  the maximum has risen by more than 8 in the exponent (P then stays below 2^8
-//                  times its offset), so in the steady state no thread touches O.
-// NS = 2: two query tiles with a softmax warpgroup each share every K and V tile, and the
-// tensor cores work on one while the other is in the softmax; for calls with more than 128
-// query rows a sequence.  NS = 1: one tile and two S buffers; for decode (the time is that of
-// reading K and V) and for head_dim 256 (whose O takes half of TMEM).
-//
+//   softmax warps  one thread a row: S from TMEM, P back over it.
+// f16 calls (P rounded to f16 once: P V then carries the rounding that the output's type has
+// anyway) keep O in TMEM; a softmax thread rescales it only when its row's maximum has risen by
+// more than 8 in the exponent (P then stays below 2^8 times its offset), so in the steady state
+// no thread touches O.  NS = 2: two query tiles with a softmax warpgroup each share every K and
+// V tile, and the tensor cores work on one while the other is in the softmax; for calls with
+// more than 128 query rows a sequence.  NS = 1: one tile and two S buffers; for decode (the time
+// is that of reading K and V) and for head_dim 256 (whose O takes half of TMEM).
 // f32 calls keep f32 precision: Q = Qhi + Qlo and P = Phi + Plo (f16 each, 22 bits), twice the
-// products, all summed in f32.  f16 calls round P to f16 once: P V then carries the rounding
-// that the output's type has anyway.
+// products.  The tensor cores' f32 sums drop what lies below an addend's last place, always
+// towards zero (measured: 1.4e-8 of the sum a step), so a long sum in TMEM drifts: over 2500
+// steps it is off by 4e-5.  Here O therefore sums one slot tile in TMEM, low products first, and
+// correction warps add the tiles up in registers, rounding to nearest.  Tiles are independent
+// of one another (each has its own maximum and sum), so the softmax keeps no state.
 //
 // All (sequence, KV head, query tile, slot tile) of a call form one list, of which every CTA
 // takes an equal contiguous share (few rows over a long cache and many rows over a short one
@@ -50,9 +53,26 @@ using paged::View;
 using ptx::mbar_arrive;
 using ptx::mbar_expect_tx;
 using ptx::mbar_init;
-using ptx::mbar_wait;
 using ptx::smem_u32;
 using namespace tc05;
+
+// Bounded wait as ptx::mbar_wait, all inline: kernels that move registers between warpgroups
+// cannot call functions.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* err) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = ptx::global_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((i & 31) == 0) {
+            if (*abort) return false;
+            if (ptx::global_ns() - t0 > ptx::kWaitNs) {
+                atomicOr(err, MLZC_DEVERR_WAIT_TIMEOUT);
+                *abort = 1;
+                return false;
+            }
+        }
+    }
+}
 
 constexpr int kSmemMax = 232448;
 constexpr int kBarBytes = 512;
@@ -79,49 +99,60 @@ struct AttnArgs {
     int4* head;                // [cta]: sequence (-1: none), kv head, query tile, last CTA of the tile begun in record 1
 };
 
+constexpr int BN = 128;        // slots a tile
+
 template <int D_, int NS_, bool HL_>
 struct Cfg {
     static constexpr int D = D_, NS = NS_;
     static constexpr bool HL = HL_;
-    static constexpr int BN = D == 256 ? 64 : 128;
-    static constexpr int SUBS = D / 64;
+    // dims of a ring unit (a K or V tile is UN units); beside f32 queries of 256 dims (128 KB)
+    // half units leave a ring of five
+    static constexpr int DU = D == 64 || (HL && D == 256) ? 64 : 128;
+    static constexpr int UN = D / DU;
+    static constexpr int SUBS = DU / 64;
     static constexpr uint32_t kQSub = 128 * 128;          // bytes of a 64-value block of a Q tile
-    static constexpr uint32_t kQTile = kQSub * SUBS;
+    static constexpr uint32_t kQTile = kQSub * (D / 64);
     static constexpr uint32_t kQBytes = kQTile * NS * (HL ? 2 : 1);   // [tile][hi, lo]
-    static constexpr uint32_t kSub = BN * 128;            // bytes of a 64-value block of a K / V tile
-    static constexpr uint32_t kSlot = kSub * SUBS;
-    static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - (int)kQBytes) / (int)kSlot;
+    static constexpr uint32_t kSub = BN * 128;            // bytes of a 64-value block of a unit
+    static constexpr uint32_t kUnit = kSub * SUBS;
+    static constexpr uint32_t kStats = HL ? 4 * 128 * 8 : 0;
+    static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - (int)kStats - (int)kQBytes) / (int)kUnit;
     static constexpr int ST = kFit > 8 ? 8 : kFit;
-    static constexpr size_t kSmem = 1024 + kBarBytes + kQBytes + (size_t)ST * kSlot;
-    static constexpr int kSoftWarps = 4 * NS;
-    static constexpr int kThreads = (kSoftWarps + 4) * 32;
+    static constexpr size_t kSmem = 1024 + kBarBytes + kStats + kQBytes + (size_t)ST * kUnit;
+    // warps: softmax (f32 calls of 64 dims are bound by the exponentials: two warpgroups take
+    // turns at the tiles), correction (f32; 128 dims a thread at most), then the four of the
+    // other roles
+    static constexpr int kSoftWarps = 4 * (HL ? (D == 64 ? 2 : 1) : NS);
+    static constexpr int CD = D < 128 ? D : 128;          // dims of a correction thread
+    static constexpr int kCorrWarps = HL ? 4 * (D / CD) : 0;
+    static constexpr int kMisc = kSoftWarps + kCorrWarps;
+    static constexpr int kThreads = (kMisc + 4) * 32;
     static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
     static constexpr uint32_t kOCol = 2 * BN;             // O of tile i at + i * D
     static_assert(2 * BN + NS * D <= 512, "TMEM");
     static_assert(ST >= 3, "ring");
+    static_assert(!HL || NS == 1, "f32 calls take one query tile");
 };
 
 // Barriers in shared memory.
 struct Bars {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_step, o_done[2], o_empty[2];
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_step, o_done[2], o_empty[2], stat_full[4];
     uint32_t tmem;
     int abort;
     long long first, count, total;   // this CTA's share of the list; its start's place
     int b, h, t, tile;
-    long long scan[12];
+    long long scan[16];
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 
 // Slots that query tile t of a sequence sees, and its slot tiles (one at least, so that rows
 // which see nothing are written too).
-template <int BN>
 __device__ __forceinline__ int visible(const Seq& s, int t, int tokens) {
     const int64_t e = (int64_t)(t + 1) * tokens;
     return max(0, s.kv - s.rows + (int)(e < s.rows ? e : s.rows));
 }
-template <int BN>
 __device__ __forceinline__ int tiles_of(const Seq& s, int t, int tokens) {
-    return max(1, (visible<BN>(s, t, tokens) + BN - 1) / BN);
+    return max(1, (visible(s, t, tokens) + BN - 1) / BN);
 }
 
 // A walk over this CTA's share: piece after piece (the tiles of one query tile).
@@ -151,14 +182,14 @@ struct Walk {
                 }
             }
         }
-        const int all = tiles_of<C::BN>(s, t, tokens) - tile;
+        const int all = tiles_of(s, t, tokens) - tile;
         n = (int)min((long long)all, left);
         left -= n;
         return true;
     }
     __device__ int tok0(const AttnArgs& a) const { return t * a.tq * C::NS; }
     __device__ int tiles(const AttnArgs& a) const { return C::NS == 2 && tok0(a) + a.tq < s.rows ? 2 : 1; }
-    __device__ bool ends(const AttnArgs& a) const { return tile + n == tiles_of<C::BN>(s, t, a.tq * C::NS); }
+    __device__ bool ends(const AttnArgs& a) const { return tile + n == tiles_of(s, t, a.tq * C::NS); }
 };
 
 // Finds this CTA's share.  Threads own runs of sequences: their tile counts are summed over the
@@ -173,7 +204,7 @@ __device__ void plan(const AttnArgs& a, Bars* B) {
     for (int b = b0; b < b1; ++b) {
         const Seq s = paged::load_seq(a.c, b);
         long long one = 0;
-        for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of<C::BN>(s, t, tokens);
+        for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens);
         mine += one * a.c.n_head_kv;
     }
     long long upto = mine;
@@ -197,13 +228,13 @@ __device__ void plan(const AttnArgs& a, Bars* B) {
         for (int b = b0; b < b1; ++b) {
             const Seq s = paged::load_seq(a.c, b);
             long long one = 0;
-            for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of<C::BN>(s, t, tokens);
+            for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens);
             if (r >= one * a.c.n_head_kv) { r -= one * a.c.n_head_kv; continue; }
             B->b = b;
             B->h = (int)(r / one);
             r %= one;
             int t = 0;
-            while (r >= tiles_of<C::BN>(s, t, tokens)) r -= tiles_of<C::BN>(s, t++, tokens);
+            while (r >= tiles_of(s, t, tokens)) r -= tiles_of(s, t++, tokens);
             B->t = t;
             B->tile = (int)r;
             break;
@@ -224,13 +255,61 @@ __device__ __forceinline__ void put32(__half* p, const float (&x)[32]) {
                                                     ptx::pack_h2(x[8 * i + 4], x[8 * i + 5]), ptx::pack_h2(x[8 * i + 6], x[8 * i + 7]));
 }
 
+// A query row's place: thread `row` of a query tile.
+struct Row {
+    int row, tok_of, head_of;            // token and head in the tile
+    __device__ Row(const AttnArgs& a, int r) : row(r), tok_of(r / a.G), head_of(r % a.G) {}
+    template <class C>
+    __device__ int tok(const AttnArgs& a, const Walk<C>& w, int slot) const { return w.tok0(a) + slot * a.tq + tok_of; }
+    template <class C>
+    __device__ bool real(const AttnArgs& a, const Walk<C>& w, int slot) const {
+        return row < a.tq * a.G && tok(a, w, slot) < w.s.rows;
+    }
+};
+
+// cap * tanh(s scale / cap) = cap (1 - e) / (1 + e), e = exp(-2 |s| scale / cap) = 2^(|s| cap_in).
+__device__ __forceinline__ float capped(float s, float cap_in, float cap) {
+    const float e = ex2(fabsf(s) * cap_in);
+    return copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, s);
+}
+
+// Where a piece's rows go: dst and lse when it is the whole query tile, else a record.
+template <class C>
+struct Sink {
+    bool whole;
+    int t, h;
+    size_t r;
+    __device__ Sink(const AttnArgs& a, const Walk<C>& w, const Row& q, int slot) {
+        whole = w.tile == 0 && w.ends(a);
+        t = w.s.row0 + q.tok(a, w, slot);
+        h = w.h * a.G + q.head_of;
+        r = ((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * a.rec_rows + slot * 128 + q.row;
+    }
+    // the row's sum: of 2^(...) = 2^e2 * l
+    __device__ void sums(const AttnArgs& a, float e2, float l) const {
+        if (!whole)
+            a.ml[r] = make_float2(e2, l);
+        else if (a.lse)
+            *reinterpret_cast<float*>(a.lse + (size_t)t * a.lse_tok + (size_t)h * a.lse_head) = l > 0.0f ? (e2 + log2f(l)) * kLn2 : -INFINITY;
+    }
+    // dims i .. i + 31 of O
+    __device__ void put(const AttnArgs& a, int i, float (&o)[32], float inv) const {
+        using Out = typename std::conditional<C::HL, float, __half>::type;
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] *= inv;
+            put32(reinterpret_cast<Out*>(a.dst + (size_t)t * a.d_tok + (size_t)h * a.d_head) + i, o);
+        } else {
+            put32(a.rec + r * C::D + i, o);
+        }
+    }
+};
+
 template <class C>
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_t tmem, int warp, int lane) {
-    constexpr int BN = C::BN, D = C::D;
-    using Out = typename std::conditional<C::HL, float, __half>::type;
+    constexpr int D = C::D;
     const int slot = C::NS == 2 ? warp >> 2 : 0;         // query tile of this warpgroup
-    const int row = (warp & 3) * 32 + lane;
-    const int tok_of = row / a.G, head_of = row % a.G;   // this row's token and head in its tile
+    const Row q(a, (warp & 3) * 32 + lane);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t o_col = lanes + C::kOCol + slot * D;
     const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
@@ -241,10 +320,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
     Walk<C> w(B);
     while (w.next(a)) {
         if (slot >= w.tiles(a)) continue;
-        const int tok = w.tok0(a) + slot * a.tq + tok_of;
-        const bool real = row < a.tq * a.G && tok < w.s.rows;
-        const bool busy = __any_sync(~0u, real);
-        const int own = w.s.kv - w.s.rows + tok;         // last slot this row sees
+        const bool real = q.real(a, w, slot), busy = __any_sync(~0u, real);
+        const int own = w.s.kv - w.s.rows + q.tok(a, w, slot);   // last slot this row sees
         float m = -INFINITY, l = 0.0f;
         for (int it = 0; it < w.n; ++it, ++g) {
             const int buf = C::NS == 2 ? slot : (int)(g & 1);
@@ -259,12 +336,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                     tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                 tmem_ld_wait();
                 if (a.softcap > 0.0f) {
-                    // cap * tanh(s scale / cap) = cap (1 - e) / (1 + e), e = exp(-2 |s| scale / cap)
 #pragma unroll
-                    for (int i = 0; i < BN; ++i) {
-                        const float e = ex2(fabsf(x[i]) * cap_in);
-                        x[i] = copysignf(__fdividef(1.0f - e, 1.0f + e) * a.softcap, x[i]);
-                    }
+                    for (int i = 0; i < BN; ++i) x[i] = capped(x[i], cap_in, a.softcap);
                 }
                 const int limit = own - (w.tile + it) * BN;
                 if (__any_sync(~0u, limit < BN - 1)) {
@@ -303,25 +376,13 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                     uint32_t hi[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        float& p0 = x[i * 32 + 2 * j];
-                        float& p1 = x[i * 32 + 2 * j + 1];
-                        p0 = ex2(fmaf(p0, c2, off));
-                        p1 = ex2(fmaf(p1, c2, off));
+                        const float p0 = ex2(fmaf(x[i * 32 + 2 * j], c2, off));
+                        const float p1 = ex2(fmaf(x[i * 32 + 2 * j + 1], c2, off));
                         sum[j & 1] += p0;
                         sum[2 + (j & 1)] += p1;
                         hi[j] = ptx::pack_h2(p0, p1);
-                        if (C::HL) {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
-                            p0 -= f.x;
-                            p1 -= f.y;
-                        }
                     }
-                    tmem_st16(s_col + i * 16, hi);
-                    if (C::HL) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) hi[j] = ptx::pack_h2(x[i * 32 + 2 * j], x[i * 32 + 2 * j + 1]);
-                        tmem_st16(s_col + BN / 2 + i * 16, hi);
-                    }
+                    tmem_st16(s_col + i * 32, hi);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_st_wait();
@@ -333,34 +394,16 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
         // the piece's O
         if (!mbar_wait(smem_u32(&B->o_done[slot]), piece & 1, abort, a.c.err)) return;
         tc_fence_after();
-        const bool begins = w.tile == 0, ends = w.ends(a);
         if (busy) {
-            const float e2 = m == -INFINITY ? -INFINITY : m * c2 - kPOffset;   // sum of 2^(...) = 2^e2 * l
+            const Sink<C> sink(a, w, q, slot);
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const int t = w.s.row0 + tok, h = w.h * a.G + head_of;
-            const size_t r = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * a.rec_rows + slot * 128 + row;
-            if (real) {
-                if (begins && ends) {
-                    if (a.lse)
-                        *reinterpret_cast<float*>(a.lse + (size_t)t * a.lse_tok + (size_t)h * a.lse_head) =
-                            l > 0.0f ? (e2 + log2f(l)) * kLn2 : -INFINITY;
-                } else {
-                    a.ml[r] = make_float2(e2, l);
-                }
-            }
+            if (real) sink.sums(a, m == -INFINITY ? -INFINITY : m * c2 - kPOffset, l);
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 float o[32];
                 tmem_ld32(o_col + i, *reinterpret_cast<uint32_t(*)[32]>(o));
                 tmem_ld_wait();
-                if (!real) continue;
-                if (begins && ends) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] *= inv;
-                    put32(reinterpret_cast<Out*>(a.dst + (size_t)t * a.d_tok + (size_t)h * a.d_head) + i, o);
-                } else {
-                    put32(a.rec + r * D + i, o);
-                }
+                if (real) sink.put(a, i, o, inv);
             }
         }
         tc_fence_before();
@@ -370,42 +413,180 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
     }
 }
 
+// Softmax of an f32 call: a tile's rows by themselves.  Phi of 32 slots goes to the first 16
+// columns of their scores, Plo to the other 16; (exponent of the row's scale, sum) to stats.
+template <class C>
+__device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, float2* stats, uint32_t tmem, int warp, int lane) {
+    constexpr int kTurns = C::kSoftWarps / 4;
+    const int turn = warp >> 2;
+    const Row q(a, (warp & 3) * 32 + lane);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
+    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    volatile int* abort = &B->abort;
+    uint32_t g = 0;
+    Walk<C> w(B);
+    while (w.next(a)) {
+        const bool busy = __any_sync(~0u, q.real(a, w, 0));
+        const int own = w.s.kv - w.s.rows + q.tok(a, w, 0);
+        for (int it = 0; it < w.n; ++it, ++g) {
+            if (kTurns == 2 && (int)(g & 1) != turn) continue;
+            const int buf = g & 1;
+            if (!mbar_wait(smem_u32(&B->s_full[buf]), (g >> 1) & 1, abort, a.c.err)) return;
+            tc_fence_after();
+            if (busy) {
+                const uint32_t s_col = lanes + C::kSCol + buf * BN;
+                const int limit = own - (w.tile + it) * BN;
+                const bool cut = __any_sync(~0u, limit < BN - 1);
+                float m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < BN; i += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(s_col + i, r);
+                    tmem_ld_wait();
+                    if (a.softcap > 0.0f || cut) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float x = __uint_as_float(r[j]);
+                            if (a.softcap > 0.0f) x = capped(x, cap_in, a.softcap);
+                            r[j] = __float_as_uint(i + j > limit ? -INFINITY : x);
+                        }
+                        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));
+                        tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(r + 16));
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(r[j]));
+                    m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                }
+                tmem_st_wait();
+                const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < BN; i += 32) {
+                    uint32_t r[32], hi[16], lo[16];
+                    tmem_ld32(s_col + i, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float p0 = ex2(fmaf(__uint_as_float(r[2 * j]), c2, off));
+                        const float p1 = ex2(fmaf(__uint_as_float(r[2 * j + 1]), c2, off));
+                        sum[j & 1] += p0;
+                        sum[2 + (j & 1)] += p1;
+                        ptx::split_h2(p0, p1, hi[j], lo[j]);
+                    }
+                    tmem_st16(s_col + i, hi);
+                    tmem_st16(s_col + i + 16, lo);
+                }
+                stats[(g & 3) * 128 + q.row] =
+                    make_float2(m == -INFINITY ? -INFINITY : m * c2 - kPOffset, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&B->p_full[buf]));
+                mbar_arrive(smem_u32(&B->stat_full[g & 3]));
+            }
+        }
+    }
+}
+
+// Adds up the tiles of an f32 call: O += 2^(e - E) O_tile, rounded to nearest, with E the
+// largest exponent so far (raised, and O rescaled, when a tile's lies more than 8 above it).
+// stats has four places: the softmax fills that of tile g + 4 only after tile g + 1 was read.
+template <class C>
+__device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, const float2* stats, uint32_t tmem, int warp, int lane) {
+    constexpr int CD = C::CD;
+    const int part = (warp - C::kSoftWarps) >> 2;        // dims [part * CD, + CD)
+    const Row q(a, (warp & 3) * 32 + lane);
+    const uint32_t o_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::kOCol + part * CD;
+    volatile int* abort = &B->abort;
+    uint32_t g = 0;
+    Walk<C> w(B);
+    while (w.next(a)) {
+        const bool real = q.real(a, w, 0), busy = __any_sync(~0u, real);
+        float o[CD], e = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CD; ++i) o[i] = 0.0f;
+        for (int it = 0; it < w.n; ++it, ++g) {
+            if (!mbar_wait(smem_u32(&B->stat_full[g & 3]), (g >> 2) & 1, abort, a.c.err)) return;
+            float2 st = make_float2(-INFINITY, 0.0f);
+            if (busy) st = stats[(g & 3) * 128 + q.row];
+            if (!mbar_wait(smem_u32(&B->o_done[0]), g & 1, abort, a.c.err)) return;
+            tc_fence_after();
+            if (busy) {
+                if (__any_sync(~0u, st.x > e + kRescale)) {
+                    const float to = st.x > e + kRescale ? st.x : e;
+                    const float f = e == -INFINITY ? 0.0f : ex2(e - to);
+                    e = to;
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < CD; ++i) o[i] *= f;
+                }
+                const float f = st.x == -INFINITY ? 0.0f : ex2(st.x - e);
+                l = fmaf(st.y, f, l);
+#pragma unroll
+                for (int i = 0; i < CD; i += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(o_col + i, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(__uint_as_float(r[j]), f, o[i + j]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&B->o_empty[0]));
+        }
+        if (real) {
+            const Sink<C> sink(a, w, q, 0);
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            if (part == 0) sink.sums(a, e, l);
+#pragma unroll
+            for (int i = 0; i < CD; i += 32) sink.put(a, part * CD + i, *reinterpret_cast<float(*)[32]>(o + i), inv);
+        }
+    }
+}
+
 // Slots of tile `i` that some row of the piece sees.
 template <class C>
 __device__ __forceinline__ int tile_rows(const AttnArgs& a, const Walk<C>& w, int i) {
-    return min(C::BN, max(0, visible<C::BN>(w.s, w.t, a.tq * C::NS) - i * C::BN));
+    return min(BN, max(0, visible(w.s, w.t, a.tq * C::NS) - i * BN));
 }
 
 template <class C>
 __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t ring, int lane) {
     volatile int* abort = &B->abort;
-    const int boxes = C::BN / a.box;          // <= 16
+    const int boxes = BN / a.box;             // <= 16
     uint32_t at = 0;
     bool ok = true;
     // the page of box `lane` of slot tile i
     auto page_of = [&](const Walk<C>& w, int i) {
-        const int j = i * C::BN + lane * a.box;
+        const int j = i * BN + lane * a.box;
         return lane < boxes && lane * a.box < tile_rows(a, w, i) ? paged::load_page(a.c, w.b, j / a.c.page) : -1;
     };
     auto load = [&](const Walk<C>& w, int i, int page, const CUtensorMap* map) {
-        const uint32_t st = at % C::ST;
-        if (!mbar_wait(smem_u32(&B->empty[st]), ((at / C::ST) & 1) ^ 1, abort, a.c.err)) return false;
         const int n = (tile_rows(a, w, i) + a.box - 1) / a.box;
-        const uint32_t bar = smem_u32(&B->full[st]);
-        if (lane == 0) {
-            if (n) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
-            else mbar_arrive(bar);
-        }
-        __syncwarp();
-        if (lane < n) {
-            const int j = i * C::BN + lane * a.box;
-            // a page outside the pools is a coordinate outside the map, which reads as zeros
-            const int pg = page < 0 ? a.c.n_pages : page;
+        const int row = (i * BN + lane * a.box) % a.c.page;
+        // a page outside the pools is a coordinate outside the map, which reads as zeros
+        const int pg = page < 0 ? a.c.n_pages : page;
 #pragma unroll
-            for (int u = 0; u < C::SUBS; ++u)
-                tma_load_4d(ring + st * C::kSlot + u * C::kSub + lane * a.box * 128, map, bar, u * 64, j % a.c.page, w.h, pg);
+        for (int unit = 0; unit < C::UN; ++unit, ++at) {
+            const uint32_t st = at % C::ST;
+            if (!mbar_wait(smem_u32(&B->empty[st]), ((at / C::ST) & 1) ^ 1, abort, a.c.err)) return false;
+            const uint32_t bar = smem_u32(&B->full[st]);
+            if (lane == 0) {
+                if (n) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            if (lane < n) {
+#pragma unroll
+                for (int u = 0; u < C::SUBS; ++u)
+                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, map, bar, (unit * C::SUBS + u) * 64, row, w.h, pg);
+            }
         }
-        ++at;
         return true;
     };
     Walk<C> w(B);
@@ -445,10 +626,10 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
         const int nt = w.tiles(a);
         if constexpr (!C::HL) {
             if (lane == 0) {
-                mbar_expect_tx(bar, (uint32_t)nt * a.tq * a.G * 128 * C::SUBS);
+                mbar_expect_tx(bar, (uint32_t)nt * a.tq * a.G * 128 * (C::D / 64));
                 for (int i = 0; i < nt; ++i)
 #pragma unroll
-                    for (int u = 0; u < C::SUBS; ++u)
+                    for (int u = 0; u < (C::D / 64); ++u)
                         tma_load_3d(qs + i * C::kQTile + u * C::kQSub, &a.mq, bar, u * 64, w.h * a.G, w.s.row0 + w.tok0(a) + i * a.tq);
             }
         } else {
@@ -489,13 +670,13 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
 
 template <class C>
 __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs, uint32_t ring, uint32_t tmem, int lane) {
-    constexpr int BN = C::BN, D = C::D, NS = C::NS;
+    constexpr int NS = C::NS, DU = C::DU;
     constexpr uint32_t idesc_s = umma_idesc_f16(128, BN);
-    constexpr uint32_t idesc_o = umma_idesc_f16(128, D) | kIdescBMnMajor;
+    constexpr uint32_t idesc_o = umma_idesc_f16(128, DU) | kIdescBMnMajor;
     volatile int* abort = &B->abort;
     uint32_t at = 0, seg = 0, g[2] = {0, 0}, piece[2] = {0, 0};
     uint32_t last_bar = 0, last_par = 0;     // of the latest commit to a ring barrier
-    // waits for the ring's next slot and takes it
+    // waits for the ring's next unit and takes it
     auto take = [&](uint32_t& st) {
         st = at % C::ST;
         if (!mbar_wait(smem_u32(&B->full[st]), (at / C::ST) & 1, abort, a.c.err)) return false;
@@ -503,34 +684,35 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
         ++at;
         return true;
     };
+    // frees unit `st`, the ring's `index`-th, when the products issued so far are done
     auto release = [&](uint32_t st, uint32_t index) {
         if (lane == 0) umma_commit(smem_u32(&B->empty[st]));
         last_bar = smem_u32(&B->empty[st]);
         last_par = (index / C::ST) & 1;
     };
-    auto scores = [&](int tile, int buf, uint32_t st) {
+    auto scores = [&](int tile, int buf, int unit, uint32_t st) {
         if (lane == 0) {
-            const uint64_t k = umma_desc_sw128(ring + st * C::kSlot);
+            const uint64_t k = umma_desc_sw128(ring + st * C::kUnit);
 #pragma unroll
-            for (int half = 0; half < (C::HL ? 2 : 1); ++half) {
-                const uint64_t q = umma_desc_sw128(qs + (tile * (C::HL ? 2 : 1) + half) * C::kQTile);
+            for (int part = C::HL ? 1 : 0; part >= 0; --part) {      // lo, then hi
+                const uint64_t q = umma_desc_sw128(qs + (tile * (C::HL ? 2 : 1) + part) * C::kQTile + unit * C::SUBS * C::kQSub);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                for (int i = 0; i < DU / 16; ++i)
                     umma_f16(tmem + C::kSCol + buf * BN, q + (((i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
-                             k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s, half + i > 0 ? 1u : 0u);
+                             k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s,
+                             unit > 0 || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
             }
-            umma_commit(smem_u32(&B->s_full[buf]));
         }
     };
-    auto values = [&](int tile, int buf, uint32_t st, bool add) {
+    auto values = [&](int tile, int buf, int unit, uint32_t st, bool add) {
         if (lane == 0) {
-            const uint64_t v = umma_desc_mn_sw128(ring + st * C::kSlot, C::kSub);
+            const uint64_t v = umma_desc_mn_sw128(ring + st * C::kUnit, C::kSub);
 #pragma unroll
-            for (int half = 0; half < (C::HL ? 2 : 1); ++half)
+            for (int part = C::HL ? 1 : 0; part >= 0; --part)
 #pragma unroll
                 for (int i = 0; i < BN / 16; ++i)
-                    umma_f16_ta(tmem + C::kOCol + tile * D, tmem + C::kSCol + buf * BN + half * (BN / 2) + i * 8, v + ((i * 2048) >> 4),
-                                idesc_o, add || half + i > 0 ? 1u : 0u);
+                    umma_f16_ta(tmem + C::kOCol + tile * C::D + unit * DU, tmem + C::kSCol + buf * BN + (i >> 1) * 32 + (i & 1) * 8 + part * 16,
+                                v + ((i * 2048) >> 4), idesc_o, add || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
         }
     };
     // V rows that no row of the piece sees may hold anything (a page's unused rows) or have not
@@ -541,59 +723,86 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
         for (int x = n * 8 + lane; x < BN * 8; x += 32)
 #pragma unroll
             for (int u = 0; u < C::SUBS; ++u)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * C::kSlot + u * C::kSub + x * 16), "r"(0) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * C::kUnit + u * C::kSub + x * 16), "r"(0) : "memory");
         fence_proxy_async_smem();
         __syncwarp();
+    };
+    // S of one query tile (NS = 1): all units of K
+    auto scores_all = [&](int buf) {
+        for (int unit = 0; unit < C::UN; ++unit) {
+            uint32_t st;
+            if (!take(st)) return false;
+            scores(0, buf, unit, st);
+            release(st, at - 1);
+        }
+        if (lane == 0) umma_commit(smem_u32(&B->s_full[buf]));
+        return true;
     };
     bool ok = true;
     Walk<C> w(B);
     while (ok && w.next(a)) {
         const int nt = w.tiles(a);
-        uint32_t ks = 0, vs = 0;
-        ok = mbar_wait(smem_u32(&B->q_full), seg & 1, abort, a.c.err) && take(ks);
+        ok = mbar_wait(smem_u32(&B->q_full), seg & 1, abort, a.c.err);
         if (!ok) break;
         ++seg;
         tc_fence_after();
-        if constexpr (NS == 2) {
-            for (int i = 0; i < nt; ++i) scores(i, i, ks);
-        } else {
-            scores(0, g[0] & 1, ks);
-        }
-        release(ks, at - 1);
-        if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
-        for (int it = 0; ok && it < w.n; ++it) {
-            const bool more = it + 1 < w.n;
-            if constexpr (NS == 1) {
-                if (more) {
-                    if (!(ok = take(ks))) break;
-                    scores(0, (g[0] + 1) & 1, ks);
-                    release(ks, at - 1);
+        if constexpr (NS == 1) {
+            if (!(ok = scores_all(g[0] & 1))) break;
+            if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
+            for (int it = 0; it < w.n; ++it, ++g[0]) {
+                const int buf = g[0] & 1;
+                if (it + 1 < w.n) {
+                    if (!(ok = scores_all(buf ^ 1))) break;
                     if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
                 }
-            }
-            if (!(ok = take(vs))) break;
-            const uint32_t v_at = at - 1;
-            blank(w, w.tile + it, vs);
-            for (int i = 0; ok && i < nt; ++i) {
-                const int buf = NS == 2 ? i : (int)(g[0] & 1);
-                ok = mbar_wait(smem_u32(&B->p_full[buf]), NS == 2 ? g[i] & 1 : (g[0] >> 1) & 1, abort, a.c.err);
-                if (ok && it == 0) ok = mbar_wait(smem_u32(&B->o_empty[i]), (piece[i] & 1) ^ 1, abort, a.c.err);
+                ok = mbar_wait(smem_u32(&B->p_full[buf]), (g[0] >> 1) & 1, abort, a.c.err);
+                // O free: f32 calls empty it tile by tile, the others piece by piece
+                const uint32_t turn = C::HL ? g[0] : piece[0];
+                if (ok && (C::HL || it == 0)) ok = mbar_wait(smem_u32(&B->o_empty[0]), (turn & 1) ^ 1, abort, a.c.err);
+                for (int unit = 0; ok && unit < C::UN; ++unit) {
+                    uint32_t st;
+                    if (!(ok = take(st))) break;
+                    blank(w, w.tile + it, st);
+                    tc_fence_after();
+                    values(0, buf, unit, st, !C::HL && it > 0);
+                    release(st, at - 1);
+                }
                 if (!ok) break;
-                tc_fence_after();
-                values(i, buf, vs, it > 0);
-                if (NS == 1 && lane == 0) umma_commit(smem_u32(&B->o_step));
-                if (!more && lane == 0) umma_commit(smem_u32(&B->o_done[i]));
-                if constexpr (NS == 2) {
+                if (lane == 0) {
+                    if (C::HL || it + 1 == w.n) umma_commit(smem_u32(&B->o_done[0]));
+                    if (!C::HL) umma_commit(smem_u32(&B->o_step));
+                }
+            }
+        } else {
+            uint32_t ks = 0, vs = 0;
+            if (!(ok = take(ks))) break;
+            for (int i = 0; i < nt; ++i) {
+                scores(i, i, 0, ks);
+                if (lane == 0) umma_commit(smem_u32(&B->s_full[i]));
+            }
+            release(ks, at - 1);
+            if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
+            for (int it = 0; ok && it < w.n; ++it) {
+                const bool more = it + 1 < w.n;
+                if (!(ok = take(vs))) break;
+                const uint32_t v_at = at - 1;
+                blank(w, w.tile + it, vs);
+                for (int i = 0; ok && i < nt; ++i) {
+                    ok = mbar_wait(smem_u32(&B->p_full[i]), g[i] & 1, abort, a.c.err);
+                    if (ok && it == 0) ok = mbar_wait(smem_u32(&B->o_empty[i]), (piece[i] & 1) ^ 1, abort, a.c.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(i, i, 0, vs, it > 0);
+                    if (!more && lane == 0) umma_commit(smem_u32(&B->o_done[i]));
                     if (more) {
                         if (i == 0 && !(ok = take(ks))) break;
-                        scores(i, i, ks);
+                        scores(i, i, 0, ks);
+                        if (lane == 0) umma_commit(smem_u32(&B->s_full[i]));
                     }
+                    ++g[i];
                 }
-                ++g[i];
-            }
-            if (!ok) break;
-            release(vs, v_at);
-            if constexpr (NS == 2) {
+                if (!ok) break;
+                release(vs, v_at);
                 if (more) {
                     release(ks, at - 1);
                     if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
@@ -619,7 +828,7 @@ __device__ __forceinline__ void head_role(const AttnArgs& a, Bars* B) {
     Walk<C> w(B);
     while (w.next(a)) {
         if (w.tile == 0 && !w.ends(a)) {
-            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of<C::BN>(w.s, w.t, a.tq * C::NS);
+            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of(w.s, w.t, a.tq * C::NS);
             hd = make_int4(w.b, w.h, w.t, (int)((end * n - 1) / B->total));
         }
         at += w.n;
@@ -632,7 +841,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t qs = smem_u32(smem), ring = qs + C::kQBytes;
-    Bars* B = reinterpret_cast<Bars*>(smem + C::kQBytes + (size_t)C::ST * C::kSlot);
+    uint8_t* fixed = smem + C::kQBytes + (size_t)C::ST * C::kUnit;
+    Bars* B = reinterpret_cast<Bars*>(fixed);
+    float2* stats = reinterpret_cast<float2*>(fixed + kBarBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::ST; ++i) {
@@ -646,15 +857,16 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
             mbar_init(smem_u32(&B->s_full[i]), 1);
             mbar_init(smem_u32(&B->p_full[i]), 4);
             mbar_init(smem_u32(&B->o_done[i]), 1);
-            mbar_init(smem_u32(&B->o_empty[i]), 4);
+            mbar_init(smem_u32(&B->o_empty[i]), C::HL ? C::kCorrWarps : 4);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&B->stat_full[i]), 4);
         B->abort = 0;
         ptx::mbar_init_fence();
         tma_prefetch_desc(&a.mk);
         tma_prefetch_desc(&a.mv);
         if (!C::HL) tma_prefetch_desc(&a.mq);
     }
-    if (warp == C::kSoftWarps + 1) tmem_alloc(smem_u32(&B->tmem), 512);
+    if (warp == C::kMisc + 1) tmem_alloc(smem_u32(&B->tmem), 512);
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     plan<C>(a, B);
@@ -662,14 +874,31 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B->tmem;
-    if (warp < C::kSoftWarps) softmax_role<C>(a, B, tmem, warp, lane);
-    else if (warp == C::kSoftWarps) load_role<C>(a, B, ring, lane);
-    else if (warp == C::kSoftWarps + 1) mma_role<C>(a, B, qs, ring, tmem, lane);
-    else if (warp == C::kSoftWarps + 2) q_role<C>(a, B, qs, lane);
-    else if (lane == 0) head_role<C>(a, B);
+    // Registers: the launch's share is 168 a thread with 384 threads and 128 with 512.
+    if (warp < C::kSoftWarps) {
+        if constexpr (C::HL) {
+            if constexpr (C::D == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");   // 104 + 2 x 168 + 72 = 4 x 128
+            softmax_tile_role<C>(a, B, stats, tmem, warp, lane);
+        } else {
+            if constexpr (C::NS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");    // 2 x 208 + 88 = 3 x 168
+            softmax_role<C>(a, B, tmem, warp, lane);
+        }
+    } else if (C::HL && warp < C::kMisc) {
+        if constexpr (C::HL) {
+            if constexpr (C::D == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+            correct_role<C>(a, B, stats, tmem, warp, lane);
+        }
+    } else {
+        if constexpr (C::HL && C::D == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if constexpr (C::NS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == C::kMisc) load_role<C>(a, B, ring, lane);
+        else if (warp == C::kMisc + 1) mma_role<C>(a, B, qs, ring, tmem, lane);
+        else if (warp == C::kMisc + 2) q_role<C>(a, B, qs, lane);
+        else if (lane == 0) head_role<C>(a, B);
+    }
     tc_fence_before();
     __syncthreads();
-    if (warp == C::kSoftWarps + 1) {
+    if (warp == C::kMisc + 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -727,7 +956,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_con
 }
 
 struct Plan {
-    int ns, bn, rec_rows;
+    int ns, rec_rows;
     size_t rec, ml, total;
 };
 
@@ -735,8 +964,7 @@ Plan make_plan(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, int
     Plan p{};
     const int64_t G = d->n_head_q / cache->n_head_kv, rows = cache->n_tokens * G;
     // two query tiles a CTA when the sequences fill more than one on average
-    p.ns = cache->head_dim < 256 && rows > 128 * cache->batch_size ? 2 : 1;
-    p.bn = cache->head_dim == 256 ? 64 : 128;
+    p.ns = d->type == MLZC_TYPE_F16 && cache->head_dim < 256 && rows > 128 * cache->batch_size ? 2 : 1;
     p.rec_rows = (int)std::min<int64_t>(128 * p.ns, (rows + 3) / 4 * 4);
     p.rec = (size_t)ctas * 2 * p.rec_rows * cache->head_dim * 4;
     p.ml = (size_t)ctas * 2 * p.rec_rows * 8;
@@ -795,7 +1023,7 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     const bool f32 = d->type == MLZC_TYPE_F32;
     a.G = (int)(d->n_head_q / cache->n_head_kv);
     a.tq = 128 / a.G;
-    a.box = std::gcd(cache->page_size, p.bn);
+    a.box = std::gcd(cache->page_size, BN);
     if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
     if ((st = paged::encode_pool(&a.mv, cache, true, a.box)) != MLZC_OK) return st;
     if (!f32 && (st = paged::encode_rows(&a.mq, d->q, cache->head_dim, d->n_head_q, cache->n_tokens, d->q_nb[1], d->q_nb[2],
@@ -815,11 +1043,8 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     a.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.rec);
     a.head = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.rec + p.ml);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch ((int)cache->head_dim * 10 + p.ns) {
-        case 641: return f32 ? launch<Cfg<64, 1, true>>(a, c, s) : launch<Cfg<64, 1, false>>(a, c, s);
-        case 642: return f32 ? launch<Cfg<64, 2, true>>(a, c, s) : launch<Cfg<64, 2, false>>(a, c, s);
-        case 1281: return f32 ? launch<Cfg<128, 1, true>>(a, c, s) : launch<Cfg<128, 1, false>>(a, c, s);
-        case 1282: return f32 ? launch<Cfg<128, 2, true>>(a, c, s) : launch<Cfg<128, 2, false>>(a, c, s);
-        default: return f32 ? launch<Cfg<256, 1, true>>(a, c, s) : launch<Cfg<256, 1, false>>(a, c, s);
-    }
+    const int D = (int)cache->head_dim;
+    if (f32) return D == 64 ? launch<Cfg<64, 1, true>>(a, c, s) : (D == 128 ? launch<Cfg<128, 1, true>>(a, c, s) : launch<Cfg<256, 1, true>>(a, c, s));
+    if (p.ns == 2) return D == 64 ? launch<Cfg<64, 2, false>>(a, c, s) : launch<Cfg<128, 2, false>>(a, c, s);
+    return D == 64 ? launch<Cfg<64, 1, false>>(a, c, s) : (D == 128 ? launch<Cfg<128, 1, false>>(a, c, s) : launch<Cfg<256, 1, false>>(a, c, s));
 }
