@@ -57,15 +57,16 @@ using ptx::smem_u32;
 using namespace tc05;
 
 // Bounded wait as ptx::mbar_wait, all inline: kernels that move registers between warpgroups
-// cannot call functions.
+// cannot call functions.  The timer, slow to read, is looked at after some polls only.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* err) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = ptx::global_ns();
+    uint64_t t0 = 0;
     for (uint32_t i = 1;; ++i) {
         if (ptx::mbar_try_wait(bar, parity)) return true;
         if ((i & 31) == 0) {
             if (*abort) return false;
-            if (ptx::global_ns() - t0 > ptx::kWaitNs) {
+            const uint64_t t = ptx::global_ns();
+            if (!t0) t0 = t;
+            if (t - t0 > ptx::kWaitNs) {
                 atomicOr(err, MLZC_DEVERR_WAIT_TIMEOUT);
                 *abort = 1;
                 return false;
@@ -127,6 +128,8 @@ struct Cfg {
     static constexpr int kCorrWarps = HL ? 4 * (D / CD) : 0;
     static constexpr int kMisc = kSoftWarps + kCorrWarps;
     static constexpr int kThreads = (kMisc + 4) * 32;
+    // f32: the softmax holds a row's scores in registers (256 dims: the correction needs those)
+    static constexpr bool kHold = D < 256;
     static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
     static constexpr uint32_t kOCol = 2 * BN;             // O of tile i at + i * D
     static_assert(2 * BN + NS * D <= 512, "TMEM");
@@ -136,7 +139,7 @@ struct Cfg {
 
 // Barriers in shared memory.
 struct Bars {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], o_step, o_done[2], o_empty[2], stat_full[4];
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], p_half[2], o_step, o_done[2], o_empty[2], stat_full[4];
     uint32_t tmem;
     int abort;
     long long first, count, total;   // this CTA's share of the list; its start's place
@@ -273,6 +276,19 @@ __device__ __forceinline__ float capped(float s, float cap_in, float cap) {
     return copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, s);
 }
 
+// One in so many pairs of exponentials goes to the FMA pipe: the exponential unit takes 1024
+// clocks a tile and warp scheduler, as long as a tile's matrix products.
+constexpr int kPolyEvery = 4;
+
+__device__ __forceinline__ float row_max(const float (&x)[BN]) {
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = max3(x[3 * i], x[3 * i + 1], x[3 * i + 2]);
+#pragma unroll
+    for (int i = 12; i + 1 < BN; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], x[i], x[i + 1]);
+    return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
 // Where a piece's rows go: dst and lse when it is the whole query tile, else a record.
 template <class C>
 struct Sink {
@@ -344,10 +360,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
 #pragma unroll
                     for (int i = 0; i < BN; ++i) x[i] = i > limit ? -INFINITY : x[i];
                 }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int i = 4; i < BN; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float top = row_max(x);
                 if (it == 0) {
                     m = top;
                 } else if (__any_sync(~0u, top > m + rise)) {
@@ -370,27 +383,46 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                     }
                 }
                 const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t c22 = pair(c2, c2), off2 = pair(off, off);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i) {
                     uint32_t hi[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float p0 = ex2(fmaf(x[i * 32 + 2 * j], c2, off));
-                        const float p1 = ex2(fmaf(x[i * 32 + 2 * j + 1], c2, off));
-                        sum[j & 1] += p0;
-                        sum[2 + (j & 1)] += p1;
+                        const uint64_t y = fma2(pair(x[i * 32 + 2 * j], x[i * 32 + 2 * j + 1]), c22, off2);
+                        float p0, p1;
+                        if (j % kPolyEvery == kPolyEvery - 1) {
+                            exp2_poly(y, p0, p1);
+                        } else {
+                            unpair(y, p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                        }
+                        sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
                         hi[j] = ptx::pack_h2(p0, p1);
                     }
                     tmem_st16(s_col + i * 32, hi);
+                    // the first half of P: its products start while the second is computed
+                    if (C::NS == 2 && i == BN / 64 - 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&B->p_half[buf]));
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float s0, s1;
+                unpair(add2(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
                 tmem_st_wait();
+            } else if (C::NS == 2 && lane == 0) {
+                mbar_arrive(smem_u32(&B->p_half[buf]));
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&B->p_full[buf]));
         }
+        if (m == -INFINITY) l = 0.0f;   // nothing seen (the polynomial's floor is not 0)
         // the piece's O
         if (!mbar_wait(smem_u32(&B->o_done[slot]), piece & 1, abort, a.c.err)) return;
         tc_fence_after();
@@ -438,48 +470,77 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                 const uint32_t s_col = lanes + C::kSCol + buf * BN;
                 const int limit = own - (w.tile + it) * BN;
                 const bool cut = __any_sync(~0u, limit < BN - 1);
-                float m = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < BN; i += 32) {
-                    uint32_t r[32];
-                    tmem_ld32(s_col + i, r);
-                    tmem_ld_wait();
-                    if (a.softcap > 0.0f || cut) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float x = __uint_as_float(r[j]);
-                            if (a.softcap > 0.0f) x = capped(x, cap_in, a.softcap);
-                            r[j] = __float_as_uint(i + j > limit ? -INFINITY : x);
-                        }
-                        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));
-                        tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(r + 16));
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(r[j]));
-                    m = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-                }
-                tmem_st_wait();
-                const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < BN; i += 32) {
-                    uint32_t r[32], hi[16], lo[16];
-                    tmem_ld32(s_col + i, r);
-                    tmem_ld_wait();
+                const uint64_t c22 = pair(c2, c2);
+                uint64_t sum[2] = {0, 0};
+                float m;
+                // 32 slots of P from their scores
+                auto weigh = [&](const float* x, int i, uint64_t off2) {
+                    uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float p0 = ex2(fmaf(__uint_as_float(r[2 * j]), c2, off));
-                        const float p1 = ex2(fmaf(__uint_as_float(r[2 * j + 1]), c2, off));
-                        sum[j & 1] += p0;
-                        sum[2 + (j & 1)] += p1;
-                        ptx::split_h2(p0, p1, hi[j], lo[j]);
+                        float p0, p1, h0, h1;
+                        unpair(fma2(pair(x[2 * j], x[2 * j + 1]), c22, off2), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        const uint64_t p = pair(p0, p1);
+                        sum[j & 1] = add2(sum[j & 1], p);
+                        // hi: the first 11 bits (f16 holds them), lo: the rest, within 2^-22
+                        h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                        h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                        hi[j] = ptx::pack_h2(h0, h1);
+                        unpair(fma2(pair(h0, h1), pair(-1.0f, -1.0f), p), p0, p1);
+                        lo[j] = ptx::pack_h2(p0, p1);
                     }
                     tmem_st16(s_col + i, hi);
                     tmem_st16(s_col + i + 16, lo);
+                };
+                auto clip = [&](float x, int i) {
+                    if (a.softcap > 0.0f) x = capped(x, cap_in, a.softcap);
+                    return i > limit ? -INFINITY : x;
+                };
+                if constexpr (C::kHold) {
+                    float x[BN];
+#pragma unroll
+                    for (int i = 0; i < BN / 32; ++i)
+                        tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
+                    tmem_ld_wait();
+                    if (a.softcap > 0.0f || cut) {
+#pragma unroll
+                        for (int i = 0; i < BN; ++i) x[i] = clip(x[i], i);
+                    }
+                    m = row_max(x);
+                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+#pragma unroll
+                    for (int i = 0; i < BN; i += 32) weigh(x + i, i, pair(off, off));
+                } else {
+                    m = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < BN; i += 32) {
+                        uint32_t r[32];
+                        tmem_ld32(s_col + i, r);
+                        tmem_ld_wait();
+                        if (a.softcap > 0.0f || cut) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(clip(__uint_as_float(r[j]), i + j));
+                            tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));
+                            tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(r + 16));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) m = max3(m, __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+                    }
+                    tmem_st_wait();
+                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+#pragma unroll
+                    for (int i = 0; i < BN; i += 32) {
+                        float r[32];
+                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(r));
+                        tmem_ld_wait();
+                        weigh(r, i, pair(off, off));
+                    }
                 }
-                stats[(g & 3) * 128 + q.row] =
-                    make_float2(m == -INFINITY ? -INFINITY : m * c2 - kPOffset, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                float s0, s1;
+                unpair(add2(sum[0], sum[1]), s0, s1);
+                stats[(g & 3) * 128 + q.row] = make_float2(m == -INFINITY ? -INFINITY : m * c2 - kPOffset, s0 + s1);
                 tmem_st_wait();
             }
             tc_fence_before();
@@ -527,12 +588,12 @@ __device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, const f
                 const float f = st.x == -INFINITY ? 0.0f : ex2(st.x - e);
                 l = fmaf(st.y, f, l);
 #pragma unroll
-                for (int i = 0; i < CD; i += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(o_col + i, r);
+                for (int i = 0; i < CD; i += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(o_col + i, r);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i + j] = fmaf(__uint_as_float(r[j]), f, o[i + j]);
+                    for (int j = 0; j < 32; ++j) o[i + j] = fmaf(__uint_as_float(r[j]), f, o[i + j]);
                 }
             }
             tc_fence_before();
@@ -686,33 +747,40 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
     };
     // frees unit `st`, the ring's `index`-th, when the products issued so far are done
     auto release = [&](uint32_t st, uint32_t index) {
-        if (lane == 0) umma_commit(smem_u32(&B->empty[st]));
+        if (elect_one()) umma_commit(smem_u32(&B->empty[st]));
         last_bar = smem_u32(&B->empty[st]);
         last_par = (index / C::ST) & 1;
     };
     auto scores = [&](int tile, int buf, int unit, uint32_t st) {
-        if (lane == 0) {
-            const uint64_t k = umma_desc_sw128(ring + st * C::kUnit);
+        const uint32_t k_at = uniform(ring + st * C::kUnit);
+        const uint32_t q_at = uniform(qs + tile * (C::HL ? 2 : 1) * C::kQTile + unit * C::SUBS * C::kQSub);
+        const uint32_t d = uniform(tmem + C::kSCol + buf * BN);
+        const bool first = uniform(unit) == 0;
+        if (elect_one()) {
+            const uint64_t k = umma_desc_sw128(k_at);
 #pragma unroll
             for (int part = C::HL ? 1 : 0; part >= 0; --part) {      // lo, then hi
-                const uint64_t q = umma_desc_sw128(qs + (tile * (C::HL ? 2 : 1) + part) * C::kQTile + unit * C::SUBS * C::kQSub);
+                const uint64_t q = umma_desc_sw128(q_at + part * C::kQTile);
 #pragma unroll
                 for (int i = 0; i < DU / 16; ++i)
-                    umma_f16(tmem + C::kSCol + buf * BN, q + (((i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
+                    umma_f16(d, q + (((i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
                              k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s,
-                             unit > 0 || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
+                             !first || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
             }
         }
     };
-    auto values = [&](int tile, int buf, int unit, uint32_t st, bool add) {
-        if (lane == 0) {
-            const uint64_t v = umma_desc_mn_sw128(ring + st * C::kUnit, C::kSub);
+    // key steps [i0, i1) of P V
+    auto values = [&](int tile, int buf, int unit, uint32_t st, bool add, int i0, int i1) {
+        const uint32_t v_at = uniform(ring + st * C::kUnit);
+        const uint32_t d = uniform(tmem + C::kOCol + tile * C::D + unit * DU), p = uniform(tmem + C::kSCol + buf * BN);
+        const bool sum = uniform(add) != 0;
+        if (elect_one()) {
+            const uint64_t v = umma_desc_mn_sw128(v_at, C::kSub);
 #pragma unroll
             for (int part = C::HL ? 1 : 0; part >= 0; --part)
 #pragma unroll
-                for (int i = 0; i < BN / 16; ++i)
-                    umma_f16_ta(tmem + C::kOCol + tile * C::D + unit * DU, tmem + C::kSCol + buf * BN + (i >> 1) * 32 + (i & 1) * 8 + part * 16,
-                                v + ((i * 2048) >> 4), idesc_o, add || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
+                for (int i = i0; i < i1; ++i)
+                    umma_f16_ta(d, p + (i >> 1) * 32 + (i & 1) * 8 + part * 16, v + ((i * 2048) >> 4), idesc_o, sum || i > i0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
         }
     };
     // V rows that no row of the piece sees may hold anything (a page's unused rows) or have not
@@ -735,7 +803,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
             scores(0, buf, unit, st);
             release(st, at - 1);
         }
-        if (lane == 0) umma_commit(smem_u32(&B->s_full[buf]));
+        if (elect_one()) umma_commit(smem_u32(&B->s_full[buf]));
         return true;
     };
     bool ok = true;
@@ -748,12 +816,12 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
         tc_fence_after();
         if constexpr (NS == 1) {
             if (!(ok = scores_all(g[0] & 1))) break;
-            if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
+            if (w.n == 1 && elect_one()) umma_commit(smem_u32(&B->q_empty));
             for (int it = 0; it < w.n; ++it, ++g[0]) {
                 const int buf = g[0] & 1;
                 if (it + 1 < w.n) {
                     if (!(ok = scores_all(buf ^ 1))) break;
-                    if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
+                    if (it + 2 == w.n && elect_one()) umma_commit(smem_u32(&B->q_empty));
                 }
                 ok = mbar_wait(smem_u32(&B->p_full[buf]), (g[0] >> 1) & 1, abort, a.c.err);
                 // O free: f32 calls empty it tile by tile, the others piece by piece
@@ -764,11 +832,11 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
                     if (!(ok = take(st))) break;
                     blank(w, w.tile + it, st);
                     tc_fence_after();
-                    values(0, buf, unit, st, !C::HL && it > 0);
+                    values(0, buf, unit, st, !C::HL && it > 0, 0, BN / 16);
                     release(st, at - 1);
                 }
                 if (!ok) break;
-                if (lane == 0) {
+                if (elect_one()) {
                     if (C::HL || it + 1 == w.n) umma_commit(smem_u32(&B->o_done[0]));
                     if (!C::HL) umma_commit(smem_u32(&B->o_step));
                 }
@@ -778,26 +846,29 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
             if (!(ok = take(ks))) break;
             for (int i = 0; i < nt; ++i) {
                 scores(i, i, 0, ks);
-                if (lane == 0) umma_commit(smem_u32(&B->s_full[i]));
+                if (elect_one()) umma_commit(smem_u32(&B->s_full[i]));
             }
             release(ks, at - 1);
-            if (w.n == 1 && lane == 0) umma_commit(smem_u32(&B->q_empty));
+            if (w.n == 1 && elect_one()) umma_commit(smem_u32(&B->q_empty));
             for (int it = 0; ok && it < w.n; ++it) {
                 const bool more = it + 1 < w.n;
                 if (!(ok = take(vs))) break;
                 const uint32_t v_at = at - 1;
                 blank(w, w.tile + it, vs);
                 for (int i = 0; ok && i < nt; ++i) {
-                    ok = mbar_wait(smem_u32(&B->p_full[i]), g[i] & 1, abort, a.c.err);
+                    ok = mbar_wait(smem_u32(&B->p_half[i]), g[i] & 1, abort, a.c.err);
                     if (ok && it == 0) ok = mbar_wait(smem_u32(&B->o_empty[i]), (piece[i] & 1) ^ 1, abort, a.c.err);
                     if (!ok) break;
                     tc_fence_after();
-                    values(i, i, 0, vs, it > 0);
-                    if (!more && lane == 0) umma_commit(smem_u32(&B->o_done[i]));
+                    values(i, i, 0, vs, it > 0, 0, BN / 32);
+                    if (!(ok = mbar_wait(smem_u32(&B->p_full[i]), g[i] & 1, abort, a.c.err))) break;
+                    tc_fence_after();
+                    values(i, i, 0, vs, true, BN / 32, BN / 16);
+                    if (!more && elect_one()) umma_commit(smem_u32(&B->o_done[i]));
                     if (more) {
                         if (i == 0 && !(ok = take(ks))) break;
                         scores(i, i, 0, ks);
-                        if (lane == 0) umma_commit(smem_u32(&B->s_full[i]));
+                        if (elect_one()) umma_commit(smem_u32(&B->s_full[i]));
                     }
                     ++g[i];
                 }
@@ -805,7 +876,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
                 release(vs, v_at);
                 if (more) {
                     release(ks, at - 1);
-                    if (it + 2 == w.n && lane == 0) umma_commit(smem_u32(&B->q_empty));
+                    if (it + 2 == w.n && elect_one()) umma_commit(smem_u32(&B->q_empty));
                 }
             }
         }
@@ -836,6 +907,12 @@ __device__ __forceinline__ void head_role(const AttnArgs& a, Bars* B) {
     a.head[blockIdx.x] = hd;
 }
 
+template <int FROM, int TO>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (TO > FROM) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TO));
+    if constexpr (TO < FROM) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TO));
+}
+
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_constant__ AttnArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -844,7 +921,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     uint8_t* fixed = smem + C::kQBytes + (size_t)C::ST * C::kUnit;
     Bars* B = reinterpret_cast<Bars*>(fixed);
     float2* stats = reinterpret_cast<float2*>(fixed + kBarBytes);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::ST; ++i) {
             mbar_init(smem_u32(&B->full[i]), 1);
@@ -856,6 +933,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&B->s_full[i]), 1);
             mbar_init(smem_u32(&B->p_full[i]), 4);
+            mbar_init(smem_u32(&B->p_half[i]), 4);
             mbar_init(smem_u32(&B->o_done[i]), 1);
             mbar_init(smem_u32(&B->o_empty[i]), C::HL ? C::kCorrWarps : 4);
         }
@@ -874,23 +952,24 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B->tmem;
-    // Registers: the launch's share is 168 a thread with 384 threads and 128 with 512.
+    // Registers: the launch's share is 168 a thread with 384 threads and 128 with 512; a wait
+    // for more than the launch's sum would not end.
+    constexpr int kShare = C::kThreads == 512 ? 128 : (C::kThreads == 384 ? 168 : 255);
+    constexpr int kSoft = C::HL ? (C::D == 64 ? 160 : (C::D == 128 ? 176 : 104)) : (C::NS == 2 ? 208 : 255);
+    constexpr int kCorr = C::HL ? (C::D == 64 ? 120 : (C::D == 128 ? 216 : 168)) : 0;
+    constexpr int kRest = C::HL ? (C::D == 128 ? 112 : 72) : (C::NS == 2 ? 88 : 255);
+    static_assert(kSoft * C::kSoftWarps + kCorr * C::kCorrWarps + kRest * 4 <= kShare * (C::kThreads / 32), "registers");
     if (warp < C::kSoftWarps) {
-        if constexpr (C::HL) {
-            if constexpr (C::D == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");   // 104 + 2 x 168 + 72 = 4 x 128
-            softmax_tile_role<C>(a, B, stats, tmem, warp, lane);
-        } else {
-            if constexpr (C::NS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");    // 2 x 208 + 88 = 3 x 168
-            softmax_role<C>(a, B, tmem, warp, lane);
-        }
+        set_registers<kShare, kSoft>();
+        if constexpr (C::HL) softmax_tile_role<C>(a, B, stats, tmem, warp, lane);
+        else softmax_role<C>(a, B, tmem, warp, lane);
     } else if (C::HL && warp < C::kMisc) {
         if constexpr (C::HL) {
-            if constexpr (C::D == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+            set_registers<kShare, kCorr>();
             correct_role<C>(a, B, stats, tmem, warp, lane);
         }
     } else {
-        if constexpr (C::HL && C::D == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if constexpr (C::NS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        set_registers<kShare, kRest>();
         if (warp == C::kMisc) load_role<C>(a, B, ring, lane);
         else if (warp == C::kMisc + 1) mma_role<C>(a, B, qs, ring, tmem, lane);
         else if (warp == C::kMisc + 2) q_role<C>(a, B, qs, lane);

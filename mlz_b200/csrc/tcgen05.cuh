@@ -127,6 +127,22 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// One lane of a converged warp, in a form that the compiler knows to be a single lane.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n"
+        " .reg .pred p;\n"
+        " elect.sync _|p, 0xffffffff;\n"
+        " selp.b32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(p));
+    return p != 0;
+}
+// The value of lane 0, known to the compiler to be the same in all lanes: what instructions
+// that take uniform registers (tcgen05.mma's descriptors) are computed from.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -139,6 +155,51 @@ __device__ __forceinline__ void tmem_alloc(uint32_t holder, uint32_t cols) {
 }
 __device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+
+// Pairs of f32 in one 64-bit register: two operations an instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two values on the FMA pipe, for kernels bound by the exponential unit: x = n + f with
+// |f| <= 1/2 (adding 1.5 * 2^23 rounds to an integer, left in the low bits), 2^f by its minimax
+// polynomial of degree 4 (relative error 2.6e-6, Remez), n added to the exponent.  Below -126:
+// 2^-126.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
+    float a, b, t0, t1;
+    unpair(x, a, b);
+    x = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const float kRound = 12582912.0f;
+    const uint64_t t = add2(x, pair(kRound, kRound));
+    const uint64_t n = add2(t, pair(-kRound, -kRound));
+    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
+    uint64_t p = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+    unpair(t, t0, t1);
+    unpair(p, a, b);
+    r0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+    r1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
 }  // namespace tc05
