@@ -3,6 +3,9 @@
 #pragma once
 
 #include "internal.h"
+#ifdef __CUDACC__
+#include "ptx.cuh"
+#endif
 
 namespace mlzc {
 namespace paged {
@@ -57,6 +60,24 @@ __device__ __forceinline__ int load_page(const View& c, int b, int i) {
     if ((unsigned)p < (unsigned)c.n_pages) return p;
     atomicOr(c.err, MLZC_DEVERR_BAD_INDEX);
     return -1;
+}
+// Bounded wait as ptx::mbar_wait, all inline: kernels that move registers between warpgroups
+// cannot call functions.  The timer, slow to read, is looked at after some polls only.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* err) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((i & 31) == 0) {
+            if (*abort) return false;
+            const uint64_t t = ptx::global_ns();
+            if (!t0) t0 = t;
+            if (t - t0 > ptx::kWaitNs) {
+                atomicOr(err, MLZC_DEVERR_WAIT_TIMEOUT);
+                *abort = 1;
+                return false;
+            }
+        }
+    }
 }
 #endif
 

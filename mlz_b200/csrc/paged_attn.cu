@@ -54,26 +54,8 @@ using ptx::mbar_arrive;
 using ptx::mbar_expect_tx;
 using ptx::mbar_init;
 using ptx::smem_u32;
+using paged::mbar_wait;
 using namespace tc05;
-
-// Bounded wait as ptx::mbar_wait, all inline: kernels that move registers between warpgroups
-// cannot call functions.  The timer, slow to read, is looked at after some polls only.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, unsigned int* err) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; ++i) {
-        if (ptx::mbar_try_wait(bar, parity)) return true;
-        if ((i & 31) == 0) {
-            if (*abort) return false;
-            const uint64_t t = ptx::global_ns();
-            if (!t0) t0 = t;
-            if (t - t0 > ptx::kWaitNs) {
-                atomicOr(err, MLZC_DEVERR_WAIT_TIMEOUT);
-                *abort = 1;
-                return false;
-            }
-        }
-    }
-}
 
 constexpr int kSmemMax = 232448;
 constexpr int kBarBytes = 512;
@@ -270,12 +252,6 @@ struct Row {
     }
 };
 
-// cap * tanh(s scale / cap) = cap (1 - e) / (1 + e), e = exp(-2 |s| scale / cap) = 2^(|s| cap_in).
-__device__ __forceinline__ float capped(float s, float cap_in, float cap) {
-    const float e = ex2(fabsf(s) * cap_in);
-    return copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, s);
-}
-
 // One in so many pairs of exponentials goes to the FMA pipe: the exponential unit takes 1024
 // clocks a tile and warp scheduler, as long as a tile's matrix products.
 constexpr int kPolyEvery = 4;
@@ -422,7 +398,6 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&B->p_full[buf]));
         }
-        if (m == -INFINITY) l = 0.0f;   // nothing seen (the polynomial's floor is not 0)
         // the piece's O
         if (!mbar_wait(smem_u32(&B->o_done[slot]), piece & 1, abort, a.c.err)) return;
         tc_fence_after();

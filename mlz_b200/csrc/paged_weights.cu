@@ -1,74 +1,609 @@
 // paged_weights.cu -- the attention weight that each slot of a paged KV cache received from the
-// new tokens (mlzc_paged_weights_dev).
+// new tokens (mlzc_paged_weights_dev), on the 5th-generation tensor cores.
 //
-// One warp a slot: the sum of exp(score - lse) over the query rows that see it.
+//   out[j] = acc[j] + sum over the rows r that see slot j of 2^(c s_jr - lse2_r),
+//   s_jr = <k_j, q_r>,  c = scale * log2 e,  lse2 = lse * log2 e,
+// for every (sequence, KV head); the rows are its new tokens x the query heads of the head.
+//
+// The scores are recomputed (storing them would cost 4 bytes a score) as S^T = K Q^T: slots on
+// the lanes, rows on the columns.  A slot's sum then stays in one thread, so nothing is added
+// across threads and nothing atomically, and the softmax's statistics, known from the
+// attention, enter as one constant a column: one FMA, one exponential and one add a score.  The
+// exponential unit (1024 clocks a 128 x 128 tile; the products take 512) is the bound for long
+// chunks, reading K that for decode.  kPolyEvery moves a share of the exponentials to the FMA
+// pipe.
+//
+// A CTA takes 128 slots of a head (K tile, held) and walks their query tiles: loader warp (K by
+// one TMA box a page piece, Q by one box a 64-dim block, all into one ring of units), MMA warp
+// (scores into four TMEM buffers, as many columns as there are rows), lse warp (a tile's lse2
+// into shared memory), two warpgroups that take turns at the tiles.  f32 queries come as f16 hi
+// + lo from a small preparing launch, low products summed first.
+//
+// Slot tiles x query tiles of a call form one list cut into equal shares, as in paged_attn.cu;
+// a cut slot tile's 128 partial sums are merged in order by a last launch.
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <numeric>
 
 #include "paged.h"
 #include "ptx.cuh"
+#include "tcgen05.cuh"
 
 namespace mlzc {
 namespace {
 
+using paged::mbar_wait;
 using paged::Seq;
 using paged::View;
+using ptx::mbar_arrive;
+using ptx::mbar_expect_tx;
+using ptx::mbar_init;
+using ptx::smem_u32;
+using namespace tc05;
+
+constexpr int kSmemMax = 232448;
+constexpr int kBN = 128;               // slots a tile
+constexpr int kBufs = 4;               // score buffers in TMEM (128 columns each) and lse tiles
+constexpr int kFixed = 512 + kBufs * 128 * 4 + 2 * 128 * 4;   // barriers, lse tiles, sums handed over
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 4) * 32;
+constexpr int kPolyEvery = 4;          // of so many pairs of exponentials one goes to the FMA pipe
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct WeightArgs {
     View c;
-    const char* q;
-    size_t q_head, q_tok, lse_head, lse_tok;
+    CUtensorMap mk, mq, mql;           // K pool; q rows (hi), lo
     const char* lse;
     const char* acc;
     char* out;
-    size_t a_head, a_seq, o_head, o_seq;
-    int n_head_q, f32;
+    size_t lse_head, lse_tok, a_head, a_seq, o_head, o_seq;
+    int G, tq, box, n_ctas;
     float scale, softcap;
+    float* rec;                        // [cta][2][128]: 0 continues a cut slot tile, 1 begins one
+    int4* head;                        // [cta]: sequence (-1: none), kv head, slot tile, last CTA of the tile begun
 };
 
-constexpr int kWarps = 8;
+template <int D_, bool HL_>
+struct Cfg {
+    static constexpr int D = D_;
+    static constexpr bool HL = HL_;
+    static constexpr int DU = D < 128 ? D : 128;      // dims of a ring unit (128 rows)
+    static constexpr int UN = D / DU;
+    static constexpr int SUBS = DU / 64;
+    static constexpr uint32_t kSub = 128 * 128;
+    static constexpr uint32_t kUnit = kSub * SUBS;
+    static constexpr int kFit = (kSmemMax - 1024 - kFixed) / (int)kUnit;
+    static constexpr int ST = kFit > 12 ? 12 : kFit;
+    static constexpr size_t kSmem = 1024 + kFixed + (size_t)ST * kUnit;
+    static constexpr int QU = UN * (HL ? 2 : 1);      // units of a Q tile
+    static_assert(ST >= UN + 2, "ring");
+};
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32) weights_kernel(const __grid_constant__ WeightArgs a) {
-    constexpr int E = D / 32;
-    ptx::pdl_launch_dependents();
-    ptx::pdl_wait();
-    const View& c = a.c;
-    const int lane = threadIdx.x & 31, hk = blockIdx.y, b = blockIdx.z;
-    const Seq s = paged::load_seq(c, b);
-    const int G = a.n_head_q / c.n_head_kv;
-    for (int j = blockIdx.x * kWarps + (threadIdx.x >> 5); j < s.kv; j += gridDim.x * kWarps) {
-        const int page = paged::load_page(c, b, j / c.page);
-        float k[E];
-        const __half* kr = reinterpret_cast<const __half*>(c.k + (size_t)page * c.k_page + (size_t)hk * c.k_head + (size_t)(j % c.page) * c.k_row);
-#pragma unroll
-        for (int e = 0; e < E; ++e) k[e] = page < 0 ? 0.0f : __half2float(kr[lane * E + e]);
-        float sum = 0.0f;
-        for (int i = std::max(0, j - (s.kv - s.rows)); i < s.rows; ++i)
-            for (int g = 0; g < G; ++g) {
-                const int t = s.row0 + i, h = hk * G + g;
-                const char* qr = a.q + (size_t)t * a.q_tok + (size_t)h * a.q_head;
-                float x = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int d = lane * E + e;
-                    x += k[e] * (a.f32 ? reinterpret_cast<const float*>(qr)[d] : __half2float(reinterpret_cast<const __half*>(qr)[d]));
+struct Bars {
+    uint64_t full[12], empty[12], s_full[kBufs], s_empty[kBufs], lse_full[kBufs], hand_full[2], hand_empty[2];
+    uint32_t tmem;
+    int abort;
+    long long first, count, total;
+    int b, h, t, tile;
+    long long scan[kThreads / 32];
+};
+static_assert(sizeof(Bars) <= 512, "barriers");
+
+// Query tiles of slot tile t: from the first one with a row that sees slot 128 t on; one at
+// least, so that every slot below kv_len is written.
+__device__ __forceinline__ int first_tile(const WeightArgs& a, const Seq& s, int t) {
+    return max(0, t * kBN - (s.kv - s.rows)) / a.tq;
+}
+__device__ __forceinline__ int tiles_of(const WeightArgs& a, const Seq& s, int t) {
+    return max(1, (s.rows + a.tq - 1) / a.tq - first_tile(a, s, t));
+}
+// The sum of tiles_of over a sequence's slot tiles: all alike up to the chunk's own slots.
+struct Tiles {
+    int alike, all;            // slot tiles [0, alike) have `each` query tiles
+    int each;
+    long long sum;
+    __device__ Tiles(const WeightArgs& a, const Seq& s) {
+        all = (s.kv + kBN - 1) / kBN;
+        each = tiles_of(a, s, 0);
+        const int off = max(0, s.kv - s.rows);
+        alike = min(all, off / kBN + 1);
+        sum = (long long)alike * each;
+        for (int t = alike; t < all; ++t) sum += tiles_of(a, s, t);
+    }
+};
+
+struct Walk {
+    int b, h, t, tile, n;
+    long long left;
+    Seq s;
+    bool first;
+    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(B->tile), n(0), left(B->count), first(true) {}
+    __device__ bool next(const WeightArgs& a) {
+        if (left <= 0) return false;
+        if (first) {
+            s = paged::load_seq(a.c, b);
+            first = false;
+        } else {
+            tile = 0;
+            if ((long long)(++t) * kBN >= s.kv) {
+                t = 0;
+                if (++h == a.c.n_head_kv) {
+                    h = 0;
+                    do {
+                        s = paged::load_seq(a.c, ++b);
+                    } while (s.kv == 0);
                 }
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-                x *= a.scale;
-                if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-                const float lse = *reinterpret_cast<const float*>(a.lse + (size_t)t * a.lse_tok + (size_t)h * a.lse_head);
-                if (lse != -INFINITY) sum += expf(x - lse);
             }
-        if (lane == 0) {
-            const float* in = reinterpret_cast<const float*>(a.acc + (size_t)b * a.a_seq + (size_t)hk * a.a_head);
-            float* out = reinterpret_cast<float*>(a.out + (size_t)b * a.o_seq + (size_t)hk * a.o_head);
-            out[j] = (a.acc ? in[j] : 0.0f) + sum;
+        }
+        n = (int)min((long long)(tiles_of(a, s, t) - tile), left);
+        left -= n;
+        return true;
+    }
+    __device__ bool ends(const WeightArgs& a) const { return tile + n == tiles_of(a, s, t); }
+    // first token of the piece's query tile i, and its columns
+    __device__ int tok0(const WeightArgs& a, int i) const { return (first_tile(a, s, t) + tile + i) * a.tq; }
+    __device__ int cols(const WeightArgs& a, int i) const { return max(0, min(a.tq, s.rows - tok0(a, i))) * a.G; }
+    __device__ int slots() const { return min(kBN, s.kv - t * kBN); }
+};
+
+__device__ void plan(const WeightArgs& a, Bars* B) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.c.batch + kThreads - 1) / kThreads;
+    const int b0 = tid * per, b1 = min(b0 + per, a.c.batch);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += Tiles(a, paged::load_seq(a.c, b)).sum * a.c.n_head_kv;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) B->scan[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) upto += B->scan[w];
+        total += B->scan[w];
+    }
+    const long long n = min((long long)a.n_ctas, total), c = blockIdx.x;
+    const long long lo = c < n ? total * c / n : 0, hi = c < n ? total * (c + 1) / n : 0;
+    if (tid == 0) { B->first = lo; B->count = hi - lo; B->total = total; }
+    if (hi > lo && lo >= upto - mine && lo < upto) {
+        long long r = lo - (upto - mine);
+        for (int b = b0; b < b1; ++b) {
+            const Seq s = paged::load_seq(a.c, b);
+            const Tiles k(a, s);
+            if (r >= k.sum * a.c.n_head_kv) { r -= k.sum * a.c.n_head_kv; continue; }
+            B->b = b;
+            B->h = (int)(r / k.sum);
+            r %= k.sum;
+            int t = (int)min((long long)k.alike, r / k.each);
+            r -= (long long)t * k.each;
+            while (r >= tiles_of(a, s, t)) r -= tiles_of(a, s, t++);
+            B->t = t;
+            B->tile = (int)r;
+            break;
         }
     }
+    __syncthreads();
+}
+
+// 2^x of two values: the exponential unit, or for every kPolyEvery-th pair the FMA pipe.
+__device__ __forceinline__ void exp_pair(int j, uint64_t y, float& p0, float& p1) {
+    if (j % kPolyEvery == kPolyEvery - 1) {
+        exp2_poly5(y, p0, p1);
+    } else {
+        unpair(y, p0, p1);
+        p0 = ex2(p0);
+        p1 = ex2(p1);
+    }
+}
+
+// Sums the weights of tile after tile; thread = slot.
+__device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const float* lse2, float* handed, uint32_t tmem, int warp, int lane) {
+    const int turn = warp >> 2;
+    const int slot = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
+    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    volatile int* abort = &B->abort;
+    uint32_t g = 0, item = 0;
+    Walk w(B);
+    while (w.next(a)) {
+        const bool busy = (warp & 3) * 32 < w.slots();
+        float total = 0.0f;
+        for (int it = 0; it < w.n; ++it, ++g) {
+            if ((int)(g & 1) != turn) continue;
+            const int buf = g % kBufs;
+            const uint32_t par = (g / kBufs) & 1;
+            if (!mbar_wait(smem_u32(&B->s_full[buf]), par, abort, a.c.err)) return;
+            if (!mbar_wait(smem_u32(&B->lse_full[buf]), par, abort, a.c.err)) return;
+            tc_fence_after();
+            const int cols = w.cols(a, it);
+            if (busy && cols > 0) {
+                // columns [from, cols) see this thread's slot
+                const int gap = w.t * kBN + slot - (w.s.kv - w.s.rows) - w.tok0(a, it);
+                const int from = gap > 0 ? min(gap, a.tq) * a.G : 0;
+                const bool cut = __any_sync(~0u, from > 0);
+                const float* lt = lse2 + buf * 128;
+                const uint64_t c22 = pair(c2, c2);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+                for (int i = 0; i < cols; i += 32) {
+                    float x[32];
+                    tmem_ld32(lanes + buf * 128 + i, *reinterpret_cast<uint32_t(*)[32]>(x));
+                    tmem_ld_wait();
+                    if (cut || a.softcap > 0.0f || i + 32 > cols) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float y0 = x[j], y1 = x[j + 1];
+                            if (a.softcap > 0.0f) {
+                                y0 = capped(y0, cap_in, a.softcap);
+                                y1 = capped(y1, cap_in, a.softcap);
+                            }
+                            // a column that does not count may hold anything, and so may its lse2
+                            y0 = ex2(fmaf(y0, c2, -lt[i + j]));
+                            y1 = ex2(fmaf(y1, c2, -lt[i + j + 1]));
+                            y0 = i + j >= from && i + j < cols ? y0 : 0.0f;
+                            y1 = i + j + 1 >= from && i + j + 1 < cols ? y1 : 0.0f;
+                            sum[0] = add2(sum[0], pair(y0, y1));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 L = *reinterpret_cast<const float4*>(lt + i + j);
+                            float p0, p1, p2, p3;
+                            exp_pair(j / 2, fma2(pair(x[j], x[j + 1]), c22, pair(-L.x, -L.y)), p0, p1);
+                            exp_pair(j / 2 + 1, fma2(pair(x[j + 2], x[j + 3]), c22, pair(-L.z, -L.w)), p2, p3);
+                            sum[0] = add2(sum[0], pair(p0, p1));
+                            sum[1] = add2(sum[1], pair(p2, p3));
+                        }
+                    }
+                }
+                float s0, s1;
+                unpair(add2(sum[0], sum[1]), s0, s1);
+                total += s0 + s1;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&B->s_empty[buf]));
+        }
+        // the second warpgroup hands its sums to the first, which writes
+        float* there = handed + (item & 1) * 128;
+        const uint32_t full = smem_u32(&B->hand_full[item & 1]), empty = smem_u32(&B->hand_empty[item & 1]), par = (item >> 1) & 1;
+        if (turn == 1) {
+            if (!mbar_wait(empty, par ^ 1, abort, a.c.err)) return;
+            there[slot] = total;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+        } else {
+            if (!mbar_wait(full, par, abort, a.c.err)) return;
+            total += there[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty);
+            if (w.tile == 0 && w.ends(a)) {
+                if (slot < w.slots()) {
+                    const int j = w.t * kBN + slot;
+                    const float before = a.acc ? ptx::ld_act(reinterpret_cast<const float*>(a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head) + j) : 0.0f;
+                    reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head)[j] = before + total;
+                }
+            } else {
+                a.rec[((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * 128 + slot] = total;
+            }
+        }
+        ++item;
+    }
+}
+
+// The order in which loader and MMA warp go round the ring: slots that hold the K tile at hand
+// are passed over.  A slot's phase is the parity of its uses.
+template <int ST>
+struct Ring {
+    uint32_t next = 0, uses = 0, held = 0;
+    // the next slot and the parity of its use
+    __device__ __forceinline__ void step(uint32_t& st, uint32_t& par) {
+        while ((held >> next) & 1) next = next + 1 == ST ? 0 : next + 1;
+        st = next;
+        par = (uses >> st) & 1;
+        uses ^= 1u << st;
+        next = st + 1 == ST ? 0 : st + 1;
+    }
+};
+
+template <class C>
+__device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t ring, int lane) {
+    volatile int* abort = &B->abort;
+    Ring<C::ST> r;
+    uint32_t begun = 0;                                 // slots with a copy issued
+    bool ok = true;
+    auto slot = [&](uint32_t& st) {
+        uint32_t par;
+        r.step(st, par);
+        if (!mbar_wait(smem_u32(&B->empty[st]), par ^ 1, abort, a.c.err)) {
+            r.uses ^= 1u << st;
+            return false;
+        }
+        begun |= 1u << st;
+        return true;
+    };
+    Walk w(B);
+    while (ok && w.next(a)) {
+        const int n = (w.slots() + a.box - 1) / a.box;
+        const int j = w.t * kBN + lane * a.box;
+        const int page = lane < n ? paged::load_page(a.c, w.b, j / a.c.page) : -1;
+        const int pg = page < 0 ? a.c.n_pages : page;   // outside the map: zeros
+        r.held = 0;
+        uint32_t held = 0;
+        for (int unit = 0; ok && unit < C::UN; ++unit) {
+            uint32_t st;
+            if (!(ok = slot(st))) break;
+            const uint32_t bar = smem_u32(&B->full[st]);
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
+            __syncwarp();
+            if (lane < n) {
+#pragma unroll
+                for (int u = 0; u < C::SUBS; ++u)
+                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, j % a.c.page, w.h, pg);
+            }
+            held |= 1u << st;
+        }
+        r.held = held;
+        for (int it = 0; ok && it < w.n; ++it) {
+            if (w.cols(a, it) == 0) continue;           // a sequence without new tokens
+            const int row = w.s.row0 + w.tok0(a, it);
+            for (int unit = 0; ok && unit < C::QU; ++unit) {
+                uint32_t st;
+                if (!(ok = slot(st))) break;
+                if (lane == 0) {
+                    const uint32_t bar = smem_u32(&B->full[st]);
+                    mbar_expect_tx(bar, (uint32_t)a.tq * a.G * 128 * C::SUBS);
+                    // lo first (see scores)
+                    const CUtensorMap* map = C::HL && unit < C::UN ? &a.mql : &a.mq;
+#pragma unroll
+                    for (int u = 0; u < C::SUBS; ++u)
+                        tma_load_3d(ring + st * C::kUnit + u * C::kSub, map, bar, ((unit % C::UN) * C::SUBS + u) * 64, w.h * a.G, row);
+                }
+            }
+        }
+    }
+    if (!ok) {
+        // the copies already issued land before this CTA's shared memory goes away
+        for (int i = 0; i < C::ST; ++i) {
+            const uint64_t t0 = ptx::global_ns();
+            while ((begun >> i & 1) && !ptx::mbar_try_wait(smem_u32(&B->full[i]), (r.uses >> i & 1) ^ 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+            }
+        }
+    }
+}
+
+// The lse2 of each query tile's rows.
+__device__ __forceinline__ void lse_role(const WeightArgs& a, Bars* B, float* lse2, int lane) {
+    volatile int* abort = &B->abort;
+    uint32_t g = 0;
+    Walk w(B);
+    while (w.next(a)) {
+        for (int it = 0; it < w.n; ++it, ++g) {
+            const int buf = g % kBufs;
+            const int cols = w.cols(a, it), t0 = w.s.row0 + w.tok0(a, it);
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = lane + 32 * i;
+                v[i] = c < cols ? ptx::ld_act(reinterpret_cast<const float*>(a.lse + (size_t)(t0 + c / a.G) * a.lse_tok +
+                                                                             (size_t)(w.h * a.G + c % a.G) * a.lse_head))
+                                : INFINITY;
+                // a row that saw nothing adds nothing
+                v[i] = v[i] == -INFINITY ? INFINITY : v[i] * kLog2e;
+            }
+            if (!mbar_wait(smem_u32(&B->s_empty[buf]), ((g / kBufs) & 1) ^ 1, abort, a.c.err)) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lse2[buf * 128 + lane + 32 * i] = v[i];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&B->lse_full[buf]));
+        }
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void mma_role(const WeightArgs& a, Bars* B, uint32_t ring, uint32_t tmem) {
+    volatile int* abort = &B->abort;
+    Ring<C::ST> r;
+    uint32_t g = 0, last_bar = 0, last_par = 0;
+    bool ok = true;
+    auto take = [&](uint32_t& st) {
+        uint32_t par;
+        r.step(st, par);
+        if (!mbar_wait(smem_u32(&B->full[st]), par, abort, a.c.err)) return false;
+        tc_fence_after();
+        return true;
+    };
+    auto release = [&](uint32_t st) {
+        if (elect_one()) umma_commit(smem_u32(&B->empty[st]));
+        last_bar = smem_u32(&B->empty[st]);
+        last_par = (r.uses >> st & 1) ^ 1;
+    };
+    Walk w(B);
+    while (ok && w.next(a)) {
+        uint32_t ks[C::UN], held = 0;
+        r.held = 0;
+#pragma unroll
+        for (int unit = 0; unit < C::UN; ++unit)
+            if (ok) {
+                ok = take(ks[unit]);
+                held |= 1u << ks[unit];
+            }
+        r.held = held;
+        for (int it = 0; ok && it < w.n; ++it, ++g) {
+            const int buf = g % kBufs;
+            if (!(ok = mbar_wait(smem_u32(&B->s_empty[buf]), ((g / kBufs) & 1) ^ 1, abort, a.c.err))) break;
+            tc_fence_after();
+            const int cols = w.cols(a, it);
+            if (cols > 0) {
+                // as many columns as there are rows (multiples of 16); low products first: the
+                // tensor cores' sums are cut, not rounded, at the sum's own size
+                const uint32_t idesc = uniform(umma_idesc_f16(128, 0) | ((uint32_t)((cols + 15) / 16 * 16 >> 3) << 17));
+                const uint32_t d = uniform(tmem + buf * 128);
+#pragma unroll
+                for (int unit = 0; unit < C::QU; ++unit) {
+                    uint32_t qs;
+                    if (ok) ok = take(qs);
+                    if (!ok) break;
+                    const uint32_t k_at = uniform(ring + ks[unit % C::UN] * C::kUnit), q_at = uniform(ring + qs * C::kUnit);
+                    if (elect_one()) {
+                        const uint64_t k = umma_desc_sw128(k_at), q = umma_desc_sw128(q_at);
+#pragma unroll
+                        for (int i = 0; i < C::DU / 16; ++i) {
+                            const uint32_t o = ((i >> 2) * C::kSub + (i & 3) * 32) >> 4;
+                            umma_f16(d, k + o, q + o, idesc, unit > 0 || i > 0 ? 1u : 0u);
+                        }
+                    }
+                    release(qs);
+                }
+                if (!ok) break;
+            }
+            if (elect_one()) umma_commit(smem_u32(&B->s_full[buf]));
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int unit = 0; unit < C::UN; ++unit) release(ks[unit]);
+    }
+    if (!ok && last_bar && elect_one()) {
+        umma_commit(last_bar);
+        const uint64_t t0 = ptx::global_ns();
+        while (!ptx::mbar_try_wait(last_bar, last_par) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+        }
+    }
+}
+
+// Notes the slot tile that begins in this CTA's share and ends in a later one.
+__device__ __forceinline__ void head_role(const WeightArgs& a, Bars* B) {
+    int4 hd = make_int4(-1, 0, 0, 0);
+    long long at = B->first;
+    Walk w(B);
+    while (w.next(a)) {
+        if (w.tile == 0 && !w.ends(a)) {
+            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of(a, w.s, w.t);
+            hd = make_int4(w.b, w.h, w.t, (int)((end * n - 1) / B->total));
+        }
+        at += w.n;
+    }
+    a.head[blockIdx.x] = hd;
+}
+
+template <class C>
+__global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_constant__ WeightArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t ring = smem_u32(smem);
+    uint8_t* fixed = smem + (size_t)C::ST * C::kUnit;
+    Bars* B = reinterpret_cast<Bars*>(fixed);
+    float* lse2 = reinterpret_cast<float*>(fixed + 512);
+    float* handed = lse2 + kBufs * 128;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::ST; ++i) {
+            mbar_init(smem_u32(&B->full[i]), 1);
+            mbar_init(smem_u32(&B->empty[i]), 1);
+        }
+        for (int i = 0; i < kBufs; ++i) {
+            mbar_init(smem_u32(&B->s_full[i]), 1);
+            mbar_init(smem_u32(&B->s_empty[i]), 4);
+            mbar_init(smem_u32(&B->lse_full[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&B->hand_full[i]), 4);
+            mbar_init(smem_u32(&B->hand_empty[i]), 4);
+        }
+        B->abort = 0;
+        ptx::mbar_init_fence();
+        tma_prefetch_desc(&a.mk);
+        tma_prefetch_desc(&a.mq);
+    }
+    if (warp == kEpiWarps + 1) tmem_alloc(smem_u32(&B->tmem), 512);
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    plan(a, B);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = B->tmem;
+    if (warp < kEpiWarps) sum_role(a, B, lse2, handed, tmem, warp, lane);
+    else if (warp == kEpiWarps) load_role<C>(a, B, ring, lane);
+    else if (warp == kEpiWarps + 1) mma_role<C>(a, B, ring, tmem);
+    else if (warp == kEpiWarps + 2) lse_role(a, B, lse2, lane);
+    else if (lane == 0) head_role(a, B);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kEpiWarps + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Block c: the slot tile begun by CTA c and cut, its records added in order.
+__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ WeightArgs a) {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    const int c = blockIdx.x, slot = threadIdx.x;
+    const int b = paged::ld_int(&a.head[c].x);
+    if (b < 0) return;
+    const int h = paged::ld_int(&a.head[c].y), t = paged::ld_int(&a.head[c].z), last = paged::ld_int(&a.head[c].w);
+    const Seq s = paged::load_seq(a.c, b);
+    const int j = t * kBN + slot;
+    if (j >= s.kv) return;
+    float total = 0.0f;
+    for (int i = c; i <= last; ++i) total += ptx::ld_act(&a.rec[((size_t)i * 2 + (i == c ? 1 : 0)) * 128 + slot]);
+    const float before = a.acc ? ptx::ld_act(reinterpret_cast<const float*>(a.acc + (size_t)b * a.a_seq + (size_t)h * a.a_head) + j) : 0.0f;
+    reinterpret_cast<float*>(a.out + (size_t)b * a.o_seq + (size_t)h * a.o_head)[j] = before + total;
+}
+
+// f32 q rows -> f16 hi + lo, dense [token][head][D].  8 values a thread.
+__global__ void __launch_bounds__(256) split_kernel(const char* q, size_t q_head, size_t q_tok, int n_head, int per_row, int64_t items,
+                                                    uint4* hi, uint4* lo) {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / per_row;
+        const char* p = q + (size_t)(r / n_head) * q_tok + (size_t)(r % n_head) * q_head + (size_t)(i % per_row) * 32;
+        const float4 v0 = ptx::ld_act(reinterpret_cast<const float4*>(p)), v1 = ptx::ld_act(reinterpret_cast<const float4*>(p + 16));
+        uint4 x, y;
+        ptx::split_h2(v0.x, v0.y, x.x, y.x);
+        ptx::split_h2(v0.z, v0.w, x.y, y.y);
+        ptx::split_h2(v1.x, v1.y, x.z, y.z);
+        ptx::split_h2(v1.z, v1.w, x.w, y.w);
+        hi[i] = x;
+        lo[i] = y;
+    }
+}
+
+struct Plan {
+    size_t q, rec, total;
+};
+Plan make_plan(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, int ctas) {
+    Plan p{};
+    p.q = d->type == MLZC_TYPE_F32 ? (size_t)cache->n_tokens * d->n_head_q * cache->head_dim * 2 : 0;
+    p.rec = (size_t)ctas * 2 * 128 * 4;
+    p.total = 2 * p.q + p.rec + (size_t)ctas * 16;
+    return p;
+}
+
+template <class C>
+int launch(const WeightArgs& a, const DeviceCtx* c, cudaStream_t s) {
+    static bool set[64] = {};
+    const int dev = c->device < 64 ? c->device : 63;
+    if (!set[dev] || c->device >= 64) {
+        MLZC_CUDA_TRY(cudaFuncSetAttribute(weights_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+        set[dev] = true;
+    }
+    MLZC_CUDA_TRY(launch_pdl(weights_kernel<C>, dim3(a.n_ctas), dim3(kThreads), C::kSmem, s, a));
+    MLZC_CUDA_TRY(cudaGetLastError());
+    MLZC_CUDA_TRY(launch_pdl(merge_kernel, dim3(a.n_ctas), dim3(128), 0, s, a));
+    MLZC_CUDA_TRY(cudaGetLastError());
+    count_launch(2);
+    return MLZC_OK;
 }
 
 int check_table(const char* what, const void* p, const size_t* nb, int64_t heads, int64_t batch, size_t row) {
@@ -87,7 +622,12 @@ extern "C" int mlzc_paged_weights_workspace_bytes(const mlzc_paged_cache* cache,
                                                   size_t* out_bytes) {
     if (!out_bytes) return fail(MLZC_ERR_INVALID, "paged weights: null out_bytes");
     *out_bytes = 0;
-    return paged::check_attn(cache, d, true);
+    const int st = paged::check_attn(cache, d, true);
+    if (st != MLZC_OK) return st;
+    DeviceCtx* c = current_ctx();
+    if (!c) return MLZC_ERR_CUDA;
+    *out_bytes = make_plan(cache, d, c->sm_count).total;
+    return MLZC_OK;
 }
 
 extern "C" int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, const float* acc,
@@ -101,29 +641,51 @@ extern "C" int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_
     if (st != MLZC_OK) return st;
     if (acc == out && (acc_nb[1] != out_nb[1] || acc_nb[2] != out_nb[2]))
         return fail(MLZC_ERR_INVALID, "paged weights: acc and out in place with other strides");
-    if (cache->batch_size > 65535) return fail(MLZC_ERR_UNSUPPORTED, "paged weights: batch_size above 65535");
     DeviceCtx* c = current_ctx();
     if (!c) return MLZC_ERR_CUDA;
+    const Plan p = make_plan(cache, d, c->sm_count);
+    if (!workspace || workspace_bytes < p.total)
+        return fail(MLZC_ERR_NOMEM, "paged weights: workspace of %zu bytes needed, %zu given", p.total, workspace_bytes);
+    if ((uintptr_t)workspace % 16) return fail(MLZC_ERR_INVALID, "paged weights: workspace not 16-byte aligned");
     WeightArgs a{};
     st = paged::make_view(cache, true, c, &a.c);
     if (st != MLZC_OK) return st;
-    a.q = static_cast<const char*>(d->q);
-    a.q_head = d->q_nb[1]; a.q_tok = d->q_nb[2];
+    char* ws = static_cast<char*>(workspace);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t T = cache->n_tokens, H = d->n_head_q, D = cache->head_dim;
+    const bool f32 = d->type == MLZC_TYPE_F32;
+    a.G = (int)(H / cache->n_head_kv);
+    a.tq = 128 / a.G;
+    a.box = std::gcd(cache->page_size, kBN);
+    if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
+    if (T > 0) {
+        // checked after every argument: from here on work is issued
+        if (f32) {
+            if ((st = paged::encode_rows(&a.mq, ws, D, H, T, D * 2, H * D * 2, a.G, a.tq)) != MLZC_OK) return st;
+            if ((st = paged::encode_rows(&a.mql, ws + p.q, D, H, T, D * 2, H * D * 2, a.G, a.tq)) != MLZC_OK) return st;
+            const int64_t items = T * H * (D / 8);
+            const unsigned grid = (unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)c->sm_count * 8);
+            MLZC_CUDA_TRY(launch_pdl(split_kernel, dim3(grid), dim3(256), 0, s, static_cast<const char*>(d->q), d->q_nb[1], d->q_nb[2],
+                                     (int)H, (int)(D / 8), items, reinterpret_cast<uint4*>(ws), reinterpret_cast<uint4*>(ws + p.q)));
+            MLZC_CUDA_TRY(cudaGetLastError());
+            count_launch();
+        } else if ((st = paged::encode_rows(&a.mq, d->q, D, H, T, d->q_nb[1], d->q_nb[2], a.G, a.tq)) != MLZC_OK) {
+            return st;
+        }
+    } else {
+        a.mq = a.mk;   // not read
+    }
     a.lse = reinterpret_cast<const char*>(d->lse);
     a.lse_head = d->lse_nb[0]; a.lse_tok = d->lse_nb[1];
     a.acc = reinterpret_cast<const char*>(acc);
     a.out = reinterpret_cast<char*>(out);
     if (acc) { a.a_head = acc_nb[1]; a.a_seq = acc_nb[2]; }
     a.o_head = out_nb[1]; a.o_seq = out_nb[2];
-    a.n_head_q = (int)d->n_head_q;
-    a.f32 = d->type == MLZC_TYPE_F32;
     a.scale = d->scale;
     a.softcap = (d->mode & MLZC_FA_MODE_SOFTCAP) ? d->logit_softcap : 0.0f;
-    const int D = (int)cache->head_dim;
-    const unsigned gx = (unsigned)std::min(1024, (a.c.cap + kWarps - 1) / kWarps);
-    MLZC_CUDA_TRY(launch_pdl(D == 64 ? weights_kernel<64> : (D == 128 ? weights_kernel<128> : weights_kernel<256>),
-                             dim3(gx, a.c.n_head_kv, a.c.batch), dim3(kWarps * 32), 0, static_cast<cudaStream_t>(stream), a));
-    MLZC_CUDA_TRY(cudaGetLastError());
-    count_launch();
-    return MLZC_OK;
+    a.n_ctas = c->sm_count;
+    a.rec = reinterpret_cast<float*>(ws + 2 * p.q);
+    a.head = reinterpret_cast<int4*>(ws + 2 * p.q + p.rec);
+    if (f32) return D == 64 ? launch<Cfg<64, true>>(a, c, s) : (D == 128 ? launch<Cfg<128, true>>(a, c, s) : launch<Cfg<256, true>>(a, c, s));
+    return D == 64 ? launch<Cfg<64, false>>(a, c, s) : (D == 128 ? launch<Cfg<128, false>>(a, c, s) : launch<Cfg<256, false>>(a, c, s));
 }

@@ -197,6 +197,20 @@ def test_weights(dev, q_len, kv_len, D, dtype):
     _check_weights(ref.make(dev, q_len, kv_len, D=D, dtype=dtype, seed=sum(kv_len), tail=2))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weights_many_query_tiles(dev, D, dtype):
+    """Slot tiles with far more query tiles than a CTA holds at a time, and cut between CTAs."""
+    _check_weights(ref.make(dev, [1900, 900], [2100, 900], hkv=2, group=8, D=D, dtype=dtype, seed=33))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attn_many_tiles(dev, D, dtype):
+    """Query tiles over far more slot tiles than the ring holds, several to a CTA, some cut."""
+    _check_attn(ref.make(dev, [1700, 1300], [9000, 1300], hkv=2, group=4, D=D, dtype=dtype, seed=34))
+
+
 @pytest.mark.parametrize("hkv,group", [(1, 1), (2, 3), (1, 7), (2, 33), (1, 100), (1, 128)])
 def test_weights_head_groups(dev, hkv, group):
     _check_weights(ref.make(dev, [3, 1, 17], [200, 65, 17], hkv=hkv, group=group, D=64, seed=group))
