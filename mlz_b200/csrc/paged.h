@@ -10,6 +10,25 @@
 namespace mlzc {
 namespace paged {
 
+// Division of 0 <= n < 2^31 by a divisor known at the call: q = n * mul / 2^shift (mul the
+// reciprocal rounded up, exact for all such n), instead of a division's 20 instructions.
+struct Div {
+    uint32_t d, mul, shift;
+    void set(uint32_t x) {
+        d = x;
+        shift = 0;
+        while ((1ull << shift) < x) ++shift;
+        mul = x == 1 ? 0 : (uint32_t)(((1ull << 32) * ((1ull << shift) - x)) / x + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int quot(int n) const {
+        const uint32_t hi = __umulhi((uint32_t)n, mul);
+        return (int)((hi + (uint32_t)n) >> shift);
+    }
+    __device__ __forceinline__ int rem(int n) const { return n - quot(n) * (int)d; }
+#endif
+};
+
 // Pools, block table and lengths of one call.  Strides in bytes.
 struct View {
     char* k;
@@ -20,6 +39,7 @@ struct View {
     const int* kv_len;
     const int* q_start;
     int page, max_pages, n_pages, n_head_kv, batch, n_tokens, cap;   // cap = max_pages * page
+    Div by_page;
     unsigned int* err;
 };
 

@@ -84,10 +84,10 @@ struct AttnArgs {
 
 constexpr int BN = 128;        // slots a tile
 
-template <int D_, int NS_, bool HL_>
+template <int D_, int NS_, bool HL_, bool CAP_>
 struct Cfg {
     static constexpr int D = D_, NS = NS_;
-    static constexpr bool HL = HL_;
+    static constexpr bool HL = HL_, CAP = CAP_;           // f32 queries (hi + lo); scores are capped
     // dims of a ring unit (a K or V tile is UN units); beside f32 queries of 256 dims (128 KB)
     // half units leave a ring of five
     static constexpr int DU = D == 64 || (HL && D == 256) ? 64 : 128;
@@ -304,8 +304,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
     const Row q(a, (warp & 3) * 32 + lane);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t o_col = lanes + C::kOCol + slot * D;
-    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
-    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
+    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
     const float rise = kRescale / c2;
     volatile int* abort = &B->abort;
     uint32_t g = 0, piece = 0;
@@ -327,7 +327,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                 for (int i = 0; i < BN / 32; ++i)
                     tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                 tmem_ld_wait();
-                if (a.softcap > 0.0f) {
+                if (C::CAP) {
 #pragma unroll
                     for (int i = 0; i < BN; ++i) x[i] = capped(x[i], cap_in, a.softcap);
                 }
@@ -428,8 +428,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
     const int turn = warp >> 2;
     const Row q(a, (warp & 3) * 32 + lane);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
-    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
+    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
     volatile int* abort = &B->abort;
     uint32_t g = 0;
     Walk<C> w(B);
@@ -470,7 +470,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     tmem_st16(s_col + i + 16, lo);
                 };
                 auto clip = [&](float x, int i) {
-                    if (a.softcap > 0.0f) x = capped(x, cap_in, a.softcap);
+                    if (C::CAP) x = capped(x, cap_in, a.softcap);
                     return i > limit ? -INFINITY : x;
                 };
                 if constexpr (C::kHold) {
@@ -479,7 +479,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     for (int i = 0; i < BN / 32; ++i)
                         tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                     tmem_ld_wait();
-                    if (a.softcap > 0.0f || cut) {
+                    if (C::CAP || cut) {
 #pragma unroll
                         for (int i = 0; i < BN; ++i) x[i] = clip(x[i], i);
                     }
@@ -494,7 +494,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                         uint32_t r[32];
                         tmem_ld32(s_col + i, r);
                         tmem_ld_wait();
-                        if (a.softcap > 0.0f || cut) {
+                        if (C::CAP || cut) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(clip(__uint_as_float(r[j]), i + j));
                             tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));
@@ -600,11 +600,11 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t r
     // the page of box `lane` of slot tile i
     auto page_of = [&](const Walk<C>& w, int i) {
         const int j = i * BN + lane * a.box;
-        return lane < boxes && lane * a.box < tile_rows(a, w, i) ? paged::load_page(a.c, w.b, j / a.c.page) : -1;
+        return lane < boxes && lane * a.box < tile_rows(a, w, i) ? paged::load_page(a.c, w.b, a.c.by_page.quot(j)) : -1;
     };
     auto load = [&](const Walk<C>& w, int i, int page, const CUtensorMap* map) {
         const int n = (tile_rows(a, w, i) + a.box - 1) / a.box;
-        const int row = (i * BN + lane * a.box) % a.c.page;
+        const int row = a.c.by_page.rem(i * BN + lane * a.box);
         // a page outside the pools is a coordinate outside the map, which reads as zeros
         const int pg = page < 0 ? a.c.n_pages : page;
 #pragma unroll
@@ -1097,8 +1097,14 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     a.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + p.rec);
     a.head = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.rec + p.ml);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int D = (int)cache->head_dim;
-    if (f32) return D == 64 ? launch<Cfg<64, 1, true>>(a, c, s) : (D == 128 ? launch<Cfg<128, 1, true>>(a, c, s) : launch<Cfg<256, 1, true>>(a, c, s));
-    if (p.ns == 2) return D == 64 ? launch<Cfg<64, 2, false>>(a, c, s) : launch<Cfg<128, 2, false>>(a, c, s);
-    return D == 64 ? launch<Cfg<64, 1, false>>(a, c, s) : (D == 128 ? launch<Cfg<128, 1, false>>(a, c, s) : launch<Cfg<256, 1, false>>(a, c, s));
+    const bool cap = a.softcap > 0.0f;
+#define MLZC_LAUNCH(DIM, NS)                                                                                            \
+    return f32 ? (cap ? launch<Cfg<DIM, 1, true, true>>(a, c, s) : launch<Cfg<DIM, 1, true, false>>(a, c, s))           \
+               : (cap ? launch<Cfg<DIM, NS, false, true>>(a, c, s) : launch<Cfg<DIM, NS, false, false>>(a, c, s))
+    if (cache->head_dim == 256) MLZC_LAUNCH(256, 1);
+    if (p.ns == 2 && cache->head_dim == 128) MLZC_LAUNCH(128, 2);
+    if (p.ns == 2) MLZC_LAUNCH(64, 2);
+    if (cache->head_dim == 128) MLZC_LAUNCH(128, 1);
+    MLZC_LAUNCH(64, 1);
+#undef MLZC_LAUNCH
 }

@@ -77,6 +77,7 @@ int make_view(const mlzc_paged_cache* cache, bool rows, const DeviceCtx* ctx, Vi
     v.batch = (int)cache->batch_size;
     v.n_tokens = rows ? (int)cache->n_tokens : 0;
     v.cap = (int)(cache->max_pages * cache->page_size);
+    v.by_page.set((uint32_t)v.page);
     v.err = ctx ? ctx->err : nullptr;
     return MLZC_OK;
 }

@@ -61,15 +61,17 @@ struct WeightArgs {
     char* out;
     size_t lse_head, lse_tok, a_head, a_seq, o_head, o_seq;
     int G, tq, box, n_ctas;
+    paged::Div by_tq, by_g;
     float scale, softcap;
     float* rec;                        // [cta][2][128]: 0 continues a cut slot tile, 1 begins one
     int4* head;                        // [cta]: sequence (-1: none), kv head, slot tile, last CTA of the tile begun
 };
 
-template <int D_, bool HL_>
+template <int D_, bool HL_, bool CAP_>
 struct Cfg {
     static constexpr int D = D_;
-    static constexpr bool HL = HL_;
+    static constexpr bool HL = HL_;                   // f32 queries: hi + lo
+    static constexpr bool CAP = CAP_;                 // scores are capped
     static constexpr int DU = D < 128 ? D : 128;      // dims of a ring unit (128 rows)
     static constexpr int UN = D / DU;
     static constexpr int SUBS = DU / 64;
@@ -95,10 +97,10 @@ static_assert(sizeof(Bars) <= 512, "barriers");
 // Query tiles of slot tile t: from the first one with a row that sees slot 128 t on; one at
 // least, so that every slot below kv_len is written.
 __device__ __forceinline__ int first_tile(const WeightArgs& a, const Seq& s, int t) {
-    return max(0, t * kBN - (s.kv - s.rows)) / a.tq;
+    return a.by_tq.quot(max(0, t * kBN - (s.kv - s.rows)));
 }
 __device__ __forceinline__ int tiles_of(const WeightArgs& a, const Seq& s, int t) {
-    return max(1, (s.rows + a.tq - 1) / a.tq - first_tile(a, s, t));
+    return max(1, a.by_tq.quot(s.rows + a.tq - 1) - first_tile(a, s, t));
 }
 // The sum of tiles_of over a sequence's slot tiles: all alike up to the chunk's own slots.
 struct Tiles {
@@ -203,18 +205,41 @@ __device__ __forceinline__ void exp_pair(int j, uint64_t y, float& p0, float& p1
 }
 
 // Sums the weights of tile after tile; thread = slot.
+template <class C>
 __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const float* lse2, float* handed, uint32_t tmem, int warp, int lane) {
     const int turn = warp >> 2;
     const int slot = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const float c2 = a.softcap > 0.0f ? kLog2e : a.scale * kLog2e;
-    const float cap_in = a.softcap > 0.0f ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
+    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
     volatile int* abort = &B->abort;
+    // weights of columns i, i + 1 where they count: outside [from, cols) a score may hold anything
+    auto some = [&](const float* x, const float* lt, int i, int from, int cols) {
+        float y0 = x[0], y1 = x[1];
+        if (C::CAP) {
+            y0 = capped(y0, cap_in, a.softcap);
+            y1 = capped(y1, cap_in, a.softcap);
+        }
+        y0 = ex2(fmaf(y0, c2, -lt[i]));
+        y1 = ex2(fmaf(y1, c2, -lt[i + 1]));
+        return pair(i >= from && i < cols ? y0 : 0.0f, i + 1 >= from && i + 1 < cols ? y1 : 0.0f);
+    };
     uint32_t g = 0, item = 0;
     Walk w(B);
     while (w.next(a)) {
-        const bool busy = (warp & 3) * 32 < w.slots();
-        float total = 0.0f;
+        // a piece of one tile (decode) is all of one warpgroup's; of a longer one the second
+        // warpgroup hands its sums to the first, which writes
+        const bool alone = w.n == 1;
+        if (alone && (int)(g & 1) != turn) {
+            ++g;
+            continue;
+        }
+        const bool writes = alone || turn == 0, whole = w.tile == 0 && w.ends(a);
+        const bool busy = (warp & 3) * 32 < w.slots(), real = slot < w.slots();
+        const int j = w.t * kBN + slot;
+        float before = 0.0f, total = 0.0f;
+        if (writes && whole && real && a.acc)
+            before = ptx::ld_act(reinterpret_cast<const float*>(a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head) + j);
         for (int it = 0; it < w.n; ++it, ++g) {
             if ((int)(g & 1) != turn) continue;
             const int buf = g % kBufs;
@@ -225,39 +250,37 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
             const int cols = w.cols(a, it);
             if (busy && cols > 0) {
                 // columns [from, cols) see this thread's slot
-                const int gap = w.t * kBN + slot - (w.s.kv - w.s.rows) - w.tok0(a, it);
+                const int gap = j - (w.s.kv - w.s.rows) - w.tok0(a, it);
                 const int from = gap > 0 ? min(gap, a.tq) * a.G : 0;
-                const bool cut = __any_sync(~0u, from > 0);
                 const float* lt = lse2 + buf * 128;
-                const uint64_t c22 = pair(c2, c2);
+                const uint32_t s_col = lanes + buf * 128;
                 uint64_t sum[2] = {0, 0};
+                if (C::CAP || cols <= 96 || __any_sync(~0u, from > 0)) {
 #pragma unroll 1
-                for (int i = 0; i < cols; i += 32) {
-                    float x[32];
-                    tmem_ld32(lanes + buf * 128 + i, *reinterpret_cast<uint32_t(*)[32]>(x));
+                    for (int i = 0; i < cols; i += 32) {
+                        float x[32];
+                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(x));
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
+                    }
+                } else {
+                    const uint64_t c22 = pair(c2, c2);
+                    float x[128];
+#pragma unroll
+                    for (int i = 0; i < 128; i += 32)
+                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i));
                     tmem_ld_wait();
-                    if (cut || a.softcap > 0.0f || i + 32 > cols) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float y0 = x[j], y1 = x[j + 1];
-                            if (a.softcap > 0.0f) {
-                                y0 = capped(y0, cap_in, a.softcap);
-                                y1 = capped(y1, cap_in, a.softcap);
-                            }
-                            // a column that does not count may hold anything, and so may its lse2
-                            y0 = ex2(fmaf(y0, c2, -lt[i + j]));
-                            y1 = ex2(fmaf(y1, c2, -lt[i + j + 1]));
-                            y0 = i + j >= from && i + j < cols ? y0 : 0.0f;
-                            y1 = i + j + 1 >= from && i + j + 1 < cols ? y1 : 0.0f;
-                            sum[0] = add2(sum[0], pair(y0, y1));
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 L = *reinterpret_cast<const float4*>(lt + i + j);
+                    for (int i = 0; i < 128; i += 4) {
+                        if (i >= 96 && i + 4 > cols) {       // 128 / G is no whole number
+                            sum[0] = add2(sum[0], some(x + i, lt, i, 0, cols));
+                            sum[1] = add2(sum[1], some(x + i + 2, lt, i + 2, 0, cols));
+                        } else {
+                            const float4 L = *reinterpret_cast<const float4*>(lt + i);
                             float p0, p1, p2, p3;
-                            exp_pair(j / 2, fma2(pair(x[j], x[j + 1]), c22, pair(-L.x, -L.y)), p0, p1);
-                            exp_pair(j / 2 + 1, fma2(pair(x[j + 2], x[j + 3]), c22, pair(-L.z, -L.w)), p2, p3);
+                            exp_pair(i / 2, fma2(pair(x[i], x[i + 1]), c22, pair(-L.x, -L.y)), p0, p1);
+                            exp_pair(i / 2 + 1, fma2(pair(x[i + 2], x[i + 3]), c22, pair(-L.z, -L.w)), p2, p3);
                             sum[0] = add2(sum[0], pair(p0, p1));
                             sum[1] = add2(sum[1], pair(p2, p3));
                         }
@@ -271,30 +294,28 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&B->s_empty[buf]));
         }
-        // the second warpgroup hands its sums to the first, which writes
-        float* there = handed + (item & 1) * 128;
-        const uint32_t full = smem_u32(&B->hand_full[item & 1]), empty = smem_u32(&B->hand_empty[item & 1]), par = (item >> 1) & 1;
-        if (turn == 1) {
-            if (!mbar_wait(empty, par ^ 1, abort, a.c.err)) return;
-            there[slot] = total;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full);
-        } else {
-            if (!mbar_wait(full, par, abort, a.c.err)) return;
-            total += there[slot];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty);
-            if (w.tile == 0 && w.ends(a)) {
-                if (slot < w.slots()) {
-                    const int j = w.t * kBN + slot;
-                    const float before = a.acc ? ptx::ld_act(reinterpret_cast<const float*>(a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head) + j) : 0.0f;
-                    reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head)[j] = before + total;
-                }
+        if (!alone) {
+            float* there = handed + (item & 1) * 128;
+            const uint32_t full = smem_u32(&B->hand_full[item & 1]), empty = smem_u32(&B->hand_empty[item & 1]), par = (item >> 1) & 1;
+            ++item;
+            if (turn == 1) {
+                if (!mbar_wait(empty, par ^ 1, abort, a.c.err)) return;
+                there[slot] = total;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full);
             } else {
-                a.rec[((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * 128 + slot] = total;
+                if (!mbar_wait(full, par, abort, a.c.err)) return;
+                total += there[slot];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty);
             }
         }
-        ++item;
+        if (!writes) continue;
+        if (whole) {
+            if (real) reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head)[j] = before + total;
+        } else {
+            a.rec[((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * 128 + slot] = total;
+        }
     }
 }
 
@@ -329,11 +350,16 @@ __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t
         begun |= 1u << st;
         return true;
     };
-    Walk w(B);
-    while (ok && w.next(a)) {
+    // the page of this lane's box, one slot tile ahead
+    auto page_of = [&](const Walk& w) {
+        return lane * a.box < w.slots() ? paged::load_page(a.c, w.b, a.c.by_page.quot(w.t * kBN + lane * a.box)) : -1;
+    };
+    Walk w(B), ahead(B);
+    int page = ahead.next(a) ? page_of(ahead) : -1, next_page = -1;
+    for (; ok && w.next(a); page = next_page) {
+        if (ahead.next(a)) next_page = page_of(ahead);
         const int n = (w.slots() + a.box - 1) / a.box;
         const int j = w.t * kBN + lane * a.box;
-        const int page = lane < n ? paged::load_page(a.c, w.b, j / a.c.page) : -1;
         const int pg = page < 0 ? a.c.n_pages : page;   // outside the map: zeros
         r.held = 0;
         uint32_t held = 0;
@@ -346,7 +372,7 @@ __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t
             if (lane < n) {
 #pragma unroll
                 for (int u = 0; u < C::SUBS; ++u)
-                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, j % a.c.page, w.h, pg);
+                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, a.c.by_page.rem(j), w.h, pg);
             }
             held |= 1u << st;
         }
@@ -379,21 +405,23 @@ __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t
     }
 }
 
-// The lse2 of each query tile's rows.
-__device__ __forceinline__ void lse_role(const WeightArgs& a, Bars* B, float* lse2, int lane) {
+// The lse2 of each query tile's rows; two warps take turns, so that one's loads are under way
+// while the other waits.
+__device__ __forceinline__ void lse_role(const WeightArgs& a, Bars* B, float* lse2, int turn, int lane) {
     volatile int* abort = &B->abort;
     uint32_t g = 0;
     Walk w(B);
     while (w.next(a)) {
         for (int it = 0; it < w.n; ++it, ++g) {
+            if ((int)(g & 1) != turn) continue;
             const int buf = g % kBufs;
             const int cols = w.cols(a, it), t0 = w.s.row0 + w.tok0(a, it);
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = lane + 32 * i;
-                v[i] = c < cols ? ptx::ld_act(reinterpret_cast<const float*>(a.lse + (size_t)(t0 + c / a.G) * a.lse_tok +
-                                                                             (size_t)(w.h * a.G + c % a.G) * a.lse_head))
+                v[i] = c < cols ? ptx::ld_act(reinterpret_cast<const float*>(a.lse + (size_t)(t0 + a.by_g.quot(c)) * a.lse_tok +
+                                                                             (size_t)(w.h * a.G + a.by_g.rem(c)) * a.lse_head))
                                 : INFINITY;
                 // a row that saw nothing adds nothing
                 v[i] = v[i] == -INFINITY ? INFINITY : v[i] * kLog2e;
@@ -530,11 +558,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B->tmem;
-    if (warp < kEpiWarps) sum_role(a, B, lse2, handed, tmem, warp, lane);
+    if (warp < kEpiWarps) sum_role<C>(a, B, lse2, handed, tmem, warp, lane);
     else if (warp == kEpiWarps) load_role<C>(a, B, ring, lane);
     else if (warp == kEpiWarps + 1) mma_role<C>(a, B, ring, tmem);
-    else if (warp == kEpiWarps + 2) lse_role(a, B, lse2, lane);
-    else if (lane == 0) head_role(a, B);
+    else {
+        lse_role(a, B, lse2, warp - kEpiWarps - 2, lane);
+        if (warp == kEpiWarps + 3 && lane == 0) head_role(a, B);
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == kEpiWarps + 1) {
@@ -656,6 +686,8 @@ extern "C" int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_
     const bool f32 = d->type == MLZC_TYPE_F32;
     a.G = (int)(H / cache->n_head_kv);
     a.tq = 128 / a.G;
+    a.by_tq.set((uint32_t)a.tq);
+    a.by_g.set((uint32_t)a.G);
     a.box = std::gcd(cache->page_size, kBN);
     if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
     if (T > 0) {
@@ -686,6 +718,12 @@ extern "C" int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_
     a.n_ctas = c->sm_count;
     a.rec = reinterpret_cast<float*>(ws + 2 * p.q);
     a.head = reinterpret_cast<int4*>(ws + 2 * p.q + p.rec);
-    if (f32) return D == 64 ? launch<Cfg<64, true>>(a, c, s) : (D == 128 ? launch<Cfg<128, true>>(a, c, s) : launch<Cfg<256, true>>(a, c, s));
-    return D == 64 ? launch<Cfg<64, false>>(a, c, s) : (D == 128 ? launch<Cfg<128, false>>(a, c, s) : launch<Cfg<256, false>>(a, c, s));
+    const bool cap = a.softcap > 0.0f;
+#define MLZC_LAUNCH(DIM)                                                                                                \
+    return f32 ? (cap ? launch<Cfg<DIM, true, true>>(a, c, s) : launch<Cfg<DIM, true, false>>(a, c, s))                 \
+               : (cap ? launch<Cfg<DIM, false, true>>(a, c, s) : launch<Cfg<DIM, false, false>>(a, c, s))
+    if (D == 64) MLZC_LAUNCH(64);
+    if (D == 128) MLZC_LAUNCH(128);
+    MLZC_LAUNCH(256);
+#undef MLZC_LAUNCH
 }
