@@ -13,7 +13,6 @@ from ._lib import (EXPORTS, FA_MODE_ALIBI, FA_MODE_GQA_BATCH, FA_MODE_SOFTCAP, L
                    UNIQUE_ID_BYTES, FaDesc, MlzcError, TensorView, check, get_launch_overlap,
                    last_error, launch_count, lib, set_launch_overlap)
 from ._lib import DEVERR_BAD_INDEX, ROPE_ADJACENT, ROPE_HALVES
-from .paged import PagedCache, paged_attn, paged_attn_workspace_bytes, paged_evict, paged_store, paged_weights
 from .ops import (Comm, Weight, device_errors, flash_attn_dispatch, flash_attn_dispatch_quant,
                   flash_attn_workspace_bytes,
                   ggml_simd_try_flash_attn, ggml_simd_try_mul_mat, init, make_fa_desc, mul_mat,
@@ -31,3 +30,14 @@ __all__ = [
     "weight_type_of", "PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store",
     "paged_weights", "DEVERR_BAD_INDEX", "ROPE_ADJACENT", "ROPE_HALVES",
 ]
+
+_PAGED = ("PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store", "paged_weights")
+
+
+def __getattr__(name):
+    """The paged-cache calls, loaded (with torch) by the first use of one."""
+    if name not in _PAGED:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import paged
+    globals().update({n: getattr(paged, n) for n in _PAGED})
+    return globals()[name]

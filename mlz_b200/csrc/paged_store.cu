@@ -6,7 +6,7 @@
 // The angle is carried as a fraction of a turn in 64-bit fixed point.  With
 // F_j = freq_j / 2 pi * 2^64 (computed once on the host in extended precision and passed as a
 // kernel argument), pos * F_j modulo 2^64 IS the fraction: the integer product drops whole
-// turns exactly, so a position of two million is as exact as position two (f32 angles of far
+// turns exactly, so a position of two million is nearly as exact as position two (f32 angles of far
 // positions lose all their bits).  The top 32 bits go to sincospi.
 //
 // Bound by HBM (each row read once, written once; 12 bytes per k or v value in f32, 8 per q
@@ -174,11 +174,16 @@ extern "C" int mlzc_paged_store_dev(const mlzc_paged_cache* cache, const mlzc_pa
                       (d->n_axes > 1 && d->positions_nb < (size_t)T * 4)))
             return fail(MLZC_ERR_INVALID, "paged store: positions null, misaligned or overlapping");
         const long double two_pi = 6.283185307179586476925286766559005768L;
+        // powers of the step between pairs from two short tables (a dozen roundings of 2^-64)
+        const long double step = powl((long double)d->freq_base, -2.0L / d->n_rot);
+        long double fine[8] = {1.0L}, coarse = (long double)d->freq_scale / two_pi;
+        for (int i = 1; i < 8; ++i) fine[i] = fine[i - 1] * step;
         int j = 0;
         for (int ax = 0; ax < d->n_axes; ++ax)
             for (int i = 0; i < d->sections[ax]; ++i, ++j) {
+                if (j > 0 && j % 8 == 0) coarse *= fine[7] * step;
                 a.axis[j] = (uint8_t)ax;
-                const long double turns = (long double)d->freq_scale * powl((long double)d->freq_base, -2.0L * j / d->n_rot) / two_pi;
+                const long double turns = coarse * fine[j % 8];
                 a.turn[j] = (uint64_t)ldexpl(turns - floorl(turns), 64);   // whole turns a position step drop out
             }
     }

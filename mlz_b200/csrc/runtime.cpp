@@ -77,6 +77,7 @@ int cuda_fail(cudaError_t e, const char* what) {
 
 DeviceCtx* device_ctx(int device) {
     std::lock_guard<std::mutex> lk(g_ctx_mu);
+    if (device >= 0 && device < (int)g_ctx.size() && g_ctx[device]) return g_ctx[device].get();
     int ndev = 0;
     cudaError_t e = cudaGetDeviceCount(&ndev);
     if (e != cudaSuccess) { cuda_fail(e, "cudaGetDeviceCount"); return nullptr; }

@@ -13,27 +13,37 @@ one contiguous cache (src/simd/flash_attention.h:65-114).
 from __future__ import annotations
 
 import ctypes as C
+import struct
+
+import torch
 
 from ._lib import (FA_MODE_SOFTCAP, ROPE_ADJACENT, ROPE_HALVES, TYPE_F16, TYPE_F32, PagedAttnDesc, PagedCacheDesc,
                    PagedEvictDesc, PagedStoreDesc, check, lib)
 
+_F32, _F16, _I32, _U8 = torch.float32, torch.float16, torch.int32, torch.uint8
+# the descriptors, packed in one go (a field by field fill costs more than a small kernel runs)
+_ATTN = struct.Struct("iIqff2Q3Q3QQ2Q")
+_STORE = struct.Struct("8i2fQQq4Q12Q")
+_EVICT = struct.Struct("3q2Q6QQ3QQ")
+assert [x.size for x in (_ATTN, _STORE, _EVICT)] == [C.sizeof(x) for x in (PagedAttnDesc, PagedStoreDesc, PagedEvictDesc)]
 
-def _torch():
-    import torch
-    return torch
+
+# the current stream's handle by device index (current_stream builds a Stream object around it)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class _Launch:
-    """The device and stream of one call, and the workspaces that it takes there: memory that
-    torch hands to nobody else until the call's stream is past it."""
+    """The device and stream of one call, and where its outputs and workspaces come from: torch
+    hands their memory to nobody else until the call's stream is past it."""
+
+    __slots__ = ("device", "other", "given", "handle")
 
     def __init__(self, device, stream):
-        torch = _torch()
         self.device = device
         self.other = torch.cuda.current_device() != device.index
         self.given = None
         if stream is None:
-            self.handle = torch.cuda.current_stream(device).cuda_stream
+            self.handle = _raw_stream(device.index)
         elif hasattr(stream, "cuda_stream"):
             self.given, self.handle = stream, stream.cuda_stream
         else:
@@ -41,7 +51,6 @@ class _Launch:
             self.given = torch.cuda.ExternalStream(self.handle, device=device) if self.handle else torch.cuda.default_stream(device)
 
     def empty(self, shape, dtype):
-        torch = _torch()
         if self.given is None:
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(self.given):
@@ -49,15 +58,16 @@ class _Launch:
 
     def run(self, f, *args):
         if self.other:
-            with _torch().cuda.device(self.device):
+            with torch.cuda.device(self.device):
                 return check(f(*args))
         return check(f(*args))
 
 
 def _rows(what, t, cache, heads, dtype=None):
     """Checks a packed (tokens, heads, head_dim) tensor; its byte strides element, head, token."""
-    if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected (tokens, {heads or 'heads'}, {cache.head_dim})")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected (tokens, {heads or 'heads'}, {cache.head_dim})")
     if t.device != cache.device:
         raise ValueError(f"{what} is on {t.device}, the cache on {cache.device}")
     if dtype is not None and t.dtype != dtype:
@@ -68,22 +78,22 @@ def _rows(what, t, cache, heads, dtype=None):
 
 
 def _type_of(what, t):
-    torch = _torch()
-    if t.dtype == torch.float32:
+    if t.dtype == _F32:
         return TYPE_F32
-    if t.dtype == torch.float16:
+    if t.dtype == _F16:
         return TYPE_F16
     raise TypeError(f"{what}: {t.dtype}, expected float32 or float16")
 
 
 def _table(what, t, cache, last, dtype):
     """Checks a (batch, n_head_kv, >= last) table; its byte strides entry, head, sequence."""
-    if t.dim() != 3 or t.shape[0] != cache.batch or t.shape[1] != cache.n_head_kv or t.shape[2] < last:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected ({cache.batch}, {cache.n_head_kv}, {last})")
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != cache.batch or shape[1] != cache.n_head_kv or shape[2] < last:
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected ({cache.batch}, {cache.n_head_kv}, {last})")
     if t.dtype != dtype or t.device != cache.device:
         raise TypeError(f"{what}: {t.dtype} on {t.device}, expected {dtype} on {cache.device}")
     st = t.stride()
-    return (C.c_size_t * 3)(st[2] * 4, st[1] * 4, st[0] * 4)
+    return st[2] * 4, st[1] * 4, st[0] * 4
 
 
 class PagedCache:
@@ -98,10 +108,9 @@ class PagedCache:
     """
 
     def __init__(self, k, v, block_table, kv_len, q_start=None):
-        torch = _torch()
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"pools {tuple(k.shape)} and {tuple(v.shape)}: expected two (pages, heads, rows, head_dim)")
-        if k.dtype != torch.float16 or v.dtype != torch.float16:
+        if k.dtype != _F16 or v.dtype != _F16:
             raise TypeError(f"pools: {k.dtype}, {v.dtype}, expected float16")
         if block_table.dim() != 2 or block_table.stride(1) != 1:
             raise ValueError("block_table: expected (batch, max_pages) with contiguous rows")
@@ -131,10 +140,28 @@ class PagedCache:
         d.kv_len = kv_len.data_ptr()
         d.q_start = q_start.data_ptr() if q_start is not None else None
 
+        self._last = (-1, None)
+        self._sizes = {}
+
     def _with(self, n_tokens):
-        d = PagedCacheDesc.from_buffer_copy(self._desc)
-        d.n_tokens = n_tokens
+        """The descriptor of a call with so many packed rows."""
+        n, d = self._last
+        if n != n_tokens:
+            d = PagedCacheDesc.from_buffer_copy(self._desc)
+            d.n_tokens = n_tokens
+            self._last = (n_tokens, d)
         return d
+
+    def _workspace(self, L, query, key, *args):
+        """Bytes of workspace by the sizes that decide them (the library's answer, asked once)."""
+        n = self._sizes.get(key)
+        if n is None:
+            out = C.c_size_t(0)
+            L.run(query, *args, C.byref(out))
+            if len(self._sizes) >= 64:
+                self._sizes.clear()
+            n = self._sizes[key] = out.value
+        return n
 
 
 def paged_store(cache, k, v, *, q=None, q_out=None, positions=None, sections=None, n_rot=0, pairs="halves",
@@ -144,77 +171,67 @@ def paged_store(cache, k, v, *, q=None, q_out=None, positions=None, sections=Non
     and returned.  positions: (axes, tokens) or (tokens,) int32; sections: pairs of each axis,
     n_rot / 2 in all (one axis: may be None); pairs: "halves" (j, j + n_rot / 2) or "adjacent"
     (2j, 2j + 1)."""
-    torch = _torch()
     T = k.shape[0]
-    d = PagedStoreDesc()
-    d.type = _type_of("k", k)
+    kind = _type_of("k", k)
     if pairs not in ("halves", "adjacent"):
         raise ValueError(f"pairs {pairs!r}: expected 'halves' or 'adjacent'")
-    d.pairs = ROPE_HALVES if pairs == "halves" else ROPE_ADJACENT
-    d.n_rot = n_rot
-    d.freq_base, d.freq_scale = freq_base, freq_scale
-    d.k_nb[:] = _rows("k", k, cache, cache.n_head_kv)
-    d.v_nb[:] = _rows("v", v, cache, cache.n_head_kv, k.dtype)
+    knb = _rows("k", k, cache, cache.n_head_kv)
+    vnb = _rows("v", v, cache, cache.n_head_kv, k.dtype)
     if v.shape[0] != T or (q is not None and q.shape[0] != T):
         raise ValueError("k, v and q differ in their tokens")
+    n_axes, sec, pos, pos_nb = 0, (0, 0, 0, 0), 0, 0
     if n_rot:
         if positions is None:
             raise ValueError("n_rot without positions")
         if positions.dim() == 1:
             positions = positions[None]
-        if positions.dtype != torch.int32 or positions.device != cache.device:
+        if positions.dtype != _I32 or positions.device != cache.device:
             raise TypeError(f"positions: {positions.dtype} on {positions.device}, expected int32 on {cache.device}")
-        if sections is None:
-            sections = [n_rot // 2]
-        if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] != len(sections):
-            raise ValueError(f"positions {tuple(positions.shape)}: expected ({len(sections)}, {T})")
+        sec = (n_rot // 2,) if sections is None else tuple(sections)
+        n_axes = len(sec)
+        if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] != n_axes:
+            raise ValueError(f"positions {tuple(positions.shape)}: expected ({n_axes}, {T})")
         if T > 1 and positions.stride(1) != 1:
             raise ValueError("positions of an axis must be contiguous")
-        if len(sections) > 4:
+        if n_axes > 4:
             raise ValueError("at most 4 position axes")
-        d.n_axes = len(sections)
-        d.sections[:len(sections)] = sections
-        d.positions, d.positions_nb = positions.data_ptr(), positions.stride(0) * 4
+        sec += (0,) * (4 - n_axes)
+        pos, pos_nb = positions.data_ptr(), positions.stride(0) * 4
     L = _Launch(cache.device, stream)
+    hq, qp, qo, qnb, onb = 0, 0, 0, (0, 0, 0), (0, 0, 0)
     if q is not None:
-        d.n_head_q = q.shape[1]
-        d.q_nb[:] = _rows("q", q, cache, None, k.dtype)
+        hq, qnb = q.shape[1], _rows("q", q, cache, None, k.dtype)
         if q_out is None:
             q_out = L.empty(q.shape, q.dtype)
         if q_out.shape != q.shape:
             raise ValueError(f"q_out {tuple(q_out.shape)}, q {tuple(q.shape)}")
-        d.q_dst_nb[:] = _rows("q_out", q_out, cache, None, k.dtype)
-        d.q, d.q_dst = q.data_ptr(), q_out.data_ptr()
+        onb = _rows("q_out", q_out, cache, None, k.dtype)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
-    d.k, d.v = k.data_ptr(), v.data_ptr()
+    d = PagedStoreDesc.from_buffer_copy(_STORE.pack(
+        kind, ROPE_HALVES if pairs == "halves" else ROPE_ADJACENT, n_rot, n_axes, *sec, freq_base, freq_scale, pos, pos_nb, hq,
+        qp, k.data_ptr(), v.data_ptr(), qo, *qnb, *knb, *vnb, *onb))
     L.run(lib().mlzc_paged_store_dev, C.byref(cache._with(T)), C.byref(d), L.handle)
     return q_out
 
 
-def _attn_desc(cache, q, scale, softcap):
-    d = PagedAttnDesc()
-    d.type = _type_of("q", q)
-    d.n_head_q, d.scale = q.shape[1], scale
-    if softcap:
-        d.mode, d.logit_softcap = FA_MODE_SOFTCAP, softcap
-    d.q = q.data_ptr()
-    d.q_nb[:] = _rows("q", q, cache, None)
-    return d
-
-
-def _lse_into(d, lse, q, cache):
-    torch = _torch()
-    if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != cache.device:
-        raise ValueError(f"lse: {lse.dtype} {tuple(lse.shape)} on {lse.device}, expected float32 {tuple(q.shape[:2])} on {cache.device}")
-    d.lse = lse.data_ptr()
-    d.lse_nb[:] = (lse.stride(1) * 4, lse.stride(0) * 4)
-
-
-def _workspace(L, query, *args):
-    n = C.c_size_t(0)
-    L.run(query, *args, C.byref(n))
-    return n.value
+def _attn_desc(cache, q, scale, softcap, out=None, lse=None):
+    """Descriptor of the attention and weights calls, its tensors checked."""
+    kind = _type_of("q", q)
+    qnb = _rows("q", q, cache, None)
+    dst, dnb, lp, lnb = 0, (0, 0, 0), 0, (0, 0)
+    if out is not None:
+        if out.shape != q.shape:
+            raise ValueError(f"out {tuple(out.shape)}, q {tuple(q.shape)}")
+        dst, dnb = out.data_ptr(), _rows("out", out, cache, None, q.dtype)
+    if lse is not None:
+        if lse.shape != q.shape[:2] or lse.dtype != _F32 or lse.device != cache.device:
+            raise ValueError(f"lse: {lse.dtype} {tuple(lse.shape)} on {lse.device}, expected float32 {tuple(q.shape[:2])} on {cache.device}")
+        st = lse.stride()
+        lp, lnb = lse.data_ptr(), (st[1] * 4, st[0] * 4)
+    return PagedAttnDesc.from_buffer_copy(_ATTN.pack(kind, FA_MODE_SOFTCAP if softcap else 0, q.shape[1], scale, softcap,
+                                                     q.data_ptr(), dst, *qnb, *dnb, lp, *lnb))
 
 
 def _given(workspace, need, L):
@@ -222,7 +239,7 @@ def _given(workspace, need, L):
     if workspace is None:
         if not need:
             return None, 0, None
-        workspace = L.empty(need, _torch().uint8)
+        workspace = L.empty(need, _U8)
     elif workspace.device != L.device or not workspace.is_contiguous():
         raise ValueError(f"workspace: a contiguous tensor on {L.device} is expected")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -230,32 +247,27 @@ def _given(workspace, need, L):
 
 def paged_attn_workspace_bytes(cache, q, scale=1.0, *, softcap=0.0):
     """Bytes of workspace that :func:`paged_attn` needs for these tensors."""
-    d = _attn_desc(cache, q, scale, softcap)
-    d.dst, d.dst_nb[:] = d.q, list(d.q_nb)
     L = _Launch(cache.device, None)
-    return _workspace(L, lib().mlzc_paged_attn_workspace_bytes, C.byref(cache._with(q.shape[0])), C.byref(d))
+    d = _attn_desc(cache, q, scale, softcap, q)
+    return cache._workspace(L, lib().mlzc_paged_attn_workspace_bytes, ("attn", q.shape[0], q.shape[1], q.dtype),
+                            C.byref(cache._with(q.shape[0])), C.byref(d))
 
 
 def paged_attn(cache, q, scale, *, softcap=0.0, out=None, lse=None, return_lse=False, workspace=None, stream=None):
     """Attention of the new tokens q (tokens, n_head_q, head_dim), float32 or float16, over
     their sequences' slots: out of q's shape and type; with lse given (tokens, n_head_q)
     float32 or return_lse, (out, lse).  Rows that belong to no sequence are left as they were."""
-    torch = _torch()
     L = _Launch(cache.device, stream)
-    d = _attn_desc(cache, q, scale, softcap)
     if out is None:
         out = L.empty(q.shape, q.dtype)
-    if out.shape != q.shape:
-        raise ValueError(f"out {tuple(out.shape)}, q {tuple(q.shape)}")
-    d.dst_nb[:] = _rows("out", out, cache, None, q.dtype)
-    d.dst = out.data_ptr()
     if lse is None and return_lse:
-        lse = L.empty(q.shape[:2], torch.float32)
-    if lse is not None:
-        _lse_into(d, lse, q, cache)
-    cd = cache._with(q.shape[0])
-    ws, n, owner = _given(workspace, _workspace(L, lib().mlzc_paged_attn_workspace_bytes, C.byref(cd), C.byref(d)), L)
-    L.run(lib().mlzc_paged_attn_dev, C.byref(cd), C.byref(d), ws, n, L.handle)
+        lse = L.empty(q.shape[:2], _F32)
+    d = C.byref(_attn_desc(cache, q, scale, softcap, out, lse))
+    T = q.shape[0]
+    cd = C.byref(cache._with(T))
+    need = cache._workspace(L, lib().mlzc_paged_attn_workspace_bytes, ("attn", T, q.shape[1], q.dtype), cd, d)
+    ws, n, owner = _given(workspace, need, L)
+    L.run(lib().mlzc_paged_attn_dev, cd, d, ws, n, L.handle)
     return (out, lse) if lse is not None else out
 
 
@@ -264,23 +276,23 @@ def paged_weights(cache, q, lse, scale, *, softcap=0.0, acc=None, out=None, work
     query heads of each kv head, added to acc (batch, n_head_kv, capacity) float32 (None: from
     0): out (acc itself to accumulate in place; made, with zeros past kv_len, if None).  q,
     scale, softcap and lse as given to and returned by :func:`paged_attn`."""
-    torch = _torch()
     L = _Launch(cache.device, stream)
-    d = _attn_desc(cache, q, scale, softcap)
-    _lse_into(d, lse, q, cache)
+    d = C.byref(_attn_desc(cache, q, scale, softcap, None, lse))
     if out is None:
-        out = L.empty((cache.batch, cache.n_head_kv, cache.capacity), torch.float32)
+        out = L.empty((cache.batch, cache.n_head_kv, cache.capacity), _F32)
         if L.given is None:
             out.zero_()
         else:
             with torch.cuda.stream(L.given):
                 out.zero_()
-    onb = _table("out", out, cache, cache.capacity, torch.float32)
-    anb = _table("acc", acc, cache, cache.capacity, torch.float32) if acc is not None else None
-    cd = cache._with(q.shape[0])
-    ws, n, owner = _given(workspace, _workspace(L, lib().mlzc_paged_weights_workspace_bytes, C.byref(cd), C.byref(d)), L)
-    L.run(lib().mlzc_paged_weights_dev, C.byref(cd), C.byref(d), acc.data_ptr() if acc is not None else None, anb,
-          out.data_ptr(), onb, ws, n, L.handle)
+    nb = C.c_size_t * 3
+    onb = nb(*_table("out", out, cache, cache.capacity, _F32))
+    anb = nb(*_table("acc", acc, cache, cache.capacity, _F32)) if acc is not None else None
+    T = q.shape[0]
+    cd = C.byref(cache._with(T))
+    need = cache._workspace(L, lib().mlzc_paged_weights_workspace_bytes, ("weights", T, q.shape[1], q.dtype), cd, d)
+    ws, n, owner = _given(workspace, need, L)
+    L.run(lib().mlzc_paged_weights_dev, cd, d, acc.data_ptr() if acc is not None else None, anb, out.data_ptr(), onb, ws, n, L.handle)
     return out
 
 
@@ -291,26 +303,23 @@ def paged_evict(cache, weights, budget, *, n_sink=0, n_recent=0, weights_out=Non
     kv_len): kept (batch, n_head_kv, budget) int32 the former slot of each slot (-1 past the
     new length), weights_out the kept slots' weights (weights itself unless given), kv_len the
     new lengths (cache.kv_len itself is updated unless kv_len_out is given)."""
-    torch = _torch()
     L = _Launch(cache.device, stream)
     if weights_out is None:
         weights_out = weights
     if kept is None:
-        kept = L.empty((cache.batch, cache.n_head_kv, budget), torch.int32)
+        kept = L.empty((cache.batch, cache.n_head_kv, budget), _I32)
     if kv_len_out is None:
         kv_len_out = cache.kv_len
-    if tuple(kv_len_out.shape) != (cache.batch,) or kv_len_out.dtype != torch.int32 or not kv_len_out.is_contiguous() or \
+    if tuple(kv_len_out.shape) != (cache.batch,) or kv_len_out.dtype != _I32 or not kv_len_out.is_contiguous() or \
             kv_len_out.device != cache.device:
         raise ValueError("kv_len_out: expected a contiguous (batch,) int32 tensor beside the cache")
-    d = PagedEvictDesc()
-    d.budget, d.n_sink, d.n_recent = budget, n_sink, n_recent
-    d.weights, d.weights_nb = weights.data_ptr(), _table("weights", weights, cache, cache.capacity, torch.float32)
-    d.weights_out, d.weights_out_nb = weights_out.data_ptr(), _table("weights_out", weights_out, cache, cache.capacity, torch.float32)
-    d.kept, d.kept_nb = kept.data_ptr(), _table("kept", kept, cache, budget, torch.int32)
-    d.kv_len_out = kv_len_out.data_ptr()
-    cd = cache._desc
-    ws, n, owner = _given(workspace, _workspace(L, lib().mlzc_paged_evict_workspace_bytes, C.byref(cd), C.byref(d)), L)
-    L.run(lib().mlzc_paged_evict_dev, C.byref(cd), C.byref(d), ws, n, L.handle)
+    d = C.byref(PagedEvictDesc.from_buffer_copy(_EVICT.pack(
+        budget, n_sink, n_recent, weights.data_ptr(), weights_out.data_ptr(), *_table("weights", weights, cache, cache.capacity, _F32),
+        *_table("weights_out", weights_out, cache, cache.capacity, _F32), kept.data_ptr(), *_table("kept", kept, cache, budget, _I32),
+        kv_len_out.data_ptr())))
+    cd = C.byref(cache._desc)
+    ws, n, owner = _given(workspace, cache._workspace(L, lib().mlzc_paged_evict_workspace_bytes, ("evict", budget), cd, d), L)
+    L.run(lib().mlzc_paged_evict_dev, cd, d, ws, n, L.handle)
     return kept, weights_out, kv_len_out
 
 
