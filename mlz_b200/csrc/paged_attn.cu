@@ -38,8 +38,10 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <cstring>
 #include <numeric>
+#include <type_traits>
 
 #include "paged.h"
 #include "ptx.cuh"
@@ -108,8 +110,15 @@ struct Cfg {
     static constexpr int kSoftWarps = 4 * (HL ? (D == 64 ? 2 : 1) : NS);
     static constexpr int CD = D < 128 ? D : 128;          // dims of a correction thread
     static constexpr int kCorrWarps = HL ? 4 * (D / CD) : 0;
-    static constexpr int kMisc = kSoftWarps + kCorrWarps;
-    static constexpr int kThreads = (kMisc + 4) * 32;
+    static constexpr int kThreads = (4 + kSoftWarps + kCorrWarps) * 32;
+    // Measured on 4096 tokens of 16384 slots (8 KV heads of 4, f16):
+    // steps of S a tile with two query tiles: 64 dims 673 us with two, 728 with one (a step's
+    // products run beside the other's softmax); 128 dims 1027 with two (products of 64 columns
+    // read Q twice as often), 855 with one
+    static constexpr int H = NS == 2 && D == 64 ? 2 : 1;
+    // one in so many pairs of exponentials on the FMA pipe (0: none): 128 dims 855 us with 4, 947
+    // with none; 64 dims 712 and 673; 256 dims, where the products are the bound, 370 and 353
+    static constexpr int kPoly = NS == 2 && D == 128 ? 4 : 0;
     // f32: the softmax holds a row's scores in registers (256 dims: the correction needs those)
     static constexpr bool kHold = D < 256;
     static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
@@ -121,7 +130,7 @@ struct Cfg {
 
 // Barriers in shared memory.
 struct Bars {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[2], p_full[2], p_half[2], o_step, o_done[2], o_empty[2], stat_full[4];
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[4], p_full[4], o_step[2], o_done[2], o_empty[2], stat_full[4];
     uint32_t tmem;
     int abort;
     long long first, count, total;   // this CTA's share of the list; its start's place
@@ -252,16 +261,13 @@ struct Row {
     }
 };
 
-// One in so many pairs of exponentials goes to the FMA pipe: the exponential unit takes 1024
-// clocks a tile and warp scheduler, as long as a tile's matrix products.
-constexpr int kPolyEvery = 4;
-
-__device__ __forceinline__ float row_max(const float (&x)[BN]) {
+template <int N>
+__device__ __forceinline__ float row_max(const float (&x)[N]) {
     float m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = max3(x[3 * i], x[3 * i + 1], x[3 * i + 2]);
 #pragma unroll
-    for (int i = 12; i + 1 < BN; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], x[i], x[i + 1]);
+    for (int i = 12; i + 1 < N; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], x[i], x[i + 1]);
     return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
@@ -297,9 +303,40 @@ struct Sink {
     }
 };
 
+// P = 2^(c2 x + off) of N scores, rounded to f16, back over them (32 scores a column pair block:
+// their first 16 columns); returns the sum.
+template <int POLY, int N>
+__device__ __forceinline__ float weigh(const float (&x)[N], float c2, float off, uint32_t s_col) {
+    const uint64_t c22 = pair(c2, c2), off2 = pair(off, off);
+    uint64_t sum[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N / 32; ++i) {
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint64_t y = fma2(pair(x[i * 32 + 2 * j], x[i * 32 + 2 * j + 1]), c22, off2);
+            float p0, p1;
+            if (POLY && j % (POLY ? POLY : 1) == POLY - 1) {
+                exp2_poly(y, p0, p1);
+            } else {
+                unpair(y, p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+            }
+            sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
+            p[j] = ptx::pack_h2(p0, p1);
+        }
+        tmem_st16(s_col + i * 32, p);
+    }
+    float s0, s1;
+    unpair(add2(sum[0], sum[1]), s0, s1);
+    return s0 + s1;
+}
+
+// Softmax of an f16 call, step by step (a tile, or half of one: Cfg::H).
 template <class C>
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_t tmem, int warp, int lane) {
-    constexpr int D = C::D;
+    constexpr int D = C::D, H = C::H, N = BN / H;        // steps a tile, scores a step
     const int slot = C::NS == 2 ? warp >> 2 : 0;         // query tile of this warpgroup
     const Row q(a, (warp & 3) * 32 + lane);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -308,33 +345,33 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
     const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
     const float rise = kRescale / c2;
     volatile int* abort = &B->abort;
-    uint32_t g = 0, piece = 0;
+    uint32_t g = 0, piece = 0;                           // steps, pieces
     Walk<C> w(B);
     while (w.next(a)) {
         if (slot >= w.tiles(a)) continue;
         const bool real = q.real(a, w, slot), busy = __any_sync(~0u, real);
         const int own = w.s.kv - w.s.rows + q.tok(a, w, slot);   // last slot this row sees
         float m = -INFINITY, l = 0.0f;
-        for (int it = 0; it < w.n; ++it, ++g) {
-            const int buf = C::NS == 2 ? slot : (int)(g & 1);
-            const uint32_t par = C::NS == 2 ? g & 1 : (g >> 1) & 1;
-            if (!mbar_wait(smem_u32(&B->s_full[buf]), par, abort, a.c.err)) return;
+        for (int it = 0; it < w.n * H; ++it, ++g) {
+            // barriers 2 * query tile + half, or the buffer; either way one phase in two steps
+            const int buf = C::NS == 1 ? (int)(g & 1) : (H == 2 ? 2 * slot + (int)(g & 1) : slot);
+            if (!mbar_wait(smem_u32(&B->s_full[buf]), (C::NS == 1 || H == 2 ? g >> 1 : g) & 1, abort, a.c.err)) return;
             tc_fence_after();
             if (busy) {
-                const uint32_t s_col = lanes + C::kSCol + buf * BN;
-                float x[BN];
+                const uint32_t s_col = lanes + C::kSCol + buf * N;
+                float x[N];
 #pragma unroll
-                for (int i = 0; i < BN / 32; ++i)
+                for (int i = 0; i < N / 32; ++i)
                     tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                 tmem_ld_wait();
                 if (C::CAP) {
 #pragma unroll
-                    for (int i = 0; i < BN; ++i) x[i] = capped(x[i], cap_in, a.softcap);
+                    for (int i = 0; i < N; ++i) x[i] = capped(x[i], cap_in, a.softcap);
                 }
-                const int limit = own - (w.tile + it) * BN;
-                if (__any_sync(~0u, limit < BN - 1)) {
+                const int limit = own - w.tile * BN - it * N;
+                if (__any_sync(~0u, limit < N - 1)) {
 #pragma unroll
-                    for (int i = 0; i < BN; ++i) x[i] = i > limit ? -INFINITY : x[i];
+                    for (int i = 0; i < N; ++i) x[i] = i > limit ? -INFINITY : x[i];
                 }
                 const float top = row_max(x);
                 if (it == 0) {
@@ -344,9 +381,9 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                     const float al = m == -INFINITY ? 0.0f : ex2((m - to) * c2);
                     m = to;
                     l *= al;
-                    // every product up to tile g - 1 is in O: with NS = 2 this S came after it, with
-                    // NS = 1 it came after that of tile g - 2
-                    if (C::NS == 1 && !mbar_wait(smem_u32(&B->o_step), (g - 1) & 1, abort, a.c.err)) return;
+                    // O has the products of the steps before the last (this S came after them);
+                    // wait for the last's
+                    if (!mbar_wait(smem_u32(&B->o_step[slot]), (g - 1) & 1, abort, a.c.err)) return;
                     tc_fence_after();
 #pragma unroll 1
                     for (int i = 0; i < D; i += 16) {
@@ -358,41 +395,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                         tmem_st16(o_col + i, o);
                     }
                 }
-                const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                const uint64_t c22 = pair(c2, c2), off2 = pair(off, off);
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < BN / 32; ++i) {
-                    uint32_t hi[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const uint64_t y = fma2(pair(x[i * 32 + 2 * j], x[i * 32 + 2 * j + 1]), c22, off2);
-                        float p0, p1;
-                        if (j % kPolyEvery == kPolyEvery - 1) {
-                            exp2_poly(y, p0, p1);
-                        } else {
-                            unpair(y, p0, p1);
-                            p0 = ex2(p0);
-                            p1 = ex2(p1);
-                        }
-                        sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
-                        hi[j] = ptx::pack_h2(p0, p1);
-                    }
-                    tmem_st16(s_col + i * 32, hi);
-                    // the first half of P: its products start while the second is computed
-                    if (C::NS == 2 && i == BN / 64 - 1) {
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&B->p_half[buf]));
-                    }
-                }
-                float s0, s1;
-                unpair(add2(sum[0], sum[1]), s0, s1);
-                l += s0 + s1;
+                l += weigh<C::kPoly>(x, c2, m == -INFINITY ? 0.0f : kPOffset - m * c2, s_col);
                 tmem_st_wait();
-            } else if (C::NS == 2 && lane == 0) {
-                mbar_arrive(smem_u32(&B->p_half[buf]));
             }
             tc_fence_before();
             __syncwarp();
@@ -704,160 +708,185 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
     }
 }
 
+// Everything that the issued instructions take is computed from values that the compiler knows
+// to be uniform (one shuffle a ring unit), with 32-bit descriptor steps: the tensor cores hold
+// only about four products in their queue, so what this warp does between two of them has to
+// take less than four products' time.
 template <class C>
-__device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs, uint32_t ring, uint32_t tmem, int lane) {
-    constexpr int NS = C::NS, DU = C::DU;
-    constexpr uint32_t idesc_s = umma_idesc_f16(128, BN);
+__device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs, uint32_t ring, uint32_t tmem_base, int lane) {
+    constexpr int NS = C::NS, DU = C::DU, PARTS = C::HL ? 2 : 1;
+    constexpr int kCols = BN / C::H;                      // slots a step of S
+    constexpr uint32_t idesc_s = umma_idesc_f16(128, kCols);
     constexpr uint32_t idesc_o = umma_idesc_f16(128, DU) | kIdescBMnMajor;
+    const uint32_t bars = uniform(smem_u32(B)), q16 = uniform(qs >> 4), ring16 = uniform(ring >> 4), tmem = uniform(tmem_base);
+#define MLZC_BAR(member, i) (bars + (uint32_t)offsetof(Bars, member) + 8u * (uint32_t)(i))
     volatile int* abort = &B->abort;
-    uint32_t at = 0, seg = 0, g[2] = {0, 0}, piece[2] = {0, 0};
+    uint32_t slot = 0, phase = 0, seg = 0, g[2] = {0, 0}, piece[2] = {0, 0};
     uint32_t last_bar = 0, last_par = 0;     // of the latest commit to a ring barrier
-    // waits for the ring's next unit and takes it
-    auto take = [&](uint32_t& st) {
-        st = at % C::ST;
-        if (!mbar_wait(smem_u32(&B->full[st]), (at / C::ST) & 1, abort, a.c.err)) return false;
+    auto wait = [&](uint32_t bar, uint32_t par) { return mbar_wait(bar, par, abort, a.c.err); };
+    auto commit = [&](uint32_t bar) {
+        if (elect_one()) umma_commit(bar);
+    };
+    // waits for the ring's next unit and takes it: its number (uniform) and phase
+    struct Unit {
+        uint32_t st, phase;
+    };
+    auto take = [&](Unit& u) {
+        u.st = uniform(slot);
+        u.phase = phase;
+        if (!wait(MLZC_BAR(full, u.st), phase)) return false;
         tc_fence_after();
-        ++at;
+        if (++slot == C::ST) {
+            slot = 0;
+            phase ^= 1;
+        }
         return true;
     };
-    // frees unit `st`, the ring's `index`-th, when the products issued so far are done
-    auto release = [&](uint32_t st, uint32_t index) {
-        if (elect_one()) umma_commit(smem_u32(&B->empty[st]));
-        last_bar = smem_u32(&B->empty[st]);
-        last_par = (index / C::ST) & 1;
+    // frees a unit when the products issued so far are done
+    auto release = [&](const Unit& u) {
+        commit(MLZC_BAR(empty, u.st));
+        last_bar = MLZC_BAR(empty, u.st);
+        last_par = u.phase;
     };
-    auto scores = [&](int tile, int buf, int unit, uint32_t st) {
-        const uint32_t k_at = uniform(ring + st * C::kUnit);
-        const uint32_t q_at = uniform(qs + tile * (C::HL ? 2 : 1) * C::kQTile + unit * C::SUBS * C::kQSub);
-        const uint32_t d = uniform(tmem + C::kSCol + buf * BN);
-        const bool first = uniform(unit) == 0;
+    // S of query tile `tile` and the slots from `row` of the tile on, into buffer `buf`
+    auto scores = [&](int tile, int buf, int unit, const Unit& u, int row) {
+        const uint32_t k = desc_lo(ring16 + u.st * (C::kUnit >> 4) + row * 8);
+        const uint32_t q = desc_lo(q16 + ((tile * PARTS * C::kQTile + unit * C::SUBS * C::kQSub) >> 4));
+        const uint32_t d = tmem + C::kSCol + buf * kCols;
         if (elect_one()) {
-            const uint64_t k = umma_desc_sw128(k_at);
 #pragma unroll
-            for (int part = C::HL ? 1 : 0; part >= 0; --part) {      // lo, then hi
-                const uint64_t q = umma_desc_sw128(q_at + part * C::kQTile);
+            for (int part = PARTS - 1; part >= 0; --part)      // lo, then hi
 #pragma unroll
                 for (int i = 0; i < DU / 16; ++i)
-                    umma_f16(d, q + (((i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
-                             k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s,
-                             !first || i > 0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
-            }
+                    umma_f16_lo(d, q + ((part * C::kQTile + (i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
+                                k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s, unit > 0 || i > 0 || part != PARTS - 1);
         }
     };
-    // key steps [i0, i1) of P V
-    auto values = [&](int tile, int buf, int unit, uint32_t st, bool add, int i0, int i1) {
-        const uint32_t v_at = uniform(ring + st * C::kUnit);
-        const uint32_t d = uniform(tmem + C::kOCol + tile * C::D + unit * DU), p = uniform(tmem + C::kSCol + buf * BN);
-        const bool sum = uniform(add) != 0;
+    // `steps` key steps of P V, from step i0 (even) on
+    auto values = [&](int tile, int buf, int unit, const Unit& u, bool add, int i0, auto steps) {
+        const uint32_t v = desc_lo(ring16 + u.st * (C::kUnit >> 4) + i0 * 128, C::kSub);
+        const uint32_t d = tmem + C::kOCol + tile * C::D + unit * DU, p = tmem + C::kSCol + buf * BN + i0 * 16;
         if (elect_one()) {
-            const uint64_t v = umma_desc_mn_sw128(v_at, C::kSub);
 #pragma unroll
-            for (int part = C::HL ? 1 : 0; part >= 0; --part)
+            for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                for (int i = i0; i < i1; ++i)
-                    umma_f16_ta(d, p + (i >> 1) * 32 + (i & 1) * 8 + part * 16, v + ((i * 2048) >> 4), idesc_o, sum || i > i0 || part != (C::HL ? 1 : 0) ? 1u : 0u);
+                for (int i = 0; i < decltype(steps)::value; ++i)
+                    umma_f16_ta_lo(d, p + (i >> 1) * 32 + (i & 1) * 8 + part * 16, v + i * 128, idesc_o,
+                                   add || i > 0 || part != PARTS - 1);
         }
     };
+    constexpr std::integral_constant<int, BN / 16> all{};
+    constexpr std::integral_constant<int, BN / 16 / C::H> step{};
     // V rows that no row of the piece sees may hold anything (a page's unused rows) or have not
     // been copied: P is 0 there, and 0 * NaN would be NaN
-    auto blank = [&](const Walk<C>& w, int i, uint32_t st) {
+    auto blank = [&](const Walk<C>& w, int i, const Unit& u) {
         const int n = tile_rows(a, w, i);
         if (n == BN) return;
         for (int x = n * 8 + lane; x < BN * 8; x += 32)
 #pragma unroll
-            for (int u = 0; u < C::SUBS; ++u)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * C::kUnit + u * C::kSub + x * 16), "r"(0) : "memory");
+            for (int k = 0; k < C::SUBS; ++k)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + u.st * C::kUnit + k * C::kSub + x * 16), "r"(0) : "memory");
         fence_proxy_async_smem();
         __syncwarp();
     };
     // S of one query tile (NS = 1): all units of K
     auto scores_all = [&](int buf) {
+#pragma unroll
         for (int unit = 0; unit < C::UN; ++unit) {
-            uint32_t st;
-            if (!take(st)) return false;
-            scores(0, buf, unit, st);
-            release(st, at - 1);
+            Unit u;
+            if (!take(u)) return false;
+            scores(0, buf, unit, u, 0);
+            release(u);
         }
-        if (elect_one()) umma_commit(smem_u32(&B->s_full[buf]));
+        commit(MLZC_BAR(s_full, buf));
         return true;
     };
     bool ok = true;
     Walk<C> w(B);
     while (ok && w.next(a)) {
         const int nt = w.tiles(a);
-        ok = mbar_wait(smem_u32(&B->q_full), seg & 1, abort, a.c.err);
+        ok = wait(MLZC_BAR(q_full, 0), seg & 1);
         if (!ok) break;
         ++seg;
         tc_fence_after();
         if constexpr (NS == 1) {
-            if (!(ok = scores_all(g[0] & 1))) break;
-            if (w.n == 1 && elect_one()) umma_commit(smem_u32(&B->q_empty));
+            const int first = (int)uniform(g[0] & 1);
+            if (!(ok = scores_all(first))) break;
+            if (w.n == 1) commit(MLZC_BAR(q_empty, 0));
             for (int it = 0; it < w.n; ++it, ++g[0]) {
-                const int buf = g[0] & 1;
+                const int buf = (int)uniform(g[0] & 1);
                 if (it + 1 < w.n) {
                     if (!(ok = scores_all(buf ^ 1))) break;
-                    if (it + 2 == w.n && elect_one()) umma_commit(smem_u32(&B->q_empty));
+                    if (it + 2 == w.n) commit(MLZC_BAR(q_empty, 0));
                 }
-                ok = mbar_wait(smem_u32(&B->p_full[buf]), (g[0] >> 1) & 1, abort, a.c.err);
+                ok = wait(MLZC_BAR(p_full, buf), (g[0] >> 1) & 1);
                 // O free: f32 calls empty it tile by tile, the others piece by piece
                 const uint32_t turn = C::HL ? g[0] : piece[0];
-                if (ok && (C::HL || it == 0)) ok = mbar_wait(smem_u32(&B->o_empty[0]), (turn & 1) ^ 1, abort, a.c.err);
-                for (int unit = 0; ok && unit < C::UN; ++unit) {
-                    uint32_t st;
-                    if (!(ok = take(st))) break;
-                    blank(w, w.tile + it, st);
+                if (ok && (C::HL || it == 0)) ok = wait(MLZC_BAR(o_empty, 0), (turn & 1) ^ 1);
+                if (!ok) break;
+                const bool add = !C::HL && uniform(it) > 0;
+#pragma unroll
+                for (int unit = 0; unit < C::UN; ++unit) {
+                    Unit u;
+                    if (!(ok = take(u))) break;
+                    blank(w, w.tile + it, u);
                     tc_fence_after();
-                    values(0, buf, unit, st, !C::HL && it > 0, 0, BN / 16);
-                    release(st, at - 1);
+                    values(0, buf, unit, u, add, 0, all);
+                    release(u);
                 }
                 if (!ok) break;
-                if (elect_one()) {
-                    if (C::HL || it + 1 == w.n) umma_commit(smem_u32(&B->o_done[0]));
-                    if (!C::HL) umma_commit(smem_u32(&B->o_step));
-                }
+                if (C::HL || it + 1 == w.n) commit(MLZC_BAR(o_done, 0));
+                if (!C::HL) commit(MLZC_BAR(o_step, 0));
             }
         } else {
-            uint32_t ks = 0, vs = 0;
-            if (!(ok = take(ks))) break;
-            for (int i = 0; i < nt; ++i) {
-                scores(i, i, 0, ks);
-                if (elect_one()) umma_commit(smem_u32(&B->s_full[i]));
-            }
-            release(ks, at - 1);
-            if (w.n == 1 && elect_one()) umma_commit(smem_u32(&B->q_empty));
-            for (int it = 0; ok && it < w.n; ++it) {
-                const bool more = it + 1 < w.n;
-                if (!(ok = take(vs))) break;
-                const uint32_t v_at = at - 1;
-                blank(w, w.tile + it, vs);
-                for (int i = 0; ok && i < nt; ++i) {
-                    ok = mbar_wait(smem_u32(&B->p_half[i]), g[i] & 1, abort, a.c.err);
-                    if (ok && it == 0) ok = mbar_wait(smem_u32(&B->o_empty[i]), (piece[i] & 1) ^ 1, abort, a.c.err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    values(i, i, 0, vs, it > 0, 0, BN / 32);
-                    if (!(ok = mbar_wait(smem_u32(&B->p_full[i]), g[i] & 1, abort, a.c.err))) break;
-                    tc_fence_after();
-                    values(i, i, 0, vs, true, BN / 32, BN / 16);
-                    if (!more && elect_one()) umma_commit(smem_u32(&B->o_done[i]));
-                    if (more) {
-                        if (i == 0 && !(ok = take(ks))) break;
-                        scores(i, i, 0, ks);
-                        if (elect_one()) umma_commit(smem_u32(&B->s_full[i]));
+            Unit k, v;
+            if (!(ok = take(k))) break;
+#pragma unroll
+            for (int h = 0; h < C::H; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (i < nt) {
+                        scores(i, C::H * i + h, 0, k, h * kCols);
+                        commit(MLZC_BAR(s_full, C::H * i + h));
                     }
-                    ++g[i];
-                }
+            release(k);
+            if (w.n == 1) commit(MLZC_BAR(q_empty, 0));
+            for (int it = 0; ok && it < w.n; ++it) {
+                const bool more = it + 1 < w.n, begun = uniform(it) > 0;
+                if (!(ok = take(v))) break;
+                blank(w, w.tile + it, v);
+#pragma unroll
+                for (int h = 0; h < C::H; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (!ok || i >= nt) continue;
+                        const int buf = C::H * i + h;
+                        ok = wait(MLZC_BAR(p_full, buf), (C::H == 2 ? g[i] >> 1 : g[i]) & 1);
+                        if (ok && it == 0 && h == 0) ok = wait(MLZC_BAR(o_empty, i), (piece[i] & 1) ^ 1);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        values(i, i, 0, v, begun || h > 0, h * (BN / 16 / C::H), step);
+                        commit(MLZC_BAR(o_step, i));
+                        if (!more && h == C::H - 1) commit(MLZC_BAR(o_done, i));
+                        if (more) {
+                            if (h == 0 && i == 0 && !(ok = take(k))) continue;
+                            scores(i, buf, 0, k, h * kCols);
+                            commit(MLZC_BAR(s_full, buf));
+                        }
+                        ++g[i];
+                    }
                 if (!ok) break;
-                release(vs, v_at);
+                release(v);
                 if (more) {
-                    release(ks, at - 1);
-                    if (it + 2 == w.n && elect_one()) umma_commit(smem_u32(&B->q_empty));
+                    release(k);
+                    if (it + 2 == w.n) commit(MLZC_BAR(q_empty, 0));
                 }
             }
         }
         for (int i = 0; i < nt; ++i) ++piece[i];
     }
-    if (!ok && last_bar && lane == 0) {
+#undef MLZC_BAR
+    if (!ok && last_bar && elect_one()) {
         // the products already issued end before TMEM is released
         umma_commit(last_bar);
         const uint64_t t0 = ptx::global_ns();
@@ -896,7 +925,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     uint8_t* fixed = smem + C::kQBytes + (size_t)C::ST * C::kUnit;
     Bars* B = reinterpret_cast<Bars*>(fixed);
     float2* stats = reinterpret_cast<float2*>(fixed + kBarBytes);
-    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    // the loading and issuing warps come first (a scheduler prefers its lower warps), then the
+    // softmax and correction warpgroups, numbered from 0 in their roles
+    const int warp = (int)uniform(threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::ST; ++i) {
             mbar_init(smem_u32(&B->full[i]), 1);
@@ -904,13 +935,14 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
         }
         mbar_init(smem_u32(&B->q_full), 1);
         mbar_init(smem_u32(&B->q_empty), 1);
-        mbar_init(smem_u32(&B->o_step), 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&B->s_full[i]), 1);
-            mbar_init(smem_u32(&B->p_full[i]), 4);
-            mbar_init(smem_u32(&B->p_half[i]), 4);
+            mbar_init(smem_u32(&B->o_step[i]), 1);
             mbar_init(smem_u32(&B->o_done[i]), 1);
             mbar_init(smem_u32(&B->o_empty[i]), C::HL ? C::kCorrWarps : 4);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&B->s_full[i]), 1);
+            mbar_init(smem_u32(&B->p_full[i]), 4);
         }
         for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&B->stat_full[i]), 4);
         B->abort = 0;
@@ -919,7 +951,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
         tma_prefetch_desc(&a.mv);
         if (!C::HL) tma_prefetch_desc(&a.mq);
     }
-    if (warp == C::kMisc + 1) tmem_alloc(smem_u32(&B->tmem), 512);
+    if (warp == -3) tmem_alloc(smem_u32(&B->tmem), 512);
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     plan<C>(a, B);
@@ -934,25 +966,25 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     constexpr int kCorr = C::HL ? (C::D == 64 ? 120 : (C::D == 128 ? 216 : 168)) : 0;
     constexpr int kRest = C::HL ? (C::D == 128 ? 112 : 72) : (C::NS == 2 ? 88 : 255);
     static_assert(kSoft * C::kSoftWarps + kCorr * C::kCorrWarps + kRest * 4 <= kShare * (C::kThreads / 32), "registers");
-    if (warp < C::kSoftWarps) {
+    if (warp >= 0 && warp < C::kSoftWarps) {
         set_registers<kShare, kSoft>();
         if constexpr (C::HL) softmax_tile_role<C>(a, B, stats, tmem, warp, lane);
         else softmax_role<C>(a, B, tmem, warp, lane);
-    } else if (C::HL && warp < C::kMisc) {
+    } else if (C::HL && warp >= 0) {
         if constexpr (C::HL) {
             set_registers<kShare, kCorr>();
             correct_role<C>(a, B, stats, tmem, warp, lane);
         }
     } else {
         set_registers<kShare, kRest>();
-        if (warp == C::kMisc) load_role<C>(a, B, ring, lane);
-        else if (warp == C::kMisc + 1) mma_role<C>(a, B, qs, ring, tmem, lane);
-        else if (warp == C::kMisc + 2) q_role<C>(a, B, qs, lane);
+        if (warp == -4) load_role<C>(a, B, ring, lane);
+        else if (warp == -3) mma_role<C>(a, B, qs, ring, tmem, lane);
+        else if (warp == -2) q_role<C>(a, B, qs, lane);
         else if (lane == 0) head_role<C>(a, B);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == C::kMisc + 1) {
+    if (warp == -3) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

@@ -88,28 +88,37 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D += A . B with A (f16, two k values per 32-bit column, one row a lane) in TMEM.
-__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory descriptors in halves, for issue loops: K-major tiles as in umma_desc_sw128, and
+// tiles whose M/N axis is contiguous (64-element rows of 128 bytes, one row a k value:
+// `block_bytes` from one 64-element block of the M/N axis to the next, 1024 bytes from 8 k values
+// to the next 8).  The upper words are alike (8 rows of 128
+// bytes a swizzle atom, version, layout), and stepping through a tile is a 32-bit addition to
+// the lower one (addresses count 16 bytes and stay below 2^14).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr16, uint32_t block_bytes = 16) { return saddr16 | ((block_bytes >> 4) << 16); }
+__device__ __forceinline__ void umma_f16_lo(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n"
         " .reg .pred p;\n"
-        " setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        " .reg .b64 x, y;\n"
+        " mov.b64 x, {%1, %4};\n"
+        " mov.b64 y, {%2, %4};\n"
+        " setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n"
         "}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+        "r"(a), "r"(b), "r"(idesc), "r"(kDescHi), "r"((uint32_t)accumulate));
 }
-
-// Descriptor of a tile whose M/N axis is contiguous (64-element rows of 128 bytes, one row a k
-// value, 128-byte swizzle): `block_bytes` from one 64-element block of the M/N axis to the
-// next, 1024 bytes from 8 k values to the next 8.
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t block_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)((block_bytes >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
+// A (f16, two k values per 32-bit column, one row a lane) in TMEM.
+__device__ __forceinline__ void umma_f16_ta_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n"
+        " .reg .pred p;\n"
+        " .reg .b64 y;\n"
+        " mov.b64 y, {%2, %4};\n"
+        " setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b), "r"(idesc), "r"(kDescHi), "r"((uint32_t)accumulate));
 }
 constexpr uint32_t kIdescBMnMajor = 1u << 16;   // instruction descriptor: B with its N axis contiguous
 
