@@ -76,6 +76,7 @@ struct AttnArgs {
     char* lse;
     size_t q_head, q_tok, d_head, d_tok, lse_head, lse_tok;
     int G, tq;                 // query heads a KV head; tokens a tile (tq * G <= 128)
+    paged::Div by_g;
     int box;                   // rows of a K / V box
     float scale, softcap;      // softcap 0: none
     int n_ctas, rec_rows;
@@ -104,9 +105,8 @@ struct Cfg {
     static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - (int)kStats - (int)kQBytes) / (int)kUnit;
     static constexpr int ST = kFit > 8 ? 8 : kFit;
     static constexpr size_t kSmem = 1024 + kBarBytes + kStats + kQBytes + (size_t)ST * kUnit;
-    // warps: softmax (f32 calls of 64 dims are bound by the exponentials: two warpgroups take
-    // turns at the tiles), correction (f32; 128 dims a thread at most), then the four of the
-    // other roles
+    // warps: four that load and issue, softmax (f32 calls of 64 dims are bound by it: two
+    // warpgroups take turns at the tiles), correction (f32; 128 dims a thread at most)
     static constexpr int kSoftWarps = 4 * (HL ? (D == 64 ? 2 : 1) : NS);
     static constexpr int CD = D < 128 ? D : 128;          // dims of a correction thread
     static constexpr int kCorrWarps = HL ? 4 * (D / CD) : 0;
@@ -119,7 +119,7 @@ struct Cfg {
     // one in so many pairs of exponentials on the FMA pipe (0: none): 128 dims 855 us with 4, 947
     // with none; 64 dims 712 and 673; 256 dims, where the products are the bound, 370 and 353
     static constexpr int kPoly = NS == 2 && D == 128 ? 4 : 0;
-    // f32: the softmax holds a row's scores in registers (256 dims: the correction needs those)
+    // f32: the softmax holds a row's scores in registers (else the correction needs those)
     static constexpr bool kHold = D < 256;
     static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
     static constexpr uint32_t kOCol = 2 * BN;             // O of tile i at + i * D
@@ -252,7 +252,7 @@ __device__ __forceinline__ void put32(__half* p, const float (&x)[32]) {
 // A query row's place: thread `row` of a query tile.
 struct Row {
     int row, tok_of, head_of;            // token and head in the tile
-    __device__ Row(const AttnArgs& a, int r) : row(r), tok_of(r / a.G), head_of(r % a.G) {}
+    __device__ Row(const AttnArgs& a, int r) : row(r), tok_of(a.by_g.quot(r)), head_of(a.by_g.rem(r)) {}
     template <class C>
     __device__ int tok(const AttnArgs& a, const Walk<C>& w, int slot) const { return w.tok0(a) + slot * a.tq + tok_of; }
     template <class C>
@@ -654,15 +654,18 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t r
     }
 }
 
+// f16: one warp, by TMA.  f32: two warps split the rows into f16 hi + lo; a lane keeps its place
+// in a row (8 values) and steps through rows, with kDeep rows' loads under way (one warp with a
+// division a row took 31 000 clocks a tile of 128 x 128).
 template <class C>
-__device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, int lane) {
+__device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, int part, int lane) {
     volatile int* abort = &B->abort;
+    const uint32_t bar = smem_u32(&B->q_full);
     uint32_t piece = 0;
     bool ok = true;
     Walk<C> w(B);
     while (w.next(a)) {
         if (!(ok = mbar_wait(smem_u32(&B->q_empty), (piece & 1) ^ 1, abort, a.c.err))) break;
-        const uint32_t bar = smem_u32(&B->q_full);
         const int nt = w.tiles(a);
         if constexpr (!C::HL) {
             if (lane == 0) {
@@ -673,25 +676,35 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
                         tma_load_3d(qs + i * C::kQTile + u * C::kQSub, &a.mq, bar, u * 64, w.h * a.G, w.s.row0 + w.tok0(a) + i * a.tq);
             }
         } else {
-            constexpr int kCh = C::D / 8;     // 8 values: 32 bytes of q, 16 of each half
-            for (int i = 0; i < nt; ++i) {
-                const int t0 = w.tok0(a) + i * a.tq;
-                const int items = min(a.tq, w.s.rows - t0) * a.G * kCh;
-                const uint32_t base = qs + i * 2 * C::kQTile;
-#pragma unroll 4
-                for (int x = lane; x < items; x += 32) {
-                    const int r = x / kCh, ch = x % kCh;
-                    const char* p = a.q + (size_t)(w.s.row0 + t0 + r / a.G) * a.q_tok + (size_t)(w.h * a.G + r % a.G) * a.q_head + ch * 32;
-                    const float4 v0 = ptx::ld_act(reinterpret_cast<const float4*>(p));
-                    const float4 v1 = ptx::ld_act(reinterpret_cast<const float4*>(p + 16));
-                    uint4 hi, lo;
-                    ptx::split_h2(v0.x, v0.y, hi.x, lo.x);
-                    ptx::split_h2(v0.z, v0.w, hi.y, lo.y);
-                    ptx::split_h2(v1.x, v1.y, hi.z, lo.z);
-                    ptx::split_h2(v1.z, v1.w, hi.w, lo.w);
-                    const uint32_t to = base + (ch >> 3) * C::kQSub + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::kQTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+            constexpr int kCh = C::D / 8, kStep = 64 / kCh, kDeep = 4;   // places a row; rows a step of both warps
+            const int ch = lane % kCh, t0 = w.tok0(a);
+            const int rows = min(a.tq, w.s.rows - t0) * a.G;
+            const char* q0 = a.q + (size_t)(w.s.row0 + t0) * a.q_tok + (size_t)w.h * a.G * a.q_head + ch * 32;
+            const uint32_t to0 = qs + (ch >> 3) * C::kQSub;
+            for (int r0 = (lane + 32 * part) / kCh; r0 < rows; r0 += kStep * kDeep) {
+                float4 v[kDeep][2];
+#pragma unroll
+                for (int k = 0; k < kDeep; ++k) {
+                    const int r = r0 + k * kStep;
+                    if (r < rows) {
+                        const char* p = q0 + (size_t)a.by_g.quot(r) * a.q_tok + (size_t)a.by_g.rem(r) * a.q_head;
+                        v[k][0] = ptx::ld_act(reinterpret_cast<const float4*>(p));
+                        v[k][1] = ptx::ld_act(reinterpret_cast<const float4*>(p + 16));
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kDeep; ++k) {
+                    const int r = r0 + k * kStep;
+                    if (r < rows) {
+                        uint4 hi, lo;
+                        ptx::split_h2(v[k][0].x, v[k][0].y, hi.x, lo.x);
+                        ptx::split_h2(v[k][0].z, v[k][0].w, hi.y, lo.y);
+                        ptx::split_h2(v[k][1].x, v[k][1].y, hi.z, lo.z);
+                        ptx::split_h2(v[k][1].z, v[k][1].w, hi.w, lo.w);
+                        const uint32_t to = to0 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::kQTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                    }
                 }
             }
             fence_proxy_async_smem();
@@ -703,7 +716,7 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
     }
     if (!C::HL && !ok && piece > 0 && lane == 0) {
         const uint64_t t0 = ptx::global_ns();
-        while (!ptx::mbar_try_wait(smem_u32(&B->q_full), (piece - 1) & 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+        while (!ptx::mbar_try_wait(bar, (piece - 1) & 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
         }
     }
 }
@@ -933,7 +946,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
             mbar_init(smem_u32(&B->full[i]), 1);
             mbar_init(smem_u32(&B->empty[i]), 1);
         }
-        mbar_init(smem_u32(&B->q_full), 1);
+        mbar_init(smem_u32(&B->q_full), C::HL ? 2 : 1);
         mbar_init(smem_u32(&B->q_empty), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&B->o_step[i]), 1);
@@ -962,9 +975,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     // Registers: the launch's share is 168 a thread with 384 threads and 128 with 512; a wait
     // for more than the launch's sum would not end.
     constexpr int kShare = C::kThreads == 512 ? 128 : (C::kThreads == 384 ? 168 : 255);
-    constexpr int kSoft = C::HL ? (C::D == 64 ? 160 : (C::D == 128 ? 176 : 104)) : (C::NS == 2 ? 208 : 255);
-    constexpr int kCorr = C::HL ? (C::D == 64 ? 120 : (C::D == 128 ? 216 : 168)) : 0;
-    constexpr int kRest = C::HL ? (C::D == 128 ? 112 : 72) : (C::NS == 2 ? 88 : 255);
+    constexpr int kSoft = C::HL ? (C::D == 64 ? 152 : (C::D == 128 ? 176 : 104)) : (C::NS == 2 ? 208 : 255);
+    constexpr int kCorr = C::HL ? (C::D == 64 ? 112 : (C::D == 128 ? 216 : 160)) : 0;
+    constexpr int kRest = C::HL ? (C::D == 256 ? 88 : (C::D == 128 ? 112 : 96)) : (C::NS == 2 ? 88 : 255);
     static_assert(kSoft * C::kSoftWarps + kCorr * C::kCorrWarps + kRest * 4 <= kShare * (C::kThreads / 32), "registers");
     if (warp >= 0 && warp < C::kSoftWarps) {
         set_registers<kShare, kSoft>();
@@ -979,8 +992,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
         set_registers<kShare, kRest>();
         if (warp == -4) load_role<C>(a, B, ring, lane);
         else if (warp == -3) mma_role<C>(a, B, qs, ring, tmem, lane);
-        else if (warp == -2) q_role<C>(a, B, qs, lane);
-        else if (lane == 0) head_role<C>(a, B);
+        else if (C::HL || warp == -2) q_role<C>(a, B, qs, warp + 2, lane);
+        if (warp == -1 && lane == 0) head_role<C>(a, B);
     }
     tc_fence_before();
     __syncthreads();
@@ -1003,7 +1016,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_con
     const int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5);
     const Seq s = paged::load_seq(a.c, hb);
     const int in = row % 128, slot = row / 128;
-    const int tok = (t * tiles + slot) * a.tq + in / a.G;
+    const int tok = (t * tiles + slot) * a.tq + a.by_g.quot(in);
     if (row >= a.rec_rows || in >= a.tq * a.G || tok >= s.rows) return;
     auto rec = [&](int i) { return ((size_t)i * 2 + (i == c ? 1 : 0)) * a.rec_rows + row; };
     // lanes share the records' scales out, then every lane owns dims
@@ -1027,7 +1040,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_con
         }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int q = s.row0 + tok, head = h * a.G + in % a.G;
+    const int q = s.row0 + tok, head = h * a.G + a.by_g.rem(in);
     char* dst = a.dst + (size_t)q * a.d_tok + (size_t)head * a.d_head;
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
@@ -1109,6 +1122,7 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     const bool f32 = d->type == MLZC_TYPE_F32;
     a.G = (int)(d->n_head_q / cache->n_head_kv);
     a.tq = 128 / a.G;
+    a.by_g.set((uint32_t)a.G);
     a.box = std::gcd(cache->page_size, BN);
     if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
     if ((st = paged::encode_pool(&a.mv, cache, true, a.box)) != MLZC_OK) return st;

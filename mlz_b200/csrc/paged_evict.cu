@@ -5,12 +5,19 @@
 // and of the candidates between them the m = budget - n_sink - n_recent of the largest weight,
 // ties to the lowest slot.  Two launches:
 //   select: the m-th largest key by a radix select (weights mapped to integers of the same
-//           order), then one pass in slot order that numbers the freed slots below the budget
-//           (holes) and the kept ones behind it (movers).  There are as many of the one as of
-//           the other, so mover r goes to hole r.
+//           order, three passes of 11, 11 and 10 bits), then the freed slots below the budget
+//           (holes) and the kept ones behind it (movers) numbered in slot order.  There are as
+//           many of the one as of the other, so mover r goes to hole r.
 //   move:   rows of K and V from movers to holes.  Every source lies at or behind the budget
 //           and every target before it, so rows move in place, in any order, and only those
 //           that have to (order-keeping compaction would move nearly all of them).
+// The move is bound by HBM: 16 sequences of 512 to 8192 slots x 8 heads x 128 dims cut to 1000 take
+// 16 us for 90 MB.  The selection is bound by latency, by passes that depend on one another and
+// cost a dozen instructions a slot on the one SM that has the head: 20 us for 8192 slots.  Where
+// heads are few, a cluster of up to 8 CTAs shares one, its histograms and counts read over
+// distributed shared memory: 24 us for 32768 slots (41 with one CTA), 33 for 131072.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "paged.h"
@@ -21,9 +28,9 @@ namespace {
 
 using paged::View;
 
-constexpr int kSelThreads = 1024;
-constexpr int kItems = 4;                     // slots a thread takes per ordered step
-constexpr int kBins = 2048;                   // 11 bits a radix pass: 11 + 11 + 10
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;                   // 11 bits a radix pass
+constexpr int kHeldSlots = 24576;             // weights of so many slots fit beside a second CTA's
 
 struct EvictArgs {
     View c;
@@ -33,6 +40,9 @@ struct EvictArgs {
     char* kept;
     int* kv_len_out;
     int* holes;                               // workspace: [batch][head][budget]
+    uint32_t* words;                          // workspace: [batch][head][n_words], a bit a slot that stays
+    int n_words;
+    int held;                                 // slots of shared memory for weights (0: read from global memory)
     size_t w_head, w_seq, o_head, o_seq, kept_head, kept_seq;
 };
 
@@ -43,143 +53,223 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Inclusive sums of (a, b) over the block's threads in order; totals in *ta, *tb.  sh: 64 ints.
-__device__ __forceinline__ void block_scan2(int& a, int& b, int* ta, int* tb, int* sh) {
+namespace cg = cooperative_groups;
+
+constexpr int kRanks = 8;                     // CTAs of a cluster at most (the portable size)
+constexpr int kShare = 4096;                  // slots worth a CTA of a cluster (its barriers cost 1 us each)
+
+// Shared memory of a selecting CTA.
+struct Sel {
+    int4 hist[3][kBins / 4];                  // of each pass
+    int sums[6][kSelWarps];                   // warps' sums, a row a scan
+    int found[3][3];                          // the digit, how many keys lie above it, how many have it
+    int count[3];                             // this CTA's equals, holes, movers
+    int listed;
+    uint32_t list[2048];                      // keys with the first digit found, where they are few
+};
+constexpr int kList = 2048;
+
+__device__ __forceinline__ int warp_sum(int x) { return __reduce_add_sync(~0u, x); }
+
+// Sum of a warp-wide value over the warps before this one, and over all: sh is a row of sums.
+__device__ __forceinline__ int warps_before(int mine, int* total, int* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(~0u, a, o), y = __shfl_up_sync(~0u, b, o);
-        if (lane >= o) { a += x; b += y; }
-    }
-    if (lane == 31) { sh[warp] = a; sh[32 + warp] = b; }
+    if (lane == 0) sh[warp] = mine;
     __syncthreads();
-    if (warp == 0) {
-        int x = sh[lane], y = sh[32 + lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int p = __shfl_up_sync(~0u, x, o), q = __shfl_up_sync(~0u, y, o);
-            if (lane >= o) { x += p; y += q; }
-        }
-        sh[lane] = x;
-        sh[32 + lane] = y;
-    }
-    __syncthreads();
-    if (warp > 0) { a += sh[warp - 1]; b += sh[32 + warp - 1]; }
-    *ta = sh[31];
-    *tb = sh[63];
-    __syncthreads();
+    const int x = lane < kSelWarps ? sh[lane] : 0;
+    *total = warp_sum(x);
+    return warp_sum(lane < warp ? x : 0);
 }
 
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictArgs a) {
-    __shared__ int hist[kBins];
-    __shared__ int sh[64];
-    __shared__ int found[2];                  // the digit, and how many keys lie above it
+    __shared__ Sel sel;
+    extern __shared__ float held[];
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int n = paged::load_seq(a.c, b, false).kv;
     const int size = min(n, a.budget);
     const float* w = reinterpret_cast<const float*>(a.w + (size_t)b * a.w_seq + (size_t)h * a.w_head);
     float* wo = reinterpret_cast<float*>(a.w_out + (size_t)b * a.o_seq + (size_t)h * a.o_head);
     int* kept = reinterpret_cast<int*>(a.kept + (size_t)b * a.kept_seq + (size_t)h * a.kept_head);
     int* holes = a.holes + ((size_t)b * a.c.n_head_kv + h) * a.budget;
-    for (int i = size + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
-    if (n <= a.budget) {
-        for (int i = tid; i < n; i += kSelThreads) {
+    auto sync = [&]() {
+        if (ranks == 1) __syncthreads();
+        else cluster.sync();
+    };
+    const int all = kSelThreads * ranks, me = rank * kSelThreads + tid;
+    for (int i = size + me; i < a.budget; i += all) kept[i] = -1;
+    if (n <= a.budget) {                      // alike for the whole cluster
+        for (int i = me; i < n; i += all) {
             kept[i] = i;
             if (wo != w) wo[i] = ptx::ld_act(w + i);
         }
         return;
     }
+    // This CTA's run of slots (whole words of 32), and each warp's within it: lane l of a warp has
+    // every 32nd slot, so that loads and stores are whole lines and a slot's rank is a count of
+    // ballot bits.  Short loops on purpose: each phase runs once a launch, and with 16 slots a
+    // lane unrolled the selection of 8 heads of 32768 slots took 35 us.
+    const int lane = tid & 31, warp = tid >> 5;
+    const int share = ((n + ranks - 1) / ranks + 31) / 32 * 32, s0 = min(n, rank * share), s1 = min(n, s0 + share);
+    const int run = ((share + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, w0 = min(s1, s0 + warp * run), w1 = min(s1, w0 + run);
+    const bool hold = share <= a.held;
+    const uint32_t below = (1u << lane) - 1;
+    uint32_t* words = a.words + ((size_t)b * a.c.n_head_kv + h) * a.n_words;
+    if (hold) {
+#pragma unroll 4
+        for (int i = w0 + lane; i < w1; i += 32) held[i - s0] = ptx::ld_act(w + i);   // read by the same lane alone
+    }
+    // f(slot, weight) for this lane's slots; every lane of the warp comes along (slots at or past
+    // w1 are none of its)
+    auto each = [&](auto f) {
+#pragma unroll 2
+        for (int i = w0 + lane; i - lane < w1; i += 32) f(i, i < w1 ? (hold ? held[i - s0] : ptx::ld_act(w + i)) : 0.0f);
+    };
+    // the same with the bits of the 32 slots that stay
+    auto each_word = [&](auto f) {
+#pragma unroll 2
+        for (int i = w0 + lane; i - lane < w1; i += 32) f(i, *reinterpret_cast<volatile uint32_t*>(words + (i >> 5)));
+    };
+    auto weight = [&](int i) { return hold ? held[i - s0] : ptx::ld_act(w + i); };
     const int lo = a.sink, hi = n - a.recent;          // candidates
     int need = a.budget - a.sink - a.recent;           // of which so many stay (fewer than hi - lo)
+    const bool choose = need > 0;
     uint32_t prefix = 0, mask = 0;
-    if (need > 0) {
+    if (choose) {
+        for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) sel.hist[0][i] = make_int4(0, 0, 0, 0);
+        if (tid == 0) sel.listed = 0;
+        __syncthreads();
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11, bins = 1 << bits;
-            for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = lo + tid; i < hi; i += kSelThreads) {
-                const uint32_t k = order_key(ptx::ld_act(w + i));
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+            int* hist = reinterpret_cast<int*>(sel.hist[pass]);
+            const bool few = pass > 0 && sel.found[0][2] <= kList;
+            if (few && pass == 2) {
+                for (int i = tid; i < sel.listed; i += kSelThreads)
+                    if ((sel.list[i] & mask) == prefix) atomicAdd(&hist[sel.list[i] & (bins - 1)], 1);
+            } else {
+                each([&](int i, float v) {
+                    const uint32_t k = order_key(v);
+                    const bool in = i < w1 && i >= lo && i < hi && (k & mask) == prefix;
+                    if (in) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+                    if (few && in) sel.list[atomicAdd(&sel.listed, 1)] = k;
+                });
             }
-            __syncthreads();
-            // from the top: the digit whose keys hold the need-th largest; each thread owns two
-            const int d0 = bins - 1 - 2 * tid;
-            const int c0 = 2 * tid < bins ? hist[d0] : 0, c1 = 2 * tid < bins ? hist[d0 - 1] : 0;
-            int upto = c0 + c1, unused = 0, t0, t1;
-            block_scan2(upto, unused, &t0, &t1, sh);
-            const int before = upto - c0 - c1;
-            if (before < need && need <= upto) {
-                const bool second = need > before + c0;
-                found[0] = second ? d0 - 1 : d0;
-                found[1] = second ? before + c0 : before;
-            }
-            __syncthreads();
-            prefix |= (uint32_t)found[0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            need -= found[1];
-            __syncthreads();
-        }
-    }
-    // keys above `prefix` stay, and the first `need` equal to it
-    int equal_seen = 0, hole_seen = 0, mover_seen = 0;
-    for (int base = 0; base < n; base += kSelThreads * kItems) {
-        const int i0 = base + tid * kItems;
-        float x[kItems];
-        bool eq[kItems], stay[kItems];
-        int ne = 0;
-#pragma unroll
-        for (int j = 0; j < kItems; ++j) {
-            const int i = i0 + j;
-            x[j] = i < n ? ptx::ld_act(w + i) : 0.0f;
-            const uint32_t k = order_key(x[j]);
-            const bool cand = i >= lo && i < hi;
-            eq[j] = cand && a.budget > a.sink + a.recent && k == prefix;
-            stay[j] = i < n && (!cand || (a.budget > a.sink + a.recent && k > prefix));
-            ne += eq[j];
-        }
-        int ie = ne, unused = 0, te, t1;
-        block_scan2(ie, unused, &te, &t1, sh);
-        int r = equal_seen + ie - ne;
-        int nh = 0, nm = 0;
-#pragma unroll
-        for (int j = 0; j < kItems; ++j) {
-            if (eq[j] && r++ < need) stay[j] = true;
-            nh += i0 + j < size && !stay[j];
-            nm += i0 + j >= size && stay[j];
-        }
-        equal_seen += te;
-        int ih = nh, im = nm, th, tm;
-        block_scan2(ih, im, &th, &tm, sh);
-        int rh = hole_seen + ih - nh, rm = mover_seen + im - nm;
-#pragma unroll
-        for (int j = 0; j < kItems; ++j) {
-            const int i = i0 + j;
-            if (i < size) {
-                if (stay[j]) {
-                    kept[i] = i;
-                    if (wo != w) wo[i] = x[j];
+            sync();
+            // from the top: the digit whose keys hold the need-th largest; each thread owns four
+            const int p = tid < kBins / 4 ? bins / 4 - 1 - tid : -1;
+            int c[4] = {0, 0, 0, 0};
+            if (p >= 0) {
+                if (ranks == 1) {
+                    const int4 v = sel.hist[pass][p];
+                    c[0] = v.w; c[1] = v.z; c[2] = v.y; c[3] = v.x;
                 } else {
-                    holes[rh++] = i;
+                    int4 v[kRanks];
+#pragma unroll
+                    for (int r = 0; r < kRanks; ++r) v[r] = r < ranks ? cluster.map_shared_rank(sel.hist[pass], r)[p] : make_int4(0, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < kRanks; ++r) { c[0] += v[r].w; c[1] += v[r].z; c[2] += v[r].y; c[3] += v[r].x; }
                 }
             }
-        }
-        __syncthreads();                      // holes of this step before its movers
+            const int mine = c[0] + c[1] + c[2] + c[3];
+            int upto = mine, total;
 #pragma unroll
-        for (int j = 0; j < kItems; ++j) {
-            const int i = i0 + j;
-            if (i >= size && stay[j]) {
-                const int to = holes[rm++];
-                kept[to] = i;
-                wo[to] = x[j];
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, upto, o);
+                if (lane >= o) upto += y;
             }
+            int before = warps_before(__shfl_sync(~0u, upto, 31), &total, sel.sums[pass]) + upto - mine;
+            if (before < need && need <= before + mine) {
+                int k = 0;
+                while (need > before + c[k]) before += c[k++];
+                sel.found[pass][0] = 4 * p + 3 - k;
+                sel.found[pass][1] = before;
+                sel.found[pass][2] = c[k];
+            }
+            __syncthreads();
+            prefix |= (uint32_t)sel.found[pass][0] << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
+            need -= sel.found[pass][1];
         }
-        hole_seen += th;
-        mover_seen += tm;
     }
-    __syncthreads();                          // in place: every weight has been read
-    for (int i = size + tid; i < n; i += kSelThreads) wo[i] = 0.0f;
+    // Candidates above `prefix` stay, and the first `need` equal to it.  Counts of the CTAs before
+    // this one come from their shared memory.
+    auto from_others = [&](int which) {
+        int sum = 0;
+        if (ranks > 1) {
+#pragma unroll
+            for (int r = 0; r < kRanks; ++r) sum += r < rank ? *cluster.map_shared_rank(&sel.count[which], r) : 0;
+        }
+        return sum;
+    };
+    auto equal = [&](int i, float v) { return i < w1 && i >= lo && i < hi && order_key(v) == prefix; };
+    // equal keys need counting in order only where not all of them stay
+    const bool ties = choose && sel.found[2][2] > need;
+    int equals = 0, total;
+    if (ties) {
+        int mine = 0;
+        each([&](int i, float v) { mine += __popc(__ballot_sync(~0u, equal(i, v))); });
+        equals = warps_before(mine, &total, sel.sums[3]);
+        if (tid == 0) sel.count[0] = total;
+        sync();
+        equals += from_others(0);
+    }
+    // which slots stay, and how many are holes and movers
+    int nh = 0, nm = 0;
+    each([&](int i, float v) {
+        const uint32_t k = order_key(v);
+        const bool inside = i >= lo && i < hi;
+        bool s = !inside || (choose && k >= prefix);
+        if (ties) {
+            const bool eq = i < w1 && inside && k == prefix;
+            const uint32_t bits = __ballot_sync(~0u, eq);
+            if (eq) s = equals + __popc(bits & below) < need;
+            equals += __popc(bits);
+        }
+        const uint32_t stay = __ballot_sync(~0u, i < w1 && s);
+        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(words + (i >> 5)) = stay;
+        const int i0 = i - lane;
+        const uint32_t real = w1 - i0 >= 32 ? ~0u : (1u << (w1 - i0)) - 1, front = size - i0 >= 32 ? ~0u : (size > i0 ? (1u << (size - i0)) - 1 : 0);
+        nh += __popc(real & front & ~stay);
+        nm += __popc(stay & ~front);
+    });
+    __syncwarp();
+    int th, tm;
+    int rh = warps_before(nh, &th, sel.sums[4]), rm = warps_before(nm, &tm, sel.sums[5]);
+    if (tid == 0) {
+        sel.count[1] = th;
+        sel.count[2] = tm;
+    }
+    sync();
+    rh += from_others(1);
+    rm += from_others(2);
+    if (w0 < size)
+        each_word([&](int i, uint32_t stay) {
+            const bool mine = i < w1 && i < size, s = stay >> lane & 1, hole = mine && !s;
+            const uint32_t bits = __ballot_sync(~0u, hole);
+            if (hole) holes[rh + __popc(bits & below)] = i;
+            rh += __popc(bits);
+            if (mine && s) {
+                kept[i] = i;
+                if (wo != w) wo[i] = weight(i);
+            }
+        });
+    sync();                                   // every hole is listed, every count read
+    if (w1 > size)
+        each_word([&](int i, uint32_t stay) {
+            const bool mover = i >= size && (stay >> lane & 1);
+            const uint32_t bits = __ballot_sync(~0u, mover);
+            if (mover) {
+                const int to = holes[rm + __popc(bits & below)];
+                kept[to] = i;
+                wo[to] = weight(i);
+            }
+            rm += __popc(bits);
+            if (i >= size && i < w1) wo[i] = 0.0f;
+        });
 }
 
 constexpr int kMoveWarps = 8;
@@ -251,8 +341,39 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_kernel(const __grid_cons
     }
 }
 
+int launch_select(EvictArgs& a, const DeviceCtx* c, cudaStream_t s) {
+    // CTAs of kShare slots, as long as every head's are on the GPU together
+    int ranks = 1;
+    while (ranks < kRanks && (int64_t)a.c.n_head_kv * a.c.batch * 2 * ranks <= c->sm_count && a.c.cap > ranks * kShare) ranks *= 2;
+    a.held = std::min(kHeldSlots, (a.c.cap + ranks - 1) / ranks);
+    const size_t smem = (size_t)a.held * 4;
+    static bool set[64] = {};
+    const int dev = c->device < 64 ? c->device : 63;
+    if (!set[dev] || c->device >= 64) {
+        MLZC_CUDA_TRY(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldSlots * 4));
+        set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ranks, a.c.n_head_kv, a.c.batch);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap_mode() == MLZC_OVERLAP_OFF ? 1 : 2;
+    MLZC_CUDA_TRY(cudaLaunchKernelEx(&cfg, select_kernel, a));
+    MLZC_CUDA_TRY(cudaGetLastError());
+    return MLZC_OK;
+}
+
+size_t evict_words(const mlzc_paged_cache* cache) { return ((size_t)cache->max_pages * cache->page_size + 31) / 32; }
 size_t evict_workspace(const mlzc_paged_cache* cache, const mlzc_paged_evict_desc* d) {
-    return ((size_t)cache->batch_size * cache->n_head_kv * d->budget * 4 + 15) / 16 * 16;
+    return ((size_t)cache->batch_size * cache->n_head_kv * (d->budget + evict_words(cache)) * 4 + 15) / 16 * 16;
 }
 
 int check_table(const char* what, const void* p, const size_t* nb, int64_t heads, int64_t batch, size_t row) {
@@ -319,12 +440,14 @@ extern "C" int mlzc_paged_evict_dev(const mlzc_paged_cache* cache, const mlzc_pa
     a.kept = reinterpret_cast<char*>(d->kept);
     a.kv_len_out = d->kv_len_out;
     a.holes = static_cast<int*>(workspace);
+    a.n_words = (int)evict_words(cache);
+    a.words = reinterpret_cast<uint32_t*>(a.holes + (size_t)a.c.batch * a.c.n_head_kv * a.budget);
     a.w_head = d->weights_nb[1]; a.w_seq = d->weights_nb[2];
     a.o_head = d->weights_out_nb[1]; a.o_seq = d->weights_out_nb[2];
     a.kept_head = d->kept_nb[1]; a.kept_seq = d->kept_nb[2];
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    MLZC_CUDA_TRY(launch_pdl(select_kernel, dim3(a.c.n_head_kv, a.c.batch), dim3(kSelThreads), 0, s, a));
-    MLZC_CUDA_TRY(cudaGetLastError());
+    st = launch_select(a, c, s);
+    if (st != MLZC_OK) return st;
     // slots past the table's capacity cannot be kept
     const int slots = std::min(a.budget, a.c.cap);
     const dim3 g((unsigned)((slots + kMoveSlots - 1) / kMoveSlots), (unsigned)a.c.n_head_kv, (unsigned)a.c.batch);

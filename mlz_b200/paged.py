@@ -50,9 +50,10 @@ class _Launch:
             self.handle = int(stream)
             self.given = torch.cuda.ExternalStream(self.handle, device=device) if self.handle else torch.cuda.default_stream(device)
 
-    def empty(self, shape, dtype):
+    def empty(self, shape, dtype, like):
+        """An uninitialised tensor beside `like` (new_empty costs half of torch.empty here)."""
         if self.given is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return like.new_empty(shape, dtype=dtype)
         with torch.cuda.stream(self.given):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
@@ -202,7 +203,7 @@ def paged_store(cache, k, v, *, q=None, q_out=None, positions=None, sections=Non
     if q is not None:
         hq, qnb = q.shape[1], _rows("q", q, cache, None, k.dtype)
         if q_out is None:
-            q_out = L.empty(q.shape, q.dtype)
+            q_out = L.empty(q.shape, q.dtype, q)
         if q_out.shape != q.shape:
             raise ValueError(f"q_out {tuple(q_out.shape)}, q {tuple(q.shape)}")
         onb = _rows("q_out", q_out, cache, None, k.dtype)
@@ -234,12 +235,12 @@ def _attn_desc(cache, q, scale, softcap, out=None, lse=None):
                                                      q.data_ptr(), dst, *qnb, *dnb, lp, *lnb))
 
 
-def _given(workspace, need, L):
+def _given(workspace, need, L, like):
     """(pointer, bytes, owner) of the caller's workspace, or of one made here."""
     if workspace is None:
         if not need:
             return None, 0, None
-        workspace = L.empty(need, _U8)
+        workspace = L.empty(need, _U8, like)
     elif workspace.device != L.device or not workspace.is_contiguous():
         raise ValueError(f"workspace: a contiguous tensor on {L.device} is expected")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -259,14 +260,14 @@ def paged_attn(cache, q, scale, *, softcap=0.0, out=None, lse=None, return_lse=F
     float32 or return_lse, (out, lse).  Rows that belong to no sequence are left as they were."""
     L = _Launch(cache.device, stream)
     if out is None:
-        out = L.empty(q.shape, q.dtype)
+        out = L.empty(q.shape, q.dtype, q)
     if lse is None and return_lse:
-        lse = L.empty(q.shape[:2], _F32)
+        lse = L.empty(q.shape[:2], _F32, q)
     d = C.byref(_attn_desc(cache, q, scale, softcap, out, lse))
     T = q.shape[0]
     cd = C.byref(cache._with(T))
     need = cache._workspace(L, lib().mlzc_paged_attn_workspace_bytes, ("attn", T, q.shape[1], q.dtype), cd, d)
-    ws, n, owner = _given(workspace, need, L)
+    ws, n, owner = _given(workspace, need, L, q)
     L.run(lib().mlzc_paged_attn_dev, cd, d, ws, n, L.handle)
     return (out, lse) if lse is not None else out
 
@@ -279,7 +280,7 @@ def paged_weights(cache, q, lse, scale, *, softcap=0.0, acc=None, out=None, work
     L = _Launch(cache.device, stream)
     d = C.byref(_attn_desc(cache, q, scale, softcap, None, lse))
     if out is None:
-        out = L.empty((cache.batch, cache.n_head_kv, cache.capacity), _F32)
+        out = L.empty((cache.batch, cache.n_head_kv, cache.capacity), _F32, q)
         if L.given is None:
             out.zero_()
         else:
@@ -291,7 +292,7 @@ def paged_weights(cache, q, lse, scale, *, softcap=0.0, acc=None, out=None, work
     T = q.shape[0]
     cd = C.byref(cache._with(T))
     need = cache._workspace(L, lib().mlzc_paged_weights_workspace_bytes, ("weights", T, q.shape[1], q.dtype), cd, d)
-    ws, n, owner = _given(workspace, need, L)
+    ws, n, owner = _given(workspace, need, L, q)
     L.run(lib().mlzc_paged_weights_dev, cd, d, acc.data_ptr() if acc is not None else None, anb, out.data_ptr(), onb, ws, n, L.handle)
     return out
 
@@ -307,7 +308,7 @@ def paged_evict(cache, weights, budget, *, n_sink=0, n_recent=0, weights_out=Non
     if weights_out is None:
         weights_out = weights
     if kept is None:
-        kept = L.empty((cache.batch, cache.n_head_kv, budget), _I32)
+        kept = L.empty((cache.batch, cache.n_head_kv, budget), _I32, weights)
     if kv_len_out is None:
         kv_len_out = cache.kv_len
     if tuple(kv_len_out.shape) != (cache.batch,) or kv_len_out.dtype != _I32 or not kv_len_out.is_contiguous() or \
@@ -318,7 +319,7 @@ def paged_evict(cache, weights, budget, *, n_sink=0, n_recent=0, weights_out=Non
         *_table("weights_out", weights_out, cache, cache.capacity, _F32), kept.data_ptr(), *_table("kept", kept, cache, budget, _I32),
         kv_len_out.data_ptr())))
     cd = C.byref(cache._desc)
-    ws, n, owner = _given(workspace, cache._workspace(L, lib().mlzc_paged_evict_workspace_bytes, ("evict", budget), cd, d), L)
+    ws, n, owner = _given(workspace, cache._workspace(L, lib().mlzc_paged_evict_workspace_bytes, ("evict", budget), cd, d), L, weights)
     L.run(lib().mlzc_paged_evict_dev, cd, d, ws, n, L.handle)
     return kept, weights_out, kv_len_out
 
