@@ -13,11 +13,13 @@
 // chunks, reading K that for decode.  kPolyEvery moves a share of the exponentials to the FMA
 // pipe.
 //
-// A CTA takes 128 slots of a head (K tile, held) and walks their query tiles: loader warp (K by
-// one TMA box a page piece, Q by one box a 64-dim block, all into one ring of units), MMA warp
-// (scores into four TMEM buffers, as many columns as there are rows), lse warp (a tile's lse2
-// into shared memory), two warpgroups that take turns at the tiles.  f32 queries come as f16 hi
-// + lo from a small preparing launch, low products summed first.
+// A piece of work is what one operand is held for: a slot tile (K) and its query tiles, or,
+// where a sequence's rows fill one query tile at most (decode), that tile (Q) and a run of slot
+// tiles.  The held operand and the passing one share a ring of shared-memory units: loader warp
+// (K by one TMA box a page piece, Q by one box a 64-dim block), MMA warp (scores into four TMEM
+// buffers, as many columns as there are rows), two lse warps (a tile's lse2 into shared memory),
+// two warpgroups that take turns at the tiles.  f32 queries come as f16 hi + lo from a small
+// preparing launch, low products summed first.
 //
 // Slot tiles x query tiles of a call form one list cut into equal shares, as in paged_attn.cu;
 // a cut slot tile's 128 partial sums are merged in order by a last launch.
@@ -25,6 +27,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <cstring>
 #include <numeric>
 
@@ -47,7 +50,8 @@ using namespace tc05;
 constexpr int kSmemMax = 232448;
 constexpr int kBN = 128;               // slots a tile
 constexpr int kBufs = 4;               // score buffers in TMEM (128 columns each) and lse tiles
-constexpr int kFixed = 512 + kBufs * 128 * 4 + 2 * 128 * 4;   // barriers, lse tiles, sums handed over
+constexpr int kBarBytes = 512;
+constexpr int kFixed = kBarBytes + kBufs * 128 * 4 + 2 * 128 * 4;   // barriers, lse tiles, sums handed over
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 4) * 32;
 constexpr int kPolyEvery = 4;          // of so many pairs of exponentials one goes to the FMA pipe
@@ -81,8 +85,11 @@ struct Cfg {
     static constexpr int ST = kFit > 12 ? 12 : kFit;
     static constexpr size_t kSmem = 1024 + kFixed + (size_t)ST * kUnit;
     static constexpr int QU = UN * (HL ? 2 : 1);      // units of a Q tile
-    static_assert(ST >= UN + 2, "ring");
+    static_assert(ST >= QU + 2 && ST >= UN + 2, "ring");
 };
+
+// Address of element i of a barrier array, from the base address `bars` at hand.
+#define MLZC_BAR(member, i) (bars + (uint32_t)offsetof(Bars, member) + 8u * (uint32_t)(i))
 
 struct Bars {
     uint64_t full[12], empty[12], s_full[kBufs], s_empty[kBufs], lse_full[kBufs], hand_full[2], hand_empty[2];
@@ -92,7 +99,7 @@ struct Bars {
     int b, h, t, tile;
     long long scan[kThreads / 32];
 };
-static_assert(sizeof(Bars) <= 512, "barriers");
+static_assert(sizeof(Bars) <= kBarBytes, "barriers");
 
 // Query tiles of slot tile t: from the first one with a row that sees slot 128 t on; one at
 // least, so that every slot below kv_len is written.
@@ -118,11 +125,13 @@ struct Tiles {
 };
 
 struct Walk {
-    int b, h, t, tile, n;
+    int b, h, t, tile, n;      // sequence, kv head, slot tile, query tile (after first_tile), tiles
+    bool wide;                 // tiles of one query tile: slot tiles t .. t + n - 1
+    int lead, tiles, all;      // first_tile and tiles_of of slot tile t; slot tiles of the head
     long long left;
     Seq s;
     bool first;
-    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(B->tile), n(0), left(B->count), first(true) {}
+    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(B->tile), n(0), wide(false), left(B->count), first(true) {}
     __device__ bool next(const WeightArgs& a) {
         if (left <= 0) return false;
         if (first) {
@@ -130,7 +139,8 @@ struct Walk {
             first = false;
         } else {
             tile = 0;
-            if ((long long)(++t) * kBN >= s.kv) {
+            t += wide ? n : 1;
+            if (t >= all) {
                 t = 0;
                 if (++h == a.c.n_head_kv) {
                     h = 0;
@@ -140,15 +150,20 @@ struct Walk {
                 }
             }
         }
-        n = (int)min((long long)(tiles_of(a, s, t) - tile), left);
+        all = (s.kv + kBN - 1) / kBN;
+        wide = s.rows <= a.tq;
+        lead = wide ? 0 : first_tile(a, s, t);
+        tiles = wide ? 1 : tiles_of(a, s, t);
+        n = (int)min((long long)(wide ? all - t : tiles - tile), left);
         left -= n;
         return true;
     }
-    __device__ bool ends(const WeightArgs& a) const { return tile + n == tiles_of(a, s, t); }
-    // first token of the piece's query tile i, and its columns
-    __device__ int tok0(const WeightArgs& a, int i) const { return (first_tile(a, s, t) + tile + i) * a.tq; }
+    __device__ bool whole() const { return wide || (tile == 0 && n == tiles); }
+    // of the piece's tile i: slot tile, first token, columns, slots
+    __device__ int slot_tile(int i) const { return wide ? t + i : t; }
+    __device__ int tok0(const WeightArgs& a, int i) const { return wide ? 0 : (lead + tile + i) * a.tq; }
     __device__ int cols(const WeightArgs& a, int i) const { return max(0, min(a.tq, s.rows - tok0(a, i))) * a.G; }
-    __device__ int slots() const { return min(kBN, s.kv - t * kBN); }
+    __device__ int slots(int i) const { return min(kBN, s.kv - slot_tile(i) * kBN); }
 };
 
 __device__ void plan(const WeightArgs& a, Bars* B) {
@@ -212,6 +227,7 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
     const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const uint32_t bars = smem_u32(B);
     volatile int* abort = &B->abort;
     // weights of columns i, i + 1 where they count: outside [from, cols) a score may hold anything
     auto some = [&](const float* x, const float* lt, int i, int from, int cols) {
@@ -220,49 +236,46 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
             y0 = capped(y0, cap_in, a.softcap);
             y1 = capped(y1, cap_in, a.softcap);
         }
-        y0 = ex2(fmaf(y0, c2, -lt[i]));
-        y1 = ex2(fmaf(y1, c2, -lt[i + 1]));
+        y0 = ex2(fmaf(y0, c2, lt[i]));
+        y1 = ex2(fmaf(y1, c2, lt[i + 1]));
         return pair(i >= from && i < cols ? y0 : 0.0f, i + 1 >= from && i + 1 < cols ? y1 : 0.0f);
     };
     uint32_t g = 0, item = 0;
     Walk w(B);
     while (w.next(a)) {
-        // a piece of one tile (decode) is all of one warpgroup's; of a longer one the second
-        // warpgroup hands its sums to the first, which writes
-        const bool alone = w.n == 1;
-        if (alone && (int)(g & 1) != turn) {
-            ++g;
-            continue;
-        }
-        const bool writes = alone || turn == 0, whole = w.tile == 0 && w.ends(a);
-        const bool busy = (warp & 3) * 32 < w.slots(), real = slot < w.slots();
-        const int j = w.t * kBN + slot;
-        float before = 0.0f, total = 0.0f;
-        if (writes && whole && real && a.acc)
-            before = ptx::ld_act(reinterpret_cast<const float*>(a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head) + j);
+        const bool whole = w.whole();
+        // a slot tile with several query tiles: the second warpgroup hands its sums to the first
+        const bool shared = !w.wide && w.n > 1;
+        const char* acc = a.acc ? a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head : nullptr;
+        float* out = reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head);
+        const int past = w.s.kv - w.s.rows;
+        float total = 0.0f, before = 0.0f;
+        bool mine = false;                    // this warpgroup had a tile of the piece
         for (int it = 0; it < w.n; ++it, ++g) {
             if ((int)(g & 1) != turn) continue;
-            const int buf = g % kBufs;
+            const int buf = g % kBufs, slots = w.slots(it), j = w.slot_tile(it) * kBN + slot;
             const uint32_t par = (g / kBufs) & 1;
-            if (!mbar_wait(smem_u32(&B->s_full[buf]), par, abort, a.c.err)) return;
-            if (!mbar_wait(smem_u32(&B->lse_full[buf]), par, abort, a.c.err)) return;
+            if (whole && acc && (w.wide || !mine) && slot < slots) before = ptx::ld_act(reinterpret_cast<const float*>(acc) + j);
+            mine = true;
+            if (!mbar_wait(MLZC_BAR(s_full, buf), par, abort, a.c.err)) return;
+            if (!mbar_wait(MLZC_BAR(lse_full, buf), par, abort, a.c.err)) return;
             tc_fence_after();
             const int cols = w.cols(a, it);
-            if (busy && cols > 0) {
+            if ((warp & 3) * 32 < slots && cols > 0) {
                 // columns [from, cols) see this thread's slot
-                const int gap = j - (w.s.kv - w.s.rows) - w.tok0(a, it);
+                const int gap = j - past - w.tok0(a, it);
                 const int from = gap > 0 ? min(gap, a.tq) * a.G : 0;
                 const float* lt = lse2 + buf * 128;
                 const uint32_t s_col = lanes + buf * 128;
                 uint64_t sum[2] = {0, 0};
                 if (C::CAP || cols <= 96 || __any_sync(~0u, from > 0)) {
 #pragma unroll 1
-                    for (int i = 0; i < cols; i += 32) {
-                        float x[32];
-                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(x));
+                    for (int i = 0; i < cols; i += 16) {
+                        float x[16];
+                        tmem_ld16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(x));
                         tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 32; k += 2) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
+                        for (int k = 0; k < 16; k += 2) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
                     }
                 } else {
                     const uint64_t c22 = pair(c2, c2);
@@ -271,19 +284,23 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
                     for (int i = 0; i < 128; i += 32)
                         tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i));
                     tmem_ld_wait();
+                    auto run = [&](int i0, int i1) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += 4) {
-                        if (i >= 96 && i + 4 > cols) {       // 128 / G is no whole number
-                            sum[0] = add2(sum[0], some(x + i, lt, i, 0, cols));
-                            sum[1] = add2(sum[1], some(x + i + 2, lt, i + 2, 0, cols));
-                        } else {
+                        for (int i = i0; i < i1; i += 4) {
                             const float4 L = *reinterpret_cast<const float4*>(lt + i);
                             float p0, p1, p2, p3;
-                            exp_pair(i / 2, fma2(pair(x[i], x[i + 1]), c22, pair(-L.x, -L.y)), p0, p1);
-                            exp_pair(i / 2 + 1, fma2(pair(x[i + 2], x[i + 3]), c22, pair(-L.z, -L.w)), p2, p3);
+                            exp_pair(i / 2, fma2(pair(x[i], x[i + 1]), c22, pair(L.x, L.y)), p0, p1);
+                            exp_pair(i / 2 + 1, fma2(pair(x[i + 2], x[i + 3]), c22, pair(L.z, L.w)), p2, p3);
                             sum[0] = add2(sum[0], pair(p0, p1));
                             sum[1] = add2(sum[1], pair(p2, p3));
                         }
+                    };
+                    run(0, 96);
+                    if (cols == 128) {
+                        run(96, 128);
+                    } else {
+#pragma unroll
+                        for (int i = 96; i < 128; i += 2) sum[0] = add2(sum[0], some(x + i, lt, i, 0, cols));
                     }
                 }
                 float s0, s1;
@@ -292,34 +309,38 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&B->s_empty[buf]));
+            if (lane == 0) mbar_arrive(MLZC_BAR(s_empty, buf));
+            if (w.wide) {
+                if (slot < slots) out[j] = before + total;
+                total = 0.0f;
+                before = 0.0f;
+            }
         }
-        if (!alone) {
+        if (w.wide) continue;
+        if (shared) {
             float* there = handed + (item & 1) * 128;
-            const uint32_t full = smem_u32(&B->hand_full[item & 1]), empty = smem_u32(&B->hand_empty[item & 1]), par = (item >> 1) & 1;
+            const uint32_t full = MLZC_BAR(hand_full, item & 1), empty = MLZC_BAR(hand_empty, item & 1), par = (item >> 1) & 1;
             ++item;
             if (turn == 1) {
                 if (!mbar_wait(empty, par ^ 1, abort, a.c.err)) return;
                 there[slot] = total;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full);
-            } else {
-                if (!mbar_wait(full, par, abort, a.c.err)) return;
-                total += there[slot];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty);
+                continue;
             }
+            if (!mbar_wait(full, par, abort, a.c.err)) return;
+            total += there[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty);
+        } else if (!mine) {
+            continue;
         }
-        if (!writes) continue;
-        if (whole) {
-            if (real) reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head)[j] = before + total;
-        } else {
-            a.rec[((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * 128 + slot] = total;
-        }
+        if (!whole) a.rec[((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * 128 + slot] = total;
+        else if (slot < w.slots(0)) out[w.t * kBN + slot] = before + total;
     }
 }
 
-// The order in which loader and MMA warp go round the ring: slots that hold the K tile at hand
+// The order in which loader and MMA warp go round the ring: slots that hold the operand at hand
 // are passed over.  A slot's phase is the parity of its uses.
 template <int ST>
 struct Ring {
@@ -336,6 +357,7 @@ struct Ring {
 
 template <class C>
 __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t ring, int lane) {
+    const uint32_t bars = smem_u32(B);
     volatile int* abort = &B->abort;
     Ring<C::ST> r;
     uint32_t begun = 0;                                 // slots with a copy issued
@@ -343,100 +365,125 @@ __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t
     auto slot = [&](uint32_t& st) {
         uint32_t par;
         r.step(st, par);
-        if (!mbar_wait(smem_u32(&B->empty[st]), par ^ 1, abort, a.c.err)) {
+        if (!mbar_wait(MLZC_BAR(empty, st), par ^ 1, abort, a.c.err)) {
             r.uses ^= 1u << st;
             return false;
         }
         begun |= 1u << st;
         return true;
     };
-    // the page of this lane's box, one slot tile ahead
-    auto page_of = [&](const Walk& w) {
-        return lane * a.box < w.slots() ? paged::load_page(a.c, w.b, a.c.by_page.quot(w.t * kBN + lane * a.box)) : -1;
+    // the page of this lane's box of slot tile t
+    auto page_of = [&](const Walk& w, int t) {
+        const int j = t * kBN + lane * a.box;
+        return lane * a.box < kBN && j < w.s.kv ? paged::load_page(a.c, w.b, a.c.by_page.quot(j)) : -1;
     };
-    Walk w(B), ahead(B);
-    int page = ahead.next(a) ? page_of(ahead) : -1, next_page = -1;
-    for (; ok && w.next(a); page = next_page) {
-        if (ahead.next(a)) next_page = page_of(ahead);
-        const int n = (w.slots() + a.box - 1) / a.box;
-        const int j = w.t * kBN + lane * a.box;
+    auto load_k = [&](const Walk& w, int t, int page, uint32_t& taken) {
+        const int n = (min(kBN, w.s.kv - t * kBN) + a.box - 1) / a.box;
+        const int row = a.c.by_page.rem(t * kBN + lane * a.box);
         const int pg = page < 0 ? a.c.n_pages : page;   // outside the map: zeros
-        r.held = 0;
-        uint32_t held = 0;
-        for (int unit = 0; ok && unit < C::UN; ++unit) {
+#pragma unroll
+        for (int unit = 0; unit < C::UN; ++unit) {
             uint32_t st;
-            if (!(ok = slot(st))) break;
-            const uint32_t bar = smem_u32(&B->full[st]);
+            if (!slot(st)) return false;
+            const uint32_t bar = MLZC_BAR(full, st);
             if (lane == 0) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
             __syncwarp();
             if (lane < n) {
 #pragma unroll
                 for (int u = 0; u < C::SUBS; ++u)
-                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, a.c.by_page.rem(j), w.h, pg);
+                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, row, w.h, pg);
             }
-            held |= 1u << st;
+            taken |= 1u << st;
         }
-        r.held = held;
-        for (int it = 0; ok && it < w.n; ++it) {
-            if (w.cols(a, it) == 0) continue;           // a sequence without new tokens
-            const int row = w.s.row0 + w.tok0(a, it);
-            for (int unit = 0; ok && unit < C::QU; ++unit) {
-                uint32_t st;
-                if (!(ok = slot(st))) break;
-                if (lane == 0) {
-                    const uint32_t bar = smem_u32(&B->full[st]);
-                    mbar_expect_tx(bar, (uint32_t)a.tq * a.G * 128 * C::SUBS);
-                    // lo first (see scores)
-                    const CUtensorMap* map = C::HL && unit < C::UN ? &a.mql : &a.mq;
+        return true;
+    };
+    auto load_q = [&](const Walk& w, int i, uint32_t& taken) {
+        const int row = w.s.row0 + w.tok0(a, i);
 #pragma unroll
-                    for (int u = 0; u < C::SUBS; ++u)
-                        tma_load_3d(ring + st * C::kUnit + u * C::kSub, map, bar, ((unit % C::UN) * C::SUBS + u) * 64, w.h * a.G, row);
-                }
+        for (int unit = 0; unit < C::QU; ++unit) {
+            uint32_t st;
+            if (!slot(st)) return false;
+            if (lane == 0) {
+                const uint32_t bar = MLZC_BAR(full, st);
+                mbar_expect_tx(bar, (uint32_t)a.tq * a.G * 128 * C::SUBS);
+                // lo first (see the MMA warp)
+                const CUtensorMap* map = C::HL && unit < C::UN ? &a.mql : &a.mq;
+#pragma unroll
+                for (int u = 0; u < C::SUBS; ++u)
+                    tma_load_3d(ring + st * C::kUnit + u * C::kSub, map, bar, ((unit % C::UN) * C::SUBS + u) * 64, w.h * a.G, row);
             }
+            taken |= 1u << st;
+        }
+        return true;
+    };
+    Walk w(B);
+    while (ok && w.next(a)) {
+        uint32_t held = 0, passing = 0;
+        r.held = 0;
+        int page = page_of(w, w.t);
+        if (w.wide) {
+            if (w.s.rows > 0) ok = load_q(w, 0, held);
+            r.held = held;
+            for (int it = 0; ok && it < w.n; ++it) {
+                const int next = it + 1 < w.n ? page_of(w, w.t + it + 1) : -1;
+                ok = load_k(w, w.t + it, page, passing);
+                page = next;
+            }
+        } else {
+            ok = load_k(w, w.t, page, held);
+            r.held = held;
+            for (int it = 0; ok && it < w.n; ++it)
+                if (w.cols(a, it) > 0) ok = load_q(w, it, passing);
         }
     }
     if (!ok) {
         // the copies already issued land before this CTA's shared memory goes away
         for (int i = 0; i < C::ST; ++i) {
             const uint64_t t0 = ptx::global_ns();
-            while ((begun >> i & 1) && !ptx::mbar_try_wait(smem_u32(&B->full[i]), (r.uses >> i & 1) ^ 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
+            while ((begun >> i & 1) && !ptx::mbar_try_wait(MLZC_BAR(full, i), (r.uses >> i & 1) ^ 1) && ptx::global_ns() - t0 < ptx::kWaitNs) {
             }
         }
     }
 }
 
-// The lse2 of each query tile's rows; two warps take turns, so that one's loads are under way
-// while the other waits.
+// Minus the lse2 of each query tile's rows; two warps take turns, so that one's loads are under
+// way while the other waits.  Of a wide piece the rows are the same for every tile.
 __device__ __forceinline__ void lse_role(const WeightArgs& a, Bars* B, float* lse2, int turn, int lane) {
+    const uint32_t bars = smem_u32(B);
     volatile int* abort = &B->abort;
     uint32_t g = 0;
     Walk w(B);
     while (w.next(a)) {
+        float v[4];
+        bool have = false;
         for (int it = 0; it < w.n; ++it, ++g) {
             if ((int)(g & 1) != turn) continue;
             const int buf = g % kBufs;
-            const int cols = w.cols(a, it), t0 = w.s.row0 + w.tok0(a, it);
-            float v[4];
+            if (!w.wide || !have) {
+                const int cols = w.cols(a, it), t0 = w.s.row0 + w.tok0(a, it);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = lane + 32 * i;
-                v[i] = c < cols ? ptx::ld_act(reinterpret_cast<const float*>(a.lse + (size_t)(t0 + a.by_g.quot(c)) * a.lse_tok +
-                                                                             (size_t)(w.h * a.G + a.by_g.rem(c)) * a.lse_head))
-                                : INFINITY;
-                // a row that saw nothing adds nothing
-                v[i] = v[i] == -INFINITY ? INFINITY : v[i] * kLog2e;
+                for (int i = 0; i < 4; ++i) {
+                    const int c = lane + 32 * i;
+                    v[i] = c < cols ? ptx::ld_act(reinterpret_cast<const float*>(a.lse + (size_t)(t0 + a.by_g.quot(c)) * a.lse_tok +
+                                                                                 (size_t)(w.h * a.G + a.by_g.rem(c)) * a.lse_head))
+                                    : -INFINITY;
+                    // a row that saw nothing adds nothing
+                    v[i] = v[i] == -INFINITY ? -INFINITY : v[i] * -kLog2e;
+                }
+                have = true;
             }
-            if (!mbar_wait(smem_u32(&B->s_empty[buf]), ((g / kBufs) & 1) ^ 1, abort, a.c.err)) return;
+            if (!mbar_wait(MLZC_BAR(s_empty, buf), ((g / kBufs) & 1) ^ 1, abort, a.c.err)) return;
 #pragma unroll
             for (int i = 0; i < 4; ++i) lse2[buf * 128 + lane + 32 * i] = v[i];
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&B->lse_full[buf]));
+            if (lane == 0) mbar_arrive(MLZC_BAR(lse_full, buf));
         }
     }
 }
 
 template <class C>
-__device__ __forceinline__ void mma_role(const WeightArgs& a, Bars* B, uint32_t ring, uint32_t tmem) {
+__device__ __forceinline__ void mma_role(const WeightArgs& a, Bars* B, uint32_t ring, uint32_t tmem_base) {
+    const uint32_t bars = uniform(smem_u32(B)), ring16 = uniform(ring >> 4), tmem = uniform(tmem_base);
     volatile int* abort = &B->abort;
     Ring<C::ST> r;
     uint32_t g = 0, last_bar = 0, last_par = 0;
@@ -444,59 +491,103 @@ __device__ __forceinline__ void mma_role(const WeightArgs& a, Bars* B, uint32_t 
     auto take = [&](uint32_t& st) {
         uint32_t par;
         r.step(st, par);
-        if (!mbar_wait(smem_u32(&B->full[st]), par, abort, a.c.err)) return false;
+        st = uniform(st);
+        if (!mbar_wait(MLZC_BAR(full, st), par, abort, a.c.err)) return false;
         tc_fence_after();
         return true;
     };
-    auto release = [&](uint32_t st) {
-        if (elect_one()) umma_commit(smem_u32(&B->empty[st]));
-        last_bar = smem_u32(&B->empty[st]);
-        last_par = (r.uses >> st & 1) ^ 1;
+    auto commit = [&](uint32_t bar) {
+        if (elect_one()) umma_commit(bar);
     };
+    auto release = [&](uint32_t st) {
+        last_bar = MLZC_BAR(empty, st);
+        last_par = (r.uses >> st & 1) ^ 1;
+        commit(last_bar);
+    };
+    // the products of K unit ks and Q unit qs into buffer buf; `add` to what it holds
+    auto products = [&](int buf, uint32_t idesc, uint32_t ks, uint32_t qs, bool add) {
+        const uint32_t k = desc_lo(ring16 + ks * (C::kUnit >> 4)), q = desc_lo(ring16 + qs * (C::kUnit >> 4)), d = tmem + buf * 128;
+        if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < C::DU / 16; ++i) {
+                const uint32_t o = ((i >> 2) * C::kSub + (i & 3) * 32) >> 4;
+                umma_f16_lo(d, k + o, q + o, idesc, add || i > 0);
+            }
+        }
+    };
+    // as many columns as there are rows (multiples of 16)
+    auto idesc_of = [&](int cols) { return uniform(umma_idesc_f16(128, 0) | ((uint32_t)((cols + 15) / 16 * 16 >> 3) << 17)); };
     Walk w(B);
     while (ok && w.next(a)) {
-        uint32_t ks[C::UN], held = 0;
+        uint32_t held = 0;
         r.held = 0;
+        if (w.wide) {
+            const int cols = w.cols(a, 0);
+            const uint32_t idesc = idesc_of(cols);
+            uint32_t qs[C::QU];
 #pragma unroll
-        for (int unit = 0; unit < C::UN; ++unit)
-            if (ok) {
-                ok = take(ks[unit]);
-                held |= 1u << ks[unit];
-            }
-        r.held = held;
-        for (int it = 0; ok && it < w.n; ++it, ++g) {
-            const int buf = g % kBufs;
-            if (!(ok = mbar_wait(smem_u32(&B->s_empty[buf]), ((g / kBufs) & 1) ^ 1, abort, a.c.err))) break;
-            tc_fence_after();
-            const int cols = w.cols(a, it);
-            if (cols > 0) {
-                // as many columns as there are rows (multiples of 16); low products first: the
-                // tensor cores' sums are cut, not rounded, at the sum's own size
-                const uint32_t idesc = uniform(umma_idesc_f16(128, 0) | ((uint32_t)((cols + 15) / 16 * 16 >> 3) << 17));
-                const uint32_t d = uniform(tmem + buf * 128);
+            for (int unit = 0; unit < C::QU; ++unit)
+                if (ok && cols > 0) {
+                    ok = take(qs[unit]);
+                    held |= 1u << qs[unit];
+                }
+            r.held = held;
+            for (int it = 0; ok && it < w.n; ++it, ++g) {
+                const int buf = (int)uniform(g % kBufs);
+                if (!(ok = mbar_wait(MLZC_BAR(s_empty, buf), ((g / kBufs) & 1) ^ 1, abort, a.c.err))) break;
+                tc_fence_after();
 #pragma unroll
-                for (int unit = 0; unit < C::QU; ++unit) {
-                    uint32_t qs;
-                    if (ok) ok = take(qs);
+                for (int unit = 0; unit < C::UN; ++unit) {
+                    uint32_t ks;
+                    if (ok) ok = take(ks);
                     if (!ok) break;
-                    const uint32_t k_at = uniform(ring + ks[unit % C::UN] * C::kUnit), q_at = uniform(ring + qs * C::kUnit);
-                    if (elect_one()) {
-                        const uint64_t k = umma_desc_sw128(k_at), q = umma_desc_sw128(q_at);
+                    if (cols > 0) {
+                        // low products first: the tensor cores' sums are cut, not rounded, at the
+                        // sum's own size
 #pragma unroll
-                        for (int i = 0; i < C::DU / 16; ++i) {
-                            const uint32_t o = ((i >> 2) * C::kSub + (i & 3) * 32) >> 4;
-                            umma_f16(d, k + o, q + o, idesc, unit > 0 || i > 0 ? 1u : 0u);
-                        }
+                        for (int part = 0; part < C::QU / C::UN; ++part) products(buf, idesc, ks, qs[part * C::UN + unit], unit > 0 || part > 0);
                     }
-                    release(qs);
+                    release(ks);
                 }
                 if (!ok) break;
+                commit(MLZC_BAR(s_full, buf));
             }
-            if (elect_one()) umma_commit(smem_u32(&B->s_full[buf]));
-        }
-        if (!ok) break;
+            if (!ok) break;
 #pragma unroll
-        for (int unit = 0; unit < C::UN; ++unit) release(ks[unit]);
+            for (int unit = 0; unit < C::QU; ++unit)
+                if (cols > 0) release(qs[unit]);
+        } else {
+            uint32_t ks[C::UN];
+#pragma unroll
+            for (int unit = 0; unit < C::UN; ++unit)
+                if (ok) {
+                    ok = take(ks[unit]);
+                    held |= 1u << ks[unit];
+                }
+            r.held = held;
+            for (int it = 0; ok && it < w.n; ++it, ++g) {
+                const int buf = (int)uniform(g % kBufs);
+                if (!(ok = mbar_wait(MLZC_BAR(s_empty, buf), ((g / kBufs) & 1) ^ 1, abort, a.c.err))) break;
+                tc_fence_after();
+                const int cols = w.cols(a, it);
+                if (cols > 0) {
+                    const uint32_t idesc = idesc_of(cols);
+#pragma unroll
+                    for (int unit = 0; unit < C::QU; ++unit) {
+                        uint32_t qs;
+                        if (ok) ok = take(qs);
+                        if (!ok) break;
+                        products(buf, idesc, ks[unit % C::UN], qs, unit > 0);
+                        release(qs);
+                    }
+                    if (!ok) break;
+                }
+                commit(MLZC_BAR(s_full, buf));
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int unit = 0; unit < C::UN; ++unit) release(ks[unit]);
+        }
     }
     if (!ok && last_bar && elect_one()) {
         umma_commit(last_bar);
@@ -512,8 +603,8 @@ __device__ __forceinline__ void head_role(const WeightArgs& a, Bars* B) {
     long long at = B->first;
     Walk w(B);
     while (w.next(a)) {
-        if (w.tile == 0 && !w.ends(a)) {
-            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of(a, w.s, w.t);
+        if (!w.wide && w.tile == 0 && w.n < w.tiles) {
+            const long long n = min((long long)a.n_ctas, B->total), end = at + w.tiles;
             hd = make_int4(w.b, w.h, w.t, (int)((end * n - 1) / B->total));
         }
         at += w.n;
@@ -528,9 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     const uint32_t ring = smem_u32(smem);
     uint8_t* fixed = smem + (size_t)C::ST * C::kUnit;
     Bars* B = reinterpret_cast<Bars*>(fixed);
-    float* lse2 = reinterpret_cast<float*>(fixed + 512);
+    float* lse2 = reinterpret_cast<float*>(fixed + kBarBytes);
     float* handed = lse2 + kBufs * 128;
-    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    // the loading and issuing warps come first (a scheduler prefers its lower warps)
+    const int warp = (int)uniform(threadIdx.x >> 5) - 4, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::ST; ++i) {
             mbar_init(smem_u32(&B->full[i]), 1);
@@ -550,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
         tma_prefetch_desc(&a.mk);
         tma_prefetch_desc(&a.mq);
     }
-    if (warp == kEpiWarps + 1) tmem_alloc(smem_u32(&B->tmem), 512);
+    if (warp == -3) tmem_alloc(smem_u32(&B->tmem), 512);
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     plan(a, B);
@@ -558,16 +650,19 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B->tmem;
-    if (warp < kEpiWarps) sum_role<C>(a, B, lse2, handed, tmem, warp, lane);
-    else if (warp == kEpiWarps) load_role<C>(a, B, ring, lane);
-    else if (warp == kEpiWarps + 1) mma_role<C>(a, B, ring, tmem);
-    else {
-        lse_role(a, B, lse2, warp - kEpiWarps - 2, lane);
-        if (warp == kEpiWarps + 3 && lane == 0) head_role(a, B);
+    if (warp >= 0) {
+        sum_role<C>(a, B, lse2, handed, tmem, warp, lane);
+    } else if (warp == -4) {
+        load_role<C>(a, B, ring, lane);
+    } else if (warp == -3) {
+        mma_role<C>(a, B, ring, tmem);
+    } else {
+        lse_role(a, B, lse2, warp + 2, lane);
+        if (warp == -1 && lane == 0) head_role(a, B);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kEpiWarps + 1) {
+    if (warp == -3) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
