@@ -10,15 +10,16 @@
 // across threads and nothing atomically, and the softmax's statistics, known from the
 // attention, enter as one constant a column: one FMA, one exponential and one add a score.  The
 // exponential unit (1024 clocks a 128 x 128 tile; the products take 512) is the bound for long
-// chunks, reading K that for decode.  kPolyEvery moves a share of the exponentials to the FMA
-// pipe.
+// chunks, reading K that for decode.  Moving a share of the exponentials to the FMA pipe gains
+// nothing (175 us with and without one in four, for 2048 tokens of 8192, 8 heads of 4).
 //
 // A piece of work is what one operand is held for: a slot tile (K) and its query tiles, or,
 // where a sequence's rows fill one query tile at most (decode), that tile (Q) and a run of slot
 // tiles.  The held operand and the passing one share a ring of shared-memory units: loader warp
 // (K by one TMA box a page piece, Q by one box a 64-dim block), MMA warp (scores into four TMEM
 // buffers, as many columns as there are rows), two lse warps (a tile's lse2 into shared memory),
-// two warpgroups that take turns at the tiles.  f32 queries come as f16 hi + lo from a small
+// four warpgroups that take turns at the tiles (with two
+// the exponential unit idled half of the time: 205 us for 2048 tokens of 8192).  f32 queries come as f16 hi + lo from a small
 // preparing launch, low products summed first.
 //
 // Slot tiles x query tiles of a call form one list cut into equal shares, as in paged_attn.cu;
@@ -50,11 +51,11 @@ using namespace tc05;
 constexpr int kSmemMax = 232448;
 constexpr int kBN = 128;               // slots a tile
 constexpr int kBufs = 4;               // score buffers in TMEM (128 columns each) and lse tiles
-constexpr int kBarBytes = 512;
-constexpr int kFixed = kBarBytes + kBufs * 128 * 4 + 2 * 128 * 4;   // barriers, lse tiles, sums handed over
-constexpr int kEpiWarps = 8;
+constexpr int kBarBytes = 640;
+constexpr int kTurns = 4;              // warpgroups that take turns at the tiles
+constexpr int kFixed = kBarBytes + kBufs * 128 * 4 + 2 * (kTurns - 1) * 128 * 4;   // barriers, lse tiles, sums handed over
+constexpr int kEpiWarps = 4 * kTurns;
 constexpr int kThreads = (kEpiWarps + 4) * 32;
-constexpr int kPolyEvery = 4;          // of so many pairs of exponentials one goes to the FMA pipe
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WeightArgs {
@@ -208,17 +209,6 @@ __device__ void plan(const WeightArgs& a, Bars* B) {
     __syncthreads();
 }
 
-// 2^x of two values: the exponential unit, or for every kPolyEvery-th pair the FMA pipe.
-__device__ __forceinline__ void exp_pair(int j, uint64_t y, float& p0, float& p1) {
-    if (j % kPolyEvery == kPolyEvery - 1) {
-        exp2_poly5(y, p0, p1);
-    } else {
-        unpair(y, p0, p1);
-        p0 = ex2(p0);
-        p1 = ex2(p1);
-    }
-}
-
 // Sums the weights of tile after tile; thread = slot.
 template <class C>
 __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const float* lse2, float* handed, uint32_t tmem, int warp, int lane) {
@@ -244,18 +234,20 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
     Walk w(B);
     while (w.next(a)) {
         const bool whole = w.whole();
-        // a slot tile with several query tiles: the second warpgroup hands its sums to the first
+        // a slot tile with several query tiles: the warpgroups hand their sums to the first
         const bool shared = !w.wide && w.n > 1;
         const char* acc = a.acc ? a.acc + (size_t)w.b * a.a_seq + (size_t)w.h * a.a_head : nullptr;
         float* out = reinterpret_cast<float*>(a.out + (size_t)w.b * a.o_seq + (size_t)w.h * a.o_head);
         const int past = w.s.kv - w.s.rows;
         float total = 0.0f, before = 0.0f;
         bool mine = false;                    // this warpgroup had a tile of the piece
+        if (!w.wide && whole && acc && slot < w.slots(0) && (!shared || turn == 0))
+            before = ptx::ld_act(reinterpret_cast<const float*>(acc) + w.t * kBN + slot);
         for (int it = 0; it < w.n; ++it, ++g) {
-            if ((int)(g & 1) != turn) continue;
+            if ((int)(g % kTurns) != turn) continue;
             const int buf = g % kBufs, slots = w.slots(it), j = w.slot_tile(it) * kBN + slot;
             const uint32_t par = (g / kBufs) & 1;
-            if (whole && acc && (w.wide || !mine) && slot < slots) before = ptx::ld_act(reinterpret_cast<const float*>(acc) + j);
+            if (w.wide && acc && slot < slots) before = ptx::ld_act(reinterpret_cast<const float*>(acc) + j);
             mine = true;
             if (!mbar_wait(MLZC_BAR(s_full, buf), par, abort, a.c.err)) return;
             if (!mbar_wait(MLZC_BAR(lse_full, buf), par, abort, a.c.err)) return;
@@ -268,39 +260,27 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
                 const float* lt = lse2 + buf * 128;
                 const uint32_t s_col = lanes + buf * 128;
                 uint64_t sum[2] = {0, 0};
-                if (C::CAP || cols <= 96 || __any_sync(~0u, from > 0)) {
+                const bool some_cols = C::CAP || __any_sync(~0u, from > 0);
+                const uint64_t c22 = pair(c2, c2);
 #pragma unroll 1
-                    for (int i = 0; i < cols; i += 16) {
-                        float x[16];
-                        tmem_ld16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(x));
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int k = 0; k < 16; k += 2) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
-                    }
-                } else {
-                    const uint64_t c22 = pair(c2, c2);
-                    float x[128];
-#pragma unroll
-                    for (int i = 0; i < 128; i += 32)
-                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i));
+                for (int i = 0; i < cols; i += 32) {
+                    float x[32];
+                    tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(x));
                     tmem_ld_wait();
-                    auto run = [&](int i0, int i1) {
+                    if (some_cols || i + 32 > cols) {
 #pragma unroll
-                        for (int i = i0; i < i1; i += 4) {
-                            const float4 L = *reinterpret_cast<const float4*>(lt + i);
-                            float p0, p1, p2, p3;
-                            exp_pair(i / 2, fma2(pair(x[i], x[i + 1]), c22, pair(L.x, L.y)), p0, p1);
-                            exp_pair(i / 2 + 1, fma2(pair(x[i + 2], x[i + 3]), c22, pair(L.z, L.w)), p2, p3);
-                            sum[0] = add2(sum[0], pair(p0, p1));
-                            sum[1] = add2(sum[1], pair(p2, p3));
-                        }
-                    };
-                    run(0, 96);
-                    if (cols == 128) {
-                        run(96, 128);
+                        for (int k = 0; k < 32; k += 2)
+                            if (i + k < cols) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
                     } else {
 #pragma unroll
-                        for (int i = 96; i < 128; i += 2) sum[0] = add2(sum[0], some(x + i, lt, i, 0, cols));
+                        for (int k = 0; k < 32; k += 4) {
+                            const float4 L = *reinterpret_cast<const float4*>(lt + i + k);
+                            float y0, y1, y2, y3;
+                            unpair(fma2(pair(x[k], x[k + 1]), c22, pair(L.x, L.y)), y0, y1);
+                            unpair(fma2(pair(x[k + 2], x[k + 3]), c22, pair(L.z, L.w)), y2, y3);
+                            sum[0] = add2(sum[0], pair(ex2(y0), ex2(y1)));
+                            sum[1] = add2(sum[1], pair(ex2(y2), ex2(y3)));
+                        }
                     }
                 }
                 float s0, s1;
@@ -318,18 +298,19 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
         }
         if (w.wide) continue;
         if (shared) {
-            float* there = handed + (item & 1) * 128;
+            float* there = handed + (item & 1) * (kTurns - 1) * 128 + slot;
             const uint32_t full = MLZC_BAR(hand_full, item & 1), empty = MLZC_BAR(hand_empty, item & 1), par = (item >> 1) & 1;
             ++item;
-            if (turn == 1) {
+            if (turn > 0) {
                 if (!mbar_wait(empty, par ^ 1, abort, a.c.err)) return;
-                there[slot] = total;
+                there[(turn - 1) * 128] = total;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full);
                 continue;
             }
             if (!mbar_wait(full, par, abort, a.c.err)) return;
-            total += there[slot];
+#pragma unroll
+            for (int i = 0; i < kTurns - 1; ++i) total += there[i * 128];
             __syncwarp();
             if (lane == 0) mbar_arrive(empty);
         } else if (!mine) {
@@ -634,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_kernel(const __grid_const
             mbar_init(smem_u32(&B->lse_full[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&B->hand_full[i]), 4);
+            mbar_init(smem_u32(&B->hand_full[i]), kEpiWarps - 4);
             mbar_init(smem_u32(&B->hand_empty[i]), 4);
         }
         B->abort = 0;

@@ -191,10 +191,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 2^x of two values on the FMA pipe, for kernels bound by the exponential unit: x = n + f with
 // |f| <= 1/2 (adding 1.5 * 2^23 rounds to an integer, left in the low bits), 2^f by its minimax
-// polynomial with constant term 1 (relative error 2.8e-6 at degree 4, 1.1e-7 at degree 5; f = 0
-// is exact), n added to the exponent.  At and below -127 the result is exactly 0.
-template <int N>
-__device__ __forceinline__ void exp2_fma(uint64_t x, const float (&c)[N], float& r0, float& r1) {
+// polynomial of degree 4 with constant term 1 (relative error 2.8e-6; f = 0 is exact), n added to
+// the exponent.  At and below -127 the result is exactly 0.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
     float a, b, t0, t1;
     unpair(x, a, b);
     x = pair(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
@@ -202,21 +201,15 @@ __device__ __forceinline__ void exp2_fma(uint64_t x, const float (&c)[N], float&
     const uint64_t t = add2(x, pair(kRound, kRound));
     const uint64_t n = add2(t, pair(-kRound, -kRound));
     const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
-    uint64_t p = pair(c[N - 1], c[N - 1]);
-#pragma unroll
-    for (int i = N - 2; i >= 0; --i) p = fma2(p, f, pair(c[i], c[i]));
+    uint64_t p = pair(0.009582853876054287f, 0.009582853876054287f);
+    p = fma2(p, f, pair(0.055906426161527634f, 0.055906426161527634f));
+    p = fma2(p, f, pair(0.24024099111557007f, 0.24024099111557007f));
+    p = fma2(p, f, pair(0.6931241750717163f, 0.6931241750717163f));
+    p = fma2(p, f, pair(1.0f, 1.0f));
     unpair(t, t0, t1);
     unpair(p, a, b);
     r0 = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
     r1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
-}
-__device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
-    constexpr float c[5] = {1.0f, 0.6931241750717163f, 0.24024099111557007f, 0.055906426161527634f, 0.009582853876054287f};
-    exp2_fma(x, c, r0, r1);
-}
-__device__ __forceinline__ void exp2_poly5(uint64_t x, float& r0, float& r1) {
-    constexpr float c[6] = {1.0f, 0.6931470036506653f, 0.24022242426872253f, 0.05550733581185341f, 0.009671512991189957f, 0.001326472731307149f};
-    exp2_fma(x, c, r0, r1);
 }
 
 // cap * tanh(s scale / cap) = cap (1 - e) / (1 + e), e = exp(-2 |s| scale / cap) = 2^(|s| cap_in).
