@@ -29,6 +29,11 @@
 // steps it is off by 4e-5.  Here O therefore sums one slot tile in TMEM, low products first, and
 // correction warps add the tiles up in registers, rounding to nearest.  Tiles are independent
 // of one another (each has its own maximum and sum), so the softmax keeps no state.
+// SPREAD (f32 decode): query tiles of up to 8 rows would leave most of the 128 rows of the products
+// idle.  They lie there eight times instead: hi and lo as rows of their own, so that one pass
+// gives both parts' scores and both parts' P V, and that four times, each softmax warp taking a
+// quarter of the slots (P is 0 in the others); the correction warps add the copies up at the end
+// of a piece.
 //
 // All (sequence, KV head, query tile, slot tile) of a call form one list, of which every CTA
 // takes an equal contiguous share (few rows over a long cache and many rows over a short one
@@ -82,12 +87,12 @@ struct AttnArgs {
     int n_ctas, rec_rows;
     float* rec;                // [cta][2][rec_rows][D]: 0 continues a cut tile, 1 begins one
     float2* ml;                // [cta][2][rec_rows]: exponent of the record's scale, sum
-    int4* head;                // [cta]: sequence (-1: none), kv head, query tile, last CTA of the tile begun in record 1
+    int4* head;                // [cta]: of the query tile begun in record 1, packed row, tokens, kv head, last CTA (-1: none)
 };
 
 constexpr int BN = 128;        // slots a tile
 
-template <int D_, int NS_, bool HL_, bool CAP_>
+template <int D_, int NS_, bool HL_, bool CAP_, bool SPREAD_ = false>
 struct Cfg {
     static constexpr int D = D_, NS = NS_;
     static constexpr bool HL = HL_, CAP = CAP_;           // f32 queries (hi + lo); scores are capped
@@ -101,7 +106,10 @@ struct Cfg {
     static constexpr uint32_t kQBytes = kQTile * NS * (HL ? 2 : 1);   // [tile][hi, lo]
     static constexpr uint32_t kSub = BN * 128;            // bytes of a 64-value block of a unit
     static constexpr uint32_t kUnit = kSub * SUBS;
-    static constexpr uint32_t kStats = HL ? 4 * 128 * 8 : 0;
+    static constexpr bool kSpread = SPREAD_;              // up to 8 rows lie eight times
+    static constexpr int kPitch = D + 4;                  // floats of a staged row of O
+    static constexpr uint32_t kStage = 4 * 8 * (kPitch + 2) * 4;
+    static constexpr uint32_t kStats = HL ? 4 * 128 * 8 + (kSpread ? kStage : 0) : 0;
     static constexpr int kFit = (kSmemMax - 1024 - kBarBytes - (int)kStats - (int)kQBytes) / (int)kUnit;
     static constexpr int ST = kFit > 8 ? 8 : kFit;
     static constexpr size_t kSmem = 1024 + kBarBytes + kStats + kQBytes + (size_t)ST * kUnit;
@@ -126,15 +134,16 @@ struct Cfg {
     static_assert(2 * BN + NS * D <= 512, "TMEM");
     static_assert(ST >= 3, "ring");
     static_assert(!HL || NS == 1, "f32 calls take one query tile");
+    static_assert(!kSpread || (HL && D <= 128), "one correction warpgroup");
 };
 
 // Barriers in shared memory.
 struct Bars {
-    uint64_t full[8], empty[8], q_full, q_empty, s_full[4], p_full[4], o_step[2], o_done[2], o_empty[2], stat_full[4];
+    uint64_t full[8], empty[8], q_full, q_empty, s_full[4], p_full[4], o_step[2], o_done[2], o_empty[2], stat_full[4], copies;
     uint32_t tmem;
     int abort;
     long long first, count, total;   // this CTA's share of the list; its start's place
-    int b, h, t, tile;
+    int b, h, t, at;
     long long scan[16];
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barriers");
@@ -149,41 +158,56 @@ __device__ __forceinline__ int tiles_of(const Seq& s, int t, int tokens) {
     return max(1, (visible(s, t, tokens) + BN - 1) / BN);
 }
 
+// What a query tile costs beside its slot tiles (its Q, filling and draining the pipeline), in slot
+// tiles.  The list counts it in front of the tiles, so that CTAs with many short query tiles get
+// fewer slot tiles (24 mixed sequences, 64 dims f32: 127 us with 0, 90 with 2 to 4, 101 with 8).
+constexpr int kStart = 3;
+
 // A walk over this CTA's share: piece after piece (the tiles of one query tile).
 template <class C>
 struct Walk {
     int b, h, t, tile, n;      // the piece: slot tiles [tile, tile + n)
+    int all;                   // of so many
+    int at;                    // place in the query tile's part of the list
     long long left;
     Seq s;
     bool first;
-    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(B->tile), n(0), left(B->count), first(true) {}
+    __device__ Walk(const Bars* B) : b(B->b), h(B->h), t(B->t), tile(0), n(0), all(0), at(B->at), left(B->count), first(true) {}
     // Moves to the next piece; false at the end.
     __device__ bool next(const AttnArgs& a) {
-        if (left <= 0) return false;
         const int tokens = a.tq * C::NS;
-        if (first) {
-            s = paged::load_seq(a.c, b);
-            first = false;
-        } else {
-            tile = 0;
-            if ((int64_t)(++t) * tokens >= s.rows) {
-                t = 0;
-                if (++h == a.c.n_head_kv) {
-                    h = 0;
-                    do {
-                        s = paged::load_seq(a.c, ++b);
-                    } while (s.rows == 0);   // the list ends at a sequence with rows
+        do {
+            if (left <= 0) return false;
+            if (first) {
+                s = paged::load_seq(a.c, b);
+                first = false;
+            } else {
+                at = 0;
+                if ((int64_t)(++t) * tokens >= s.rows) {
+                    t = 0;
+                    if (++h == a.c.n_head_kv) {
+                        h = 0;
+                        do {
+                            s = paged::load_seq(a.c, ++b);
+                        } while (s.rows == 0);   // the list ends at a sequence with rows
+                    }
                 }
             }
-        }
-        const int all = tiles_of(s, t, tokens) - tile;
-        n = (int)min((long long)all, left);
-        left -= n;
+            all = tiles_of(s, t, tokens);
+            const int to = (int)min((long long)(all + kStart), at + left);
+            left -= to - at;
+            tile = max(0, at - kStart);
+            n = max(0, to - kStart) - tile;
+        } while (n == 0);                        // no more than its start
         return true;
     }
     __device__ int tok0(const AttnArgs& a) const { return t * a.tq * C::NS; }
     __device__ int tiles(const AttnArgs& a) const { return C::NS == 2 && tok0(a) + a.tq < s.rows ? 2 : 1; }
-    __device__ bool ends(const AttnArgs& a) const { return tile + n == tiles_of(s, t, a.tq * C::NS); }
+    // Rows of the piece's (first) query tile, and whether they lie eight times in it: row r of
+    // copy c at 32 c + r (hi) and 32 c + 16 + r (lo).
+    __device__ int rows(const AttnArgs& a) const { return min(a.tq, s.rows - tok0(a)) * a.G; }
+    __device__ bool spread(const AttnArgs& a) const { return C::kSpread && rows(a) <= 8; }
+    __device__ bool ends() const { return tile + n == all; }
 };
 
 // Finds this CTA's share.  Threads own runs of sequences: their tile counts are summed over the
@@ -198,7 +222,7 @@ __device__ void plan(const AttnArgs& a, Bars* B) {
     for (int b = b0; b < b1; ++b) {
         const Seq s = paged::load_seq(a.c, b);
         long long one = 0;
-        for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens);
+        for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens) + kStart;
         mine += one * a.c.n_head_kv;
     }
     long long upto = mine;
@@ -222,15 +246,15 @@ __device__ void plan(const AttnArgs& a, Bars* B) {
         for (int b = b0; b < b1; ++b) {
             const Seq s = paged::load_seq(a.c, b);
             long long one = 0;
-            for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens);
+            for (int t = 0; (int64_t)t * tokens < s.rows; ++t) one += tiles_of(s, t, tokens) + kStart;
             if (r >= one * a.c.n_head_kv) { r -= one * a.c.n_head_kv; continue; }
             B->b = b;
             B->h = (int)(r / one);
             r %= one;
             int t = 0;
-            while (r >= tiles_of(s, t, tokens)) r -= tiles_of(s, t++, tokens);
+            while (r >= tiles_of(s, t, tokens) + kStart) r -= tiles_of(s, t++, tokens) + kStart;
             B->t = t;
-            B->tile = (int)r;
+            B->at = (int)r;
             break;
         }
     }
@@ -278,7 +302,7 @@ struct Sink {
     int t, h;
     size_t r;
     __device__ Sink(const AttnArgs& a, const Walk<C>& w, const Row& q, int slot) {
-        whole = w.tile == 0 && w.ends(a);
+        whole = w.tile == 0 && w.ends();
         t = w.s.row0 + q.tok(a, w, slot);
         h = w.h * a.G + q.head_of;
         r = ((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * a.rec_rows + slot * 128 + q.row;
@@ -430,7 +454,7 @@ template <class C>
 __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, float2* stats, uint32_t tmem, int warp, int lane) {
     constexpr int kTurns = C::kSoftWarps / 4;
     const int turn = warp >> 2;
-    const Row q(a, (warp & 3) * 32 + lane);
+    const int row = (warp & 3) * 32 + lane;              // of the products
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
     const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
@@ -438,6 +462,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
     uint32_t g = 0;
     Walk<C> w(B);
     while (w.next(a)) {
+        const bool spread = w.spread(a);
+        const Row q(a, spread ? lane & 15 : row);
         const bool busy = __any_sync(~0u, q.real(a, w, 0));
         const int own = w.s.kv - w.s.rows + q.tok(a, w, 0);
         for (int it = 0; it < w.n; ++it, ++g) {
@@ -477,7 +503,37 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     if (C::CAP) x = capped(x, cap_in, a.softcap);
                     return i > limit ? -INFINITY : x;
                 };
-                if constexpr (C::kHold) {
+                if (C::kSpread && spread) {
+                    // this warp's quarter of the slots; lane and lane ^ 16 have the parts of a score
+                    const int c0 = (warp & 3) * 32;
+                    float x[32];
+                    tmem_ld32(s_col + c0, *reinterpret_cast<uint32_t(*)[32]>(x));
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] += __shfl_xor_sync(~0u, x[i], 16);
+                    if (C::CAP || cut) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = clip(x[i], c0 + i);
+                    }
+                    m = row_max(x);
+                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                    uint32_t p[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float p0, p1;
+                        unpair(fma2(pair(x[2 * j], x[2 * j + 1]), c22, pair(off, off)), p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
+                        const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                        p[j] = lane < 16 ? ptx::pack_h2(h0, h1) : ptx::pack_h2(p0 - h0, p1 - h1);
+                    }
+                    tmem_st16(s_col + c0, p);
+                    const uint32_t zero[16] = {};
+#pragma unroll
+                    for (int i = 0; i < BN; i += 32)
+                        if (i != c0) tmem_st16(s_col + i, zero);
+                } else if constexpr (C::kHold) {
                     float x[BN];
 #pragma unroll
                     for (int i = 0; i < BN / 32; ++i)
@@ -519,7 +575,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                 }
                 float s0, s1;
                 unpair(add2(sum[0], sum[1]), s0, s1);
-                stats[(g & 3) * 128 + q.row] = make_float2(m == -INFINITY ? -INFINITY : m * c2 - kPOffset, s0 + s1);
+                // (of a row that lies as hi and lo the hi lane has the sum)
+                stats[(g & 3) * 128 + row] = make_float2(m == -INFINITY ? -INFINITY : m * c2 - kPOffset, spread && lane >= 16 ? 0.0f : s0 + s1);
                 tmem_st_wait();
             }
             tc_fence_before();
@@ -536,15 +593,18 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
 // largest exponent so far (raised, and O rescaled, when a tile's lies more than 8 above it).
 // stats has four places: the softmax fills that of tile g + 4 only after tile g + 1 was read.
 template <class C>
-__device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, const float2* stats, uint32_t tmem, int warp, int lane) {
+__device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, float2* stats, uint32_t tmem, int warp, int lane) {
     constexpr int CD = C::CD;
     const int part = (warp - C::kSoftWarps) >> 2;        // dims [part * CD, + CD)
-    const Row q(a, (warp & 3) * 32 + lane);
+    const int row = (warp & 3) * 32 + lane;              // of the products
+    float* stage = reinterpret_cast<float*>(stats + 4 * 128);
     const uint32_t o_col = tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::kOCol + part * CD;
     volatile int* abort = &B->abort;
-    uint32_t g = 0;
+    uint32_t g = 0, merges = 0;
     Walk<C> w(B);
     while (w.next(a)) {
+        const bool spread = w.spread(a);
+        const Row q(a, spread ? lane & 15 : row);
         const bool real = q.real(a, w, 0), busy = __any_sync(~0u, real);
         float o[CD], e = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -552,7 +612,7 @@ __device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, const f
         for (int it = 0; it < w.n; ++it, ++g) {
             if (!mbar_wait(smem_u32(&B->stat_full[g & 3]), (g >> 2) & 1, abort, a.c.err)) return;
             float2 st = make_float2(-INFINITY, 0.0f);
-            if (busy) st = stats[(g & 3) * 128 + q.row];
+            if (busy) st = stats[(g & 3) * 128 + row];
             if (!mbar_wait(smem_u32(&B->o_done[0]), g & 1, abort, a.c.err)) return;
             tc_fence_after();
             if (busy) {
@@ -578,6 +638,52 @@ __device__ __forceinline__ void correct_role(const AttnArgs& a, Bars* B, const f
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&B->o_empty[0]));
+        }
+        if (C::kSpread && spread) {
+            // hi and lo, then the four copies through shared memory, a thread a few dims of a row
+            auto meet = [&]() {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&B->copies));
+                return mbar_wait(smem_u32(&B->copies), merges++ & 1, abort, a.c.err);
+            };
+            float2* scale = reinterpret_cast<float2*>(stage + 32 * C::kPitch);
+#pragma unroll
+            for (int i = 0; i < CD; ++i) o[i] += __shfl_xor_sync(~0u, o[i], 16);
+            if (lane < 8) {
+                const int at = (warp & 3) * 8 + lane;
+                scale[at] = make_float2(e, l);
+#pragma unroll
+                for (int i = 0; i < CD; i += 4)
+                    *reinterpret_cast<float4*>(stage + at * C::kPitch + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+            if (!meet()) return;
+            constexpr int N = CD / 16;
+            const Row r(a, row >> 4);
+            if (r.real(a, w, 0)) {
+                float2 c[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[i] = scale[i * 8 + r.row];
+                const float top = fmaxf(fmaxf(c[0].x, c[1].x), fmaxf(c[2].x, c[3].x));
+                float x[N] = {}, sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float f = c[i].x == -INFINITY ? 0.0f : ex2(c[i].x - top);
+                    sum = fmaf(f, c[i].y, sum);
+                    const float* p = stage + (i * 8 + r.row) * C::kPitch + (row & 15) * N;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) x[j] = fmaf(f, p[j], x[j]);
+                }
+                const Sink<C> sink(a, w, r, 0);
+                if ((row & 15) == 0) sink.sums(a, top, sum);
+                const float inv = sink.whole ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+                float* to = (sink.whole ? reinterpret_cast<float*>(a.dst + (size_t)sink.t * a.d_tok + (size_t)sink.h * a.d_head)
+                                        : a.rec + sink.r * C::D) + (row & 15) * N;
+#pragma unroll
+                for (int j = 0; j < N; j += 4)
+                    *reinterpret_cast<float4*>(to + j) = make_float4(x[j] * inv, x[j + 1] * inv, x[j + 2] * inv, x[j + 3] * inv);
+            }
+            if (!meet()) return;                         // the staging place is free again
+            continue;
         }
         if (real) {
             const Sink<C> sink(a, w, q, 0);
@@ -678,7 +784,8 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
         } else {
             constexpr int kCh = C::D / 8, kStep = 64 / kCh, kDeep = 4;   // places a row; rows a step of both warps
             const int ch = lane % kCh, t0 = w.tok0(a);
-            const int rows = min(a.tq, w.s.rows - t0) * a.G;
+            const int rows = w.rows(a);
+            const bool spread = w.spread(a);
             const char* q0 = a.q + (size_t)(w.s.row0 + t0) * a.q_tok + (size_t)w.h * a.G * a.q_head + ch * 32;
             const uint32_t to0 = qs + (ch >> 3) * C::kQSub;
             for (int r0 = (lane + 32 * part) / kCh; r0 < rows; r0 += kStep * kDeep) {
@@ -702,8 +809,18 @@ __device__ __forceinline__ void q_role(const AttnArgs& a, Bars* B, uint32_t qs, 
                         ptx::split_h2(v[k][1].x, v[k][1].y, hi.z, lo.z);
                         ptx::split_h2(v[k][1].z, v[k][1].w, hi.w, lo.w);
                         const uint32_t to = to0 + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::kQTile), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                        auto put = [&](uint32_t at, const uint4& v) {
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                        };
+                        if (spread) {
+                            for (int copy = 0; copy < 4; ++copy) {
+                                put(to + copy * 32 * 128, hi);
+                                put(to + copy * 32 * 128 + 16 * 128, lo);
+                            }
+                        } else {
+                            put(to, hi);
+                            put(to + C::kQTile, lo);
+                        }
                     }
                 }
             }
@@ -762,17 +879,21 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
         last_par = u.phase;
     };
     // S of query tile `tile` and the slots from `row` of the tile on, into buffer `buf`
+    bool spread = false;                     // hi and lo are rows of one Q tile
     auto scores = [&](int tile, int buf, int unit, const Unit& u, int row) {
         const uint32_t k = desc_lo(ring16 + u.st * (C::kUnit >> 4) + row * 8);
         const uint32_t q = desc_lo(q16 + ((tile * PARTS * C::kQTile + unit * C::SUBS * C::kQSub) >> 4));
         const uint32_t d = tmem + C::kSCol + buf * kCols;
         if (elect_one()) {
 #pragma unroll
-            for (int part = PARTS - 1; part >= 0; --part)      // lo, then hi
+            for (int part = PARTS - 1; part >= 0; --part) {    // lo, then hi
+                if (C::kSpread && part > 0 && spread) continue;
 #pragma unroll
                 for (int i = 0; i < DU / 16; ++i)
                     umma_f16_lo(d, q + ((part * C::kQTile + (i >> 2) * C::kQSub + (i & 3) * 32) >> 4),
-                                k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s, unit > 0 || i > 0 || part != PARTS - 1);
+                                k + (((i >> 2) * C::kSub + (i & 3) * 32) >> 4), idesc_s,
+                                unit > 0 || i > 0 || (part != PARTS - 1 && !spread));
+            }
         }
     };
     // `steps` key steps of P V, from step i0 (even) on
@@ -781,11 +902,13 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
         const uint32_t d = tmem + C::kOCol + tile * C::D + unit * DU, p = tmem + C::kSCol + buf * BN + i0 * 16;
         if (elect_one()) {
 #pragma unroll
-            for (int part = PARTS - 1; part >= 0; --part)
+            for (int part = PARTS - 1; part >= 0; --part) {
+                if (C::kSpread && part > 0 && spread) continue;
 #pragma unroll
                 for (int i = 0; i < decltype(steps)::value; ++i)
                     umma_f16_ta_lo(d, p + (i >> 1) * 32 + (i & 1) * 8 + part * 16, v + i * 128, idesc_o,
-                                   add || i > 0 || part != PARTS - 1);
+                                   add || i > 0 || (part != PARTS - 1 && !spread));
+            }
         }
     };
     constexpr std::integral_constant<int, BN / 16> all{};
@@ -818,6 +941,7 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
     Walk<C> w(B);
     while (ok && w.next(a)) {
         const int nt = w.tiles(a);
+        spread = uniform(w.spread(a)) != 0;
         ok = wait(MLZC_BAR(q_full, 0), seg & 1);
         if (!ok) break;
         ++seg;
@@ -911,15 +1035,14 @@ __device__ __forceinline__ void mma_role(const AttnArgs& a, Bars* B, uint32_t qs
 // Notes for the merge launch the query tile that begins in this CTA's share and ends in a later one.
 template <class C>
 __device__ __forceinline__ void head_role(const AttnArgs& a, Bars* B) {
-    int4 hd = make_int4(-1, 0, 0, 0);
-    long long at = B->first;
+    int4 hd = make_int4(0, 0, 0, -1);
     Walk<C> w(B);
     while (w.next(a)) {
-        if (w.tile == 0 && !w.ends(a)) {
-            const long long n = min((long long)a.n_ctas, B->total), end = at + tiles_of(w.s, w.t, a.tq * C::NS);
-            hd = make_int4(w.b, w.h, w.t, (int)((end * n - 1) / B->total));
+        if (w.tile == 0 && !w.ends()) {
+            // the share's last piece: what is left of its query tile ends so many places on
+            const long long n = min((long long)a.n_ctas, B->total), end = B->first + B->count + w.all - w.n;
+            hd = make_int4(w.s.row0 + w.tok0(a), min(a.tq * C::NS, w.s.rows - w.tok0(a)), w.h, (int)((end * n - 1) / B->total));
         }
-        at += w.n;
     }
     a.head[blockIdx.x] = hd;
 }
@@ -958,6 +1081,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
             mbar_init(smem_u32(&B->p_full[i]), 4);
         }
         for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&B->stat_full[i]), 4);
+        mbar_init(smem_u32(&B->copies), 4);
         B->abort = 0;
         ptx::mbar_init_fence();
         tma_prefetch_desc(&a.mk);
@@ -1006,41 +1130,53 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
 // Merges the records of each cut query tile: block (c, y) the tile begun by CTA c, 8 rows.
 constexpr int kMergeRows = 8;
 template <int D, typename Out>
-__global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_constant__ AttnArgs a, int tiles) {
+__global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_constant__ AttnArgs a) {
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const int c = blockIdx.x, lane = threadIdx.x & 31;
-    const int hb = paged::ld_int(&a.head[c].x);
-    if (hb < 0) return;
-    const int h = paged::ld_int(&a.head[c].y), t = paged::ld_int(&a.head[c].z), last = paged::ld_int(&a.head[c].w);
+    const uint4 hd = ptx::ld_act(reinterpret_cast<const uint4*>(&a.head[c]));
+    const int row0 = (int)hd.x, tokens = (int)hd.y, h = (int)hd.z, last = (int)hd.w;
+    if (last < 0) return;
     const int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5);
-    const Seq s = paged::load_seq(a.c, hb);
-    const int in = row % 128, slot = row / 128;
-    const int tok = (t * tiles + slot) * a.tq + a.by_g.quot(in);
-    if (row >= a.rec_rows || in >= a.tq * a.G || tok >= s.rows) return;
+    const int in = row % 128, tok = row / 128 * a.tq + a.by_g.quot(in);
+    if (row >= a.rec_rows || in >= a.tq * a.G || tok >= tokens) return;
     auto rec = [&](int i) { return ((size_t)i * 2 + (i == c ? 1 : 0)) * a.rec_rows + row; };
-    // lanes share the records' scales out, then every lane owns dims
-    float top = -INFINITY;
-    for (int i = c + lane; i <= last; i += 32) top = fmaxf(top, ptx::ld_act(&a.ml[rec(i)].x));
+    // four records at a time, their loads under way together
+    float top = -INFINITY, l = 0.0f, acc[D / 32] = {};
+    for (int i0 = c; i0 <= last; i0 += 4) {
+        uint2 m[4], v[4][D / 64];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    float l = 0.0f, acc[D / 32] = {};
-    if (top != -INFINITY) {
-#pragma unroll 4
-        for (int i = c; i <= last; ++i) {
-            const size_t r = rec(i);
-            const float f = ex2(ptx::ld_act(&a.ml[r].x) - top);
-            l += f * ptx::ld_act(&a.ml[r].y);
+        for (int k = 0; k < 4; ++k)
+            if (i0 + k <= last) {
+                const size_t r = rec(i0 + k);
+                m[k] = ptx::ld_act(reinterpret_cast<const uint2*>(&a.ml[r]));
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e) {
-                const uint2 v = ptx::ld_act(reinterpret_cast<const uint2*>(a.rec + r * D + e * 64 + lane * 2));
-                acc[2 * e] += f * __uint_as_float(v.x);
-                acc[2 * e + 1] += f * __uint_as_float(v.y);
+                for (int e = 0; e < D / 64; ++e) v[k][e] = ptx::ld_act(reinterpret_cast<const uint2*>(a.rec + r * D + e * 64 + lane * 2));
             }
-        }
+        float to = top;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i0 + k <= last) to = fmaxf(to, __uint_as_float(m[k].x));
+        if (to == -INFINITY) continue;
+        const float f0 = ex2(top - to);
+        top = to;
+        l *= f0;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) acc[e] *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i0 + k <= last) {
+                const float f = ex2(__uint_as_float(m[k].x) - to);
+                l = fmaf(f, __uint_as_float(m[k].y), l);
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) {
+                    acc[2 * e] = fmaf(f, __uint_as_float(v[k][e].x), acc[2 * e]);
+                    acc[2 * e + 1] = fmaf(f, __uint_as_float(v[k][e].y), acc[2 * e + 1]);
+                }
+            }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int q = s.row0 + tok, head = h * a.G + a.by_g.rem(in);
+    const int q = row0 + tok, head = h * a.G + a.by_g.rem(in);
     char* dst = a.dst + (size_t)q * a.d_tok + (size_t)head * a.d_head;
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
@@ -1083,7 +1219,7 @@ int launch(const AttnArgs& a, const DeviceCtx* c, cudaStream_t s) {
     MLZC_CUDA_TRY(cudaGetLastError());
     using Out = typename std::conditional<C::HL, float, __half>::type;
     const dim3 g(a.n_ctas, (a.rec_rows + kMergeRows - 1) / kMergeRows);
-    MLZC_CUDA_TRY(launch_pdl(merge_kernel<C::D, Out>, g, dim3(kMergeRows * 32), 0, s, a, C::NS));
+    MLZC_CUDA_TRY(launch_pdl(merge_kernel<C::D, Out>, g, dim3(kMergeRows * 32), 0, s, a));
     MLZC_CUDA_TRY(cudaGetLastError());
     count_launch(2);
     return MLZC_OK;
@@ -1144,6 +1280,10 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     a.head = reinterpret_cast<int4*>(static_cast<char*>(workspace) + p.rec + p.ml);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool cap = a.softcap > 0.0f;
+    // f32 decode: a token a sequence, at most 8 query rows a KV head
+    const bool spread = f32 && cache->n_tokens <= cache->batch_size && a.G <= 8;
+    if (spread && cache->head_dim == 128) return cap ? launch<Cfg<128, 1, true, true, true>>(a, c, s) : launch<Cfg<128, 1, true, false, true>>(a, c, s);
+    if (spread && cache->head_dim == 64) return cap ? launch<Cfg<64, 1, true, true, true>>(a, c, s) : launch<Cfg<64, 1, true, false, true>>(a, c, s);
 #define MLZC_LAUNCH(DIM, NS)                                                                                            \
     return f32 ? (cap ? launch<Cfg<DIM, 1, true, true>>(a, c, s) : launch<Cfg<DIM, 1, true, false>>(a, c, s))           \
                : (cap ? launch<Cfg<DIM, NS, false, true>>(a, c, s) : launch<Cfg<DIM, NS, false, false>>(a, c, s))

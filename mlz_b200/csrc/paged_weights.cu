@@ -706,9 +706,12 @@ int launch(const WeightArgs& a, const DeviceCtx* c, cudaStream_t s) {
     }
     MLZC_CUDA_TRY(launch_pdl(weights_kernel<C>, dim3(a.n_ctas), dim3(kThreads), C::kSmem, s, a));
     MLZC_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    // no sequence can have a second query tile: no slot tile is cut
+    if (a.c.n_tokens <= a.tq) return MLZC_OK;
     MLZC_CUDA_TRY(launch_pdl(merge_kernel, dim3(a.n_ctas), dim3(128), 0, s, a));
     MLZC_CUDA_TRY(cudaGetLastError());
-    count_launch(2);
+    count_launch();
     return MLZC_OK;
 }
 

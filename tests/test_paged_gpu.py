@@ -63,6 +63,17 @@ def test_attn_head_groups(dev, hkv, group, dtype):
     _check_attn(ref.make(dev, [3, 1, 17], [200, 65, 17], hkv=hkv, group=group, D=64, dtype=dtype, seed=group))
 
 
+@pytest.mark.parametrize("group", [1, 3, 8, 9])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("softcap", [0.0, 6.0])
+@pytest.mark.parametrize("q_len,kv_len", [([1] * 7, [1, 40, 128, 129, 1000, 3000, 5]), ([3, 0, 1, 0, 0, 2], [700, 9, 333, 0, 50, 64]),
+                                          ([20] + [0] * 19, [900] + [3] * 19)])
+def test_attn_f32_decode_batches(dev, q_len, kv_len, softcap, D, group):
+    """As many tokens as sequences, or fewer: few query rows a head (which f32 calls lay out
+    apart), and sequences with more among them."""
+    _check_attn(ref.make(dev, q_len, kv_len, hkv=2, group=group, D=D, dtype=F32, seed=group + D), softcap=softcap)
+
+
 @pytest.mark.parametrize("page", [8, 16, 24, 40, 64, 72, 128, 136, 256, 512])
 @pytest.mark.parametrize("layout", ["hpd", "phd"])
 def test_attn_pages(dev, page, layout):
