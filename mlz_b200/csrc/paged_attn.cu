@@ -366,7 +366,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t o_col = lanes + C::kOCol + slot * D;
     const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
-    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float cap_in = C::CAP ? a.scale / a.softcap : 0.0f;
     const float rise = kRescale / c2;
     volatile int* abort = &B->abort;
     uint32_t g = 0, piece = 0;                           // steps, pieces
@@ -388,10 +388,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                 for (int i = 0; i < N / 32; ++i)
                     tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                 tmem_ld_wait();
-                if (C::CAP) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[i] = capped(x[i], cap_in, a.softcap);
-                }
+                if (C::CAP) cap_scores(x, cap_in, a.softcap);
                 const int limit = own - w.tile * BN - it * N;
                 if (__any_sync(~0u, limit < N - 1)) {
 #pragma unroll
@@ -457,7 +454,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
     const int row = (warp & 3) * 32 + lane;              // of the products
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
-    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float cap_in = C::CAP ? a.scale / a.softcap : 0.0f;
     volatile int* abort = &B->abort;
     uint32_t g = 0;
     Walk<C> w(B);
@@ -499,10 +496,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     tmem_st16(s_col + i, hi);
                     tmem_st16(s_col + i + 16, lo);
                 };
-                auto clip = [&](float x, int i) {
-                    if (C::CAP) x = capped(x, cap_in, a.softcap);
-                    return i > limit ? -INFINITY : x;
-                };
+                auto clip = [&](float x, int i) { return i > limit ? -INFINITY : x; };
                 if (C::kSpread && spread) {
                     // this warp's quarter of the slots; lane and lane ^ 16 have the parts of a score
                     const int c0 = (warp & 3) * 32;
@@ -511,7 +505,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) x[i] += __shfl_xor_sync(~0u, x[i], 16);
-                    if (C::CAP || cut) {
+                    if (C::CAP) cap_scores(x, cap_in, a.softcap);
+                    if (cut) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) x[i] = clip(x[i], c0 + i);
                     }
@@ -539,7 +534,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     for (int i = 0; i < BN / 32; ++i)
                         tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
                     tmem_ld_wait();
-                    if (C::CAP || cut) {
+                    if (C::CAP) cap_scores(x, cap_in, a.softcap);
+                    if (cut) {
 #pragma unroll
                         for (int i = 0; i < BN; ++i) x[i] = clip(x[i], i);
                     }
@@ -555,6 +551,7 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                         tmem_ld32(s_col + i, r);
                         tmem_ld_wait();
                         if (C::CAP || cut) {
+                            if (C::CAP) cap_scores(*reinterpret_cast<float(*)[32]>(r), cap_in, a.softcap);
 #pragma unroll
                             for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(clip(__uint_as_float(r[j]), i + j));
                             tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));

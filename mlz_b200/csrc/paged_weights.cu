@@ -216,18 +216,12 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
     const int slot = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float c2 = C::CAP ? kLog2e : a.scale * kLog2e;
-    const float cap_in = C::CAP ? -2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float cap_in = C::CAP ? a.scale / a.softcap : 0.0f;
     const uint32_t bars = smem_u32(B);
     volatile int* abort = &B->abort;
     // weights of columns i, i + 1 where they count: outside [from, cols) a score may hold anything
     auto some = [&](const float* x, const float* lt, int i, int from, int cols) {
-        float y0 = x[0], y1 = x[1];
-        if (C::CAP) {
-            y0 = capped(y0, cap_in, a.softcap);
-            y1 = capped(y1, cap_in, a.softcap);
-        }
-        y0 = ex2(fmaf(y0, c2, lt[i]));
-        y1 = ex2(fmaf(y1, c2, lt[i + 1]));
+        const float y0 = ex2(fmaf(x[0], c2, lt[i])), y1 = ex2(fmaf(x[1], c2, lt[i + 1]));
         return pair(i >= from && i < cols ? y0 : 0.0f, i + 1 >= from && i + 1 < cols ? y1 : 0.0f);
     };
     uint32_t g = 0, item = 0;
@@ -260,13 +254,14 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
                 const float* lt = lse2 + buf * 128;
                 const uint32_t s_col = lanes + buf * 128;
                 uint64_t sum[2] = {0, 0};
-                const bool some_cols = C::CAP || __any_sync(~0u, from > 0);
+                const bool some_cols = __any_sync(~0u, from > 0);
                 const uint64_t c22 = pair(c2, c2);
 #pragma unroll 1
                 for (int i = 0; i < cols; i += 32) {
                     float x[32];
                     tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(x));
                     tmem_ld_wait();
+                    if (C::CAP) cap_scores(x, cap_in, a.softcap);
                     if (some_cols || i + 32 > cols) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 2)
