@@ -127,8 +127,6 @@ struct Cfg {
     // one in so many pairs of exponentials on the FMA pipe (0: none): 128 dims 855 us with 4, 947
     // with none; 64 dims 712 and 673; 256 dims, where the products are the bound, 370 and 353
     static constexpr int kPoly = NS == 2 && D == 128 ? 4 : 0;
-    // f32: the softmax holds a row's scores in registers (else the correction needs those)
-    static constexpr bool kHold = D < 256;
     static constexpr uint32_t kSCol = 0;                  // S of tile / buffer i at i * BN
     static constexpr uint32_t kOCol = 2 * BN;             // O of tile i at + i * D
     static_assert(2 * BN + NS * D <= 512, "TMEM");
@@ -383,40 +381,84 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
             tc_fence_after();
             if (busy) {
                 const uint32_t s_col = lanes + C::kSCol + buf * N;
-                float x[N];
-#pragma unroll
-                for (int i = 0; i < N / 32; ++i)
-                    tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
-                tmem_ld_wait();
-                if (C::CAP) cap_scores(x, cap_in, a.softcap);
                 const int limit = own - w.tile * BN - it * N;
-                if (__any_sync(~0u, limit < N - 1)) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[i] = i > limit ? -INFINITY : x[i];
-                }
-                const float top = row_max(x);
-                if (it == 0) {
-                    m = top;
-                } else if (__any_sync(~0u, top > m + rise)) {
-                    const float to = top > m + rise ? top : m;
-                    const float al = m == -INFINITY ? 0.0f : ex2((m - to) * c2);
-                    m = to;
-                    l *= al;
-                    // O has the products of the steps before the last (this S came after them);
-                    // wait for the last's
-                    if (!mbar_wait(smem_u32(&B->o_step[slot]), (g - 1) & 1, abort, a.c.err)) return;
-                    tc_fence_after();
+                const bool cut = __any_sync(~0u, limit < N - 1);
+                // the running maximum with a step's; O follows where it rises far
+                auto raise = [&](float top) {
+                    if (it == 0) {
+                        m = top;
+                    } else if (__any_sync(~0u, top > m + rise)) {
+                        const float to = top > m + rise ? top : m;
+                        const float al = m == -INFINITY ? 0.0f : ex2((m - to) * c2);
+                        m = to;
+                        l *= al;
+                        // O has the products of the steps before the last (this S came after
+                        // them); wait for the last's
+                        if (!mbar_wait(smem_u32(&B->o_step[slot]), (g - 1) & 1, abort, a.c.err)) return false;
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int i = 0; i < D; i += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(o_col + i, o);
-                        tmem_ld_wait();
+                        for (int i = 0; i < D; i += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_col + i, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
-                        tmem_st16(o_col + i, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
+                            tmem_st16(o_col + i, o);
+                        }
                     }
+                    return true;
+                };
+                if constexpr (C::CAP) {
+                    // 32 scores at a time in short loops, twice from TMEM: unrolled over a row the code
+                    // of a capped step outgrows the instruction cache (256 dims: 233 us for 149)
+                    float top = -INFINITY, x[2][32];
+                    auto fetch = [&](int i, float (&v)[32]) { tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
+                    auto look = [&](int i, float (&v)[32]) {
+                        cap_scores(v, cap_in, a.softcap);
+                        if (cut) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = i + j > limit ? -INFINITY : v[j];
+                        }
+                        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+                        tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+                        top = fmaxf(top, row_max(v));
+                    };
+                    fetch(0, x[0]);
+#pragma unroll 1
+                    for (int i = 0; i < N; i += 64) {
+                        tmem_ld_wait();
+                        fetch(i + 32, x[1]);
+                        look(i, x[0]);
+                        tmem_ld_wait();
+                        if (i + 64 < N) fetch(i + 64, x[0]);
+                        look(i + 32, x[1]);
+                    }
+                    tmem_st_wait();
+                    if (!raise(top)) return;
+                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                    fetch(0, x[0]);
+#pragma unroll 1
+                    for (int i = 0; i < N; i += 64) {
+                        tmem_ld_wait();
+                        fetch(i + 32, x[1]);
+                        l += weigh<C::kPoly>(x[0], c2, off, s_col + i);
+                        tmem_ld_wait();
+                        if (i + 64 < N) fetch(i + 64, x[0]);
+                        l += weigh<C::kPoly>(x[1], c2, off, s_col + i + 32);
+                    }
+                } else {
+                    float x[N];
+#pragma unroll
+                    for (int i = 0; i < N / 32; ++i)
+                        tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
+                    tmem_ld_wait();
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) x[i] = i > limit ? -INFINITY : x[i];
+                    }
+                    if (!raise(row_max(x))) return;
+                    l += weigh<C::kPoly>(x, c2, m == -INFINITY ? 0.0f : kPOffset - m * c2, s_col);
                 }
-                l += weigh<C::kPoly>(x, c2, m == -INFINITY ? 0.0f : kPOffset - m * c2, s_col);
                 tmem_st_wait();
             }
             tc_fence_before();
@@ -528,46 +570,46 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
 #pragma unroll
                     for (int i = 0; i < BN; i += 32)
                         if (i != c0) tmem_st16(s_col + i, zero);
-                } else if constexpr (C::kHold) {
-                    float x[BN];
-#pragma unroll
-                    for (int i = 0; i < BN / 32; ++i)
-                        tmem_ld32(s_col + i * 32, *reinterpret_cast<uint32_t(*)[32]>(reinterpret_cast<uint32_t*>(x) + i * 32));
-                    tmem_ld_wait();
-                    if (C::CAP) cap_scores(x, cap_in, a.softcap);
-                    if (cut) {
-#pragma unroll
-                        for (int i = 0; i < BN; ++i) x[i] = clip(x[i], i);
-                    }
-                    m = row_max(x);
-                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-#pragma unroll
-                    for (int i = 0; i < BN; i += 32) weigh(x + i, i, pair(off, off));
                 } else {
-                    m = -INFINITY;
+                    // 32 scores at a time in short loops, twice from TMEM, the next ones under way:
+                    // code unrolled over a row outgrows the instruction cache (4096 of 16384, 128
+                    // dims: 1781 us for 1649; 4096 of 8192, 256 dims: 1015 for 861)
+                    float x[2][32];
+                    auto fetch = [&](int i, float (&v)[32]) { tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
+                    auto look = [&](int i, float (&v)[32]) {
+                        if (C::CAP) cap_scores(v, cap_in, a.softcap);
+                        if (cut) {
 #pragma unroll
-                    for (int i = 0; i < BN; i += 32) {
-                        uint32_t r[32];
-                        tmem_ld32(s_col + i, r);
-                        tmem_ld_wait();
-                        if (C::CAP || cut) {
-                            if (C::CAP) cap_scores(*reinterpret_cast<float(*)[32]>(r), cap_in, a.softcap);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(clip(__uint_as_float(r[j]), i + j));
-                            tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(r));
-                            tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(r + 16));
+                            for (int j = 0; j < 32; ++j) v[j] = clip(v[j], i + j);
                         }
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) m = max3(m, __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-                    }
-                    tmem_st_wait();
-                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-#pragma unroll
-                    for (int i = 0; i < BN; i += 32) {
-                        float r[32];
-                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(r));
+                        if (C::CAP || cut) {
+                            tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+                            tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+                        }
+                        m = fmaxf(m, row_max(v));
+                    };
+                    m = -INFINITY;
+                    fetch(0, x[0]);
+#pragma unroll 1
+                    for (int i = 0; i < BN; i += 64) {
                         tmem_ld_wait();
-                        weigh(r, i, pair(off, off));
+                        fetch(i + 32, x[1]);
+                        look(i, x[0]);
+                        tmem_ld_wait();
+                        if (i + 64 < BN) fetch(i + 64, x[0]);
+                        look(i + 32, x[1]);
+                    }
+                    if (C::CAP || cut) tmem_st_wait();
+                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                    fetch(0, x[0]);
+#pragma unroll 1
+                    for (int i = 0; i < BN; i += 64) {
+                        tmem_ld_wait();
+                        fetch(i + 32, x[1]);
+                        weigh(x[0], i, pair(off, off));
+                        tmem_ld_wait();
+                        if (i + 64 < BN) fetch(i + 64, x[0]);
+                        weigh(x[1], i + 32, pair(off, off));
                     }
                 }
                 float s0, s1;
@@ -1096,9 +1138,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) attn_kernel(const __grid_const
     // Registers: the launch's share is 168 a thread with 384 threads and 128 with 512; a wait
     // for more than the launch's sum would not end.
     constexpr int kShare = C::kThreads == 512 ? 128 : (C::kThreads == 384 ? 168 : 255);
-    constexpr int kSoft = C::HL ? (C::D == 64 ? 152 : (C::D == 128 ? 176 : 104)) : (C::NS == 2 ? 208 : 255);
-    constexpr int kCorr = C::HL ? (C::D == 64 ? 112 : (C::D == 128 ? 216 : 160)) : 0;
-    constexpr int kRest = C::HL ? (C::D == 256 ? 88 : (C::D == 128 ? 112 : 96)) : (C::NS == 2 ? 88 : 255);
+    constexpr int kSoft = C::HL ? (C::D == 64 ? 136 : (C::D == 128 ? 176 : 120)) : (C::NS == 2 ? 208 : 255);
+    constexpr int kCorr = C::HL ? (C::D == 64 ? 136 : (C::D == 128 ? 216 : 160)) : 0;
+    constexpr int kRest = C::HL ? (C::D == 256 ? 72 : (C::D == 128 ? 112 : 104)) : (C::NS == 2 ? 88 : 255);
     static_assert(kSoft * C::kSoftWarps + kCorr * C::kCorrWarps + kRest * 4 <= kShare * (C::kThreads / 32), "registers");
     if (warp >= 0 && warp < C::kSoftWarps) {
         set_registers<kShare, kSoft>();

@@ -212,12 +212,6 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
     r1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // N scores (32 at a time) to cap * tanh(s * in), in = scale / cap.  Where no lane of the warp has
 // |s * in| above 1, by the odd minimax polynomial of tanh there (degree 13, Remez; 1.7e-7 relative
 // with f32 rounding) on the FMA pipe; else cap (1 - e) / (1 + e), e = exp(-2 |s in|), whose two
@@ -233,18 +227,16 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], float in, float cap) {
             top[1] = max3(top[1], fabsf(x[i + j + 2]), fabsf(x[i + j + 3]));
         }
         if (__all_sync(~0u, fmaxf(top[0], top[1]) * in <= 1.0f)) {
-            const uint64_t k = pair(in, in), c = pair(cap, cap);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                const uint64_t t = mul2(pair(x[i + j], x[i + j + 1]), k), q = mul2(t, t);
-                uint64_t p = pair(0.0010582648683339357f, 0.0010582648683339357f);
-                p = fma2(p, q, pair(-0.006259339861571789f, -0.006259339861571789f));
-                p = fma2(p, q, pair(0.020359760150313377f, 0.020359760150313377f));
-                p = fma2(p, q, pair(-0.053498707711696625f, -0.053498707711696625f));
-                p = fma2(p, q, pair(0.13326409459114075f, 0.13326409459114075f));
-                p = fma2(p, q, pair(-0.33332985639572144f, -0.33332985639572144f));
-                p = fma2(p, q, pair(1.0f, 1.0f));
-                unpair(mul2(mul2(t, p), c), x[i + j], x[i + j + 1]);
+            for (int j = 0; j < 32; ++j) {
+                const float t = x[i + j] * in, q = t * t;
+                float p = fmaf(0.0010582648683339357f, q, -0.006259339861571789f);
+                p = fmaf(p, q, 0.020359760150313377f);
+                p = fmaf(p, q, -0.053498707711696625f);
+                p = fmaf(p, q, 0.13326409459114075f);
+                p = fmaf(p, q, -0.33332985639572144f);
+                p = fmaf(p, q, 1.0f);
+                x[i + j] = t * cap * p;
             }
         } else {
             const float k = -2.0f * 1.4426950408889634f * in;
