@@ -269,7 +269,7 @@ typedef struct {
     const void* q;               /* rows [token][head][head_dim]: q_nb = element, head, token */
     const void* k;
     const void* v;
-    void* q_dst;                 /* rotated q; may be q itself */
+    void* q_dst;                 /* rotated q; may be q itself (with the same strides) */
     size_t q_nb[3], k_nb[3], v_nb[3], q_dst_nb[3];   /* heads and tokens on 16-byte boundaries */
 } mlzc_paged_store_desc;
 
@@ -284,7 +284,7 @@ typedef struct {
     uint32_t mode;               /* 0 or MLZC_FA_MODE_SOFTCAP (slots are no positions after an
                                     eviction, so ALiBi is not taken) */
     int64_t n_head_q;            /* a multiple of n_head_kv, at most 128 times it */
-    float scale, logit_softcap;  /* scale > 0 */
+    float scale, logit_softcap;  /* each (softcap in SOFTCAP mode) from 2^-40 to 2^40 */
     const void* q;               /* [token][head][head_dim], q_nb = element, head, token */
     void* dst;                   /* the same shape */
     size_t q_nb[3], dst_nb[3];   /* heads and tokens on 16-byte boundaries */
@@ -302,7 +302,8 @@ int mlzc_paged_attn_workspace_bytes(const mlzc_paged_cache* cache, const mlzc_pa
  * softcap * tanh(s / softcap) in SOFTCAP mode; KV head of query head h: h * n_head_kv /
  * n_head_q.  A token that sees nothing gets zeros and lse = -inf.
  * type F32: q, the weights and the sums keep f32 precision (q and the softmax weights go
- * through the tensor cores as f16 hi + lo pairs); type F16: q is f16 as given, the softmax
+ * through the tensor cores as f16 hi + lo pairs, so |q| <= 65504, and parts of q below
+ * 2^-25 are lost); type F16: q is f16 as given, the softmax
  * weights are rounded to f16 once, sums are f32, dst is rounded once.
  * K and V of the slots below kv_len are finite. */
 int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, void* workspace,

@@ -345,7 +345,7 @@ int launch_select(EvictArgs& a, const DeviceCtx* c, cudaStream_t s) {
     // CTAs of kShare slots, as long as every head's are on the GPU together
     int ranks = 1;
     while (ranks < kRanks && (int64_t)a.c.n_head_kv * a.c.batch * 2 * ranks <= c->sm_count && a.c.cap > ranks * kShare) ranks *= 2;
-    a.held = std::min(kHeldSlots, (a.c.cap + ranks - 1) / ranks);
+    a.held = std::min(kHeldSlots, ((a.c.cap + ranks - 1) / ranks + 31) / 32 * 32);
     const size_t smem = (size_t)a.held * 4;
     static bool set[64] = {};
     const int dev = c->device < 64 ? c->device : 63;

@@ -124,9 +124,11 @@ int check_attn(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, boo
     if (d->n_head_q < 1 || d->n_head_q % cache->n_head_kv || d->n_head_q / cache->n_head_kv > 128)
         return fail(MLZC_ERR_UNSUPPORTED, "paged attention: %lld query heads on %lld kv heads (a multiple, at most 128 times)",
                     (long long)d->n_head_q, (long long)cache->n_head_kv);
-    if (!(d->scale > 0.0f) || !std::isfinite(d->scale)) return fail(MLZC_ERR_INVALID, "paged attention: scale must be positive");
-    if ((d->mode & MLZC_FA_MODE_SOFTCAP) && (!(d->logit_softcap > 0.0f) || !std::isfinite(d->logit_softcap)))
-        return fail(MLZC_ERR_INVALID, "paged attention: SOFTCAP mode with softcap %g", (double)d->logit_softcap);
+    // their products and quotients with one another and with scores stay inside f32
+    auto usable = [](float x) { return x >= 0x1p-40f && x <= 0x1p40f; };
+    if (!usable(d->scale)) return fail(MLZC_ERR_INVALID, "paged attention: scale %g (2^-40 to 2^40)", (double)d->scale);
+    if ((d->mode & MLZC_FA_MODE_SOFTCAP) && !usable(d->logit_softcap))
+        return fail(MLZC_ERR_INVALID, "paged attention: SOFTCAP mode with softcap %g (2^-40 to 2^40)", (double)d->logit_softcap);
     if (cache->n_tokens == 0) return MLZC_OK;
     if (cache->n_tokens * d->n_head_q > kMaxInt) return fail(MLZC_ERR_INVALID, "paged attention: too many query rows");
     const size_t elem = d->type == MLZC_TYPE_F32 ? 4 : 2, row = (size_t)cache->head_dim * elem;

@@ -194,6 +194,8 @@ extern "C" int mlzc_paged_store_dev(const mlzc_paged_cache* cache, const mlzc_pa
     if (st == MLZC_OK && d->n_head_q) st = paged::check_rows("paged store: q", d->q, d->q_nb, d->n_head_q, T, rb, elem);
     if (st == MLZC_OK && d->n_head_q) st = paged::check_rows("paged store: q_dst", d->q_dst, d->q_dst_nb, d->n_head_q, T, rb, elem);
     if (st != MLZC_OK) return st;
+    if (d->n_head_q && d->q == d->q_dst && ((d->n_head_q > 1 && d->q_nb[1] != d->q_dst_nb[1]) || (T > 1 && d->q_nb[2] != d->q_dst_nb[2])))
+        return fail(MLZC_ERR_INVALID, "paged store: q_dst in place with other strides");
     DeviceCtx* c = current_ctx();
     if (!c) return MLZC_ERR_CUDA;
     st = paged::make_view(cache, true, c, &a.c);

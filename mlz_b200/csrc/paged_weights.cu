@@ -19,8 +19,11 @@
 // (K by one TMA box a page piece, Q by one box a 64-dim block), MMA warp (scores into four TMEM
 // buffers, as many columns as there are rows), two lse warps (a tile's lse2 into shared memory),
 // four warpgroups that take turns at the tiles (with two
-// the exponential unit idled half of the time: 205 us for 2048 tokens of 8192).  f32 queries come as f16 hi + lo from a small
-// preparing launch, low products summed first.
+// the exponential unit idled half of the time: 205 us for 2048 tokens of 8192).  f32 queries come
+// as f16 hi + lo from a small preparing launch, low products summed first.
+//
+// lse2 is rounded to f32 once a row (4e-7 of a weight at lse 10).  Carrying what that drops as a
+// factor a column made no weight better (the products' own sums are as far off) and cost 12 %.
 //
 // Slot tiles x query tiles of a call form one list cut into equal shares, as in paged_attn.cu;
 // a cut slot tile's 128 partial sums are merged in order by a last launch.

@@ -119,6 +119,21 @@ def test_attn_refusals(kw, status, says):
         assert st == status and says in mlz_b200.last_error(), mlz_b200.last_error()
 
 
+@pytest.mark.parametrize("kw,says", [(dict(scale=2.0 ** -41), "scale"), (dict(scale=2.0 ** 41), "scale"),
+                                     (dict(mode=16, logit_softcap=2.0 ** -41), "softcap"), (dict(mode=16, logit_softcap=2.0 ** 41), "softcap")])
+def test_scales_outside_f32s_room_are_refused(kw, says):
+    """Products of such a scale with scores, or its inverse, would leave f32."""
+    L = mlz_b200.lib()
+    assert L.mlzc_paged_attn_dev(C.byref(cache()), C.byref(attn(**kw)), None, 0, None) == INVALID and says in mlz_b200.last_error()
+
+
+def test_rotation_in_place_with_other_strides_is_refused():
+    L = mlz_b200.lib()
+    for nb in ((4, 1024, 8 * 1024), (4, 512, 16 * 512)):
+        assert L.mlzc_paged_store_dev(C.byref(cache()), C.byref(store(q_dst_nb=nb)), None) == INVALID
+        assert "in place" in mlz_b200.last_error()
+
+
 def test_attn_and_weights_own_refusals():
     L, nb = mlz_b200.lib(), (C.c_size_t * 3)(4, 256, 512)
     c = cache()
