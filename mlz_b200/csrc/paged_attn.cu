@@ -355,6 +355,42 @@ __device__ __forceinline__ float weigh(const float (&x)[N], float c2, float off,
     return s0 + s1;
 }
 
+// f(i, 32 scores from column i on) for N scores at s_col, the next ones under way: a short loop,
+// because code unrolled over a row outgrows the instruction cache (4096 of 16384, 128 dims f32:
+// 1781 us for 1649; 1024 of 2048 capped, 256 dims: 233 for 113), with one copy of its body
+// (two, to save the moves: 122).
+template <int N, typename F>
+__device__ __forceinline__ void each32(uint32_t s_col, F f) {
+    float x[32], v[32];
+    tmem_ld32(s_col, *reinterpret_cast<uint32_t(*)[32]>(x));
+#pragma unroll 1
+    for (int i = 0; i < N; i += 32) {
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = x[j];
+        if (i + 32 < N) tmem_ld32(s_col + i + 32, *reinterpret_cast<uint32_t(*)[32]>(x));
+        f(i, v);
+    }
+}
+
+// N scores at s_col capped, those past `limit` masked where `cut`, back in place; the largest.
+template <int N>
+__device__ __forceinline__ float cap_row(uint32_t s_col, float cap_in, float cap, bool cut, int limit) {
+    float top = -INFINITY;
+    each32<N>(s_col, [&](int i, float (&v)[32]) {
+        cap_scores(v, cap_in, cap);
+        if (cut) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = i + j > limit ? -INFINITY : v[j];
+        }
+        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+        tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+        top = fmaxf(top, row_max(v));
+    });
+    tmem_st_wait();
+    return top;
+}
+
 // Softmax of an f16 call, step by step (a tile, or half of one: Cfg::H).
 template <class C>
 __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_t tmem, int warp, int lane) {
@@ -409,43 +445,10 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                     return true;
                 };
                 if constexpr (C::CAP) {
-                    // 32 scores at a time in short loops, twice from TMEM: unrolled over a row the code
-                    // of a capped step outgrows the instruction cache (256 dims: 233 us for 149)
-                    float top = -INFINITY, x[2][32];
-                    auto fetch = [&](int i, float (&v)[32]) { tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
-                    auto look = [&](int i, float (&v)[32]) {
-                        cap_scores(v, cap_in, a.softcap);
-                        if (cut) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = i + j > limit ? -INFINITY : v[j];
-                        }
-                        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
-                        tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
-                        top = fmaxf(top, row_max(v));
-                    };
-                    fetch(0, x[0]);
-#pragma unroll 1
-                    for (int i = 0; i < N; i += 64) {
-                        tmem_ld_wait();
-                        fetch(i + 32, x[1]);
-                        look(i, x[0]);
-                        tmem_ld_wait();
-                        if (i + 64 < N) fetch(i + 64, x[0]);
-                        look(i + 32, x[1]);
-                    }
-                    tmem_st_wait();
+                    const float top = cap_row<N>(s_col, cap_in, a.softcap, cut, limit);
                     if (!raise(top)) return;
                     const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                    fetch(0, x[0]);
-#pragma unroll 1
-                    for (int i = 0; i < N; i += 64) {
-                        tmem_ld_wait();
-                        fetch(i + 32, x[1]);
-                        l += weigh<C::kPoly>(x[0], c2, off, s_col + i);
-                        tmem_ld_wait();
-                        if (i + 64 < N) fetch(i + 64, x[0]);
-                        l += weigh<C::kPoly>(x[1], c2, off, s_col + i + 32);
-                    }
+                    each32<N>(s_col, [&](int i, float (&v)[32]) { l += weigh<C::kPoly>(v, c2, off, s_col + i); });
                 } else {
                     float x[N];
 #pragma unroll
@@ -517,27 +520,6 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                 const uint64_t c22 = pair(c2, c2);
                 uint64_t sum[2] = {0, 0};
                 float m;
-                // 32 slots of P from their scores
-                auto weigh = [&](const float* x, int i, uint64_t off2) {
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        float p0, p1, h0, h1;
-                        unpair(fma2(pair(x[2 * j], x[2 * j + 1]), c22, off2), p0, p1);
-                        p0 = ex2(p0);
-                        p1 = ex2(p1);
-                        const uint64_t p = pair(p0, p1);
-                        sum[j & 1] = add2(sum[j & 1], p);
-                        // hi: the first 11 bits (f16 holds them), lo: the rest, within 2^-22
-                        h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
-                        h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
-                        hi[j] = ptx::pack_h2(h0, h1);
-                        unpair(fma2(pair(h0, h1), pair(-1.0f, -1.0f), p), p0, p1);
-                        lo[j] = ptx::pack_h2(p0, p1);
-                    }
-                    tmem_st16(s_col + i, hi);
-                    tmem_st16(s_col + i + 16, lo);
-                };
                 auto clip = [&](float x, int i) { return i > limit ? -INFINITY : x; };
                 if (C::kSpread && spread) {
                     // this warp's quarter of the slots; lane and lane ^ 16 have the parts of a score
@@ -571,45 +553,56 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                     for (int i = 0; i < BN; i += 32)
                         if (i != c0) tmem_st16(s_col + i, zero);
                 } else {
-                    // 32 scores at a time in short loops, twice from TMEM, the next ones under way:
-                    // code unrolled over a row outgrows the instruction cache (4096 of 16384, 128
-                    // dims: 1781 us for 1649; 4096 of 8192, 256 dims: 1015 for 861)
-                    float x[2][32];
-                    auto fetch = [&](int i, float (&v)[32]) { tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(v)); };
-                    auto look = [&](int i, float (&v)[32]) {
-                        if (C::CAP) cap_scores(v, cap_in, a.softcap);
-                        if (cut) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = clip(v[j], i + j);
-                        }
-                        if (C::CAP || cut) {
-                            tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
-                            tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
-                        }
-                        m = fmaxf(m, row_max(v));
-                    };
+                    // short loops, the scores read twice from TMEM (see each32)
                     m = -INFINITY;
-                    fetch(0, x[0]);
+                    if constexpr (C::CAP) {
+                        m = cap_row<BN>(s_col, cap_in, a.softcap, cut, limit);
+                    } else {
 #pragma unroll 1
-                    for (int i = 0; i < BN; i += 64) {
-                        tmem_ld_wait();
-                        fetch(i + 32, x[1]);
-                        look(i, x[0]);
-                        tmem_ld_wait();
-                        if (i + 64 < BN) fetch(i + 64, x[0]);
-                        look(i + 32, x[1]);
+                        for (int i = 0; i < BN; i += 32) {
+                            float v[32];
+                            tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(v));
+                            tmem_ld_wait();
+                            if (cut) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = clip(v[j], i + j);
+                                tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+                                tmem_st16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
+                            }
+                            m = fmaxf(m, row_max(v));
+                        }
+                        if (cut) tmem_st_wait();
                     }
-                    if (C::CAP || cut) tmem_st_wait();
                     const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                    fetch(0, x[0]);
+                    float x[16];
+                    tmem_ld16(s_col, *reinterpret_cast<uint32_t(*)[16]>(x));
+                    tmem_ld_wait();
 #pragma unroll 1
-                    for (int i = 0; i < BN; i += 64) {
-                        tmem_ld_wait();
-                        fetch(i + 32, x[1]);
-                        weigh(x[0], i, pair(off, off));
-                        tmem_ld_wait();
-                        if (i + 64 < BN) fetch(i + 64, x[0]);
-                        weigh(x[1], i + 32, pair(off, off));
+                    for (int i = 0; i < BN; i += 16) {
+                        uint64_t y[8];
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) y[j] = fma2(pair(x[2 * j], x[2 * j + 1]), c22, pair(off, off));
+                        if (i + 16 < BN) tmem_ld16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(x));
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            float p0, p1;
+                            unpair(y[j], p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                            const uint64_t p = pair(p0, p1);
+                            sum[j & 1] = add2(sum[j & 1], p);
+                            // hi: the first 11 bits (f16 holds them), lo: the rest, within 2^-22
+                            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                            const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                            hi[j] = ptx::pack_h2(h0, h1);
+                            unpair(fma2(pair(h0, h1), pair(-1.0f, -1.0f), p), p0, p1);
+                            lo[j] = ptx::pack_h2(p0, p1);
+                        }
+                        tmem_ld_wait();                  // lo lies over the scores just fetched
+                        const uint32_t to = s_col + (i & ~31) + (i >> 1 & 15);
+                        tmem_st8(to, hi);
+                        tmem_st8(to + 16, lo);
                     }
                 }
                 float s0, s1;

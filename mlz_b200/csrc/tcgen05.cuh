@@ -86,6 +86,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory descriptors in halves, for issue loops: K-major tiles as in umma_desc_sw128, and
@@ -212,39 +218,35 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
     r1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
-// N scores (32 at a time) to cap * tanh(s * in), in = scale / cap.  Where no lane of the warp has
-// |s * in| above 1, by the odd minimax polynomial of tanh there (degree 13, Remez; 1.7e-7 relative
-// with f32 rounding) on the FMA pipe; else cap (1 - e) / (1 + e), e = exp(-2 |s in|), whose two
-// more uses of the exponential unit a score would be the bound.
+// N scores to cap * tanh(s * in), in = scale / cap.  Where no lane of the warp has |s * in| above 1,
+// by the odd minimax polynomial of tanh there (degree 13, Remez; 1.7e-7 relative with f32 rounding)
+// on the FMA pipe; else cap (1 - e) / (1 + e), e = exp(-2 |s in|), whose two more uses of the
+// exponential unit a score would be the bound.
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&x)[N], float in, float cap) {
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i += 32) {
-        float top[2] = {0.0f, 0.0f};
+    for (int j = 0; j < N; ++j) x[j] *= in;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            top[0] = max3(top[0], fabsf(x[i + j]), fabsf(x[i + j + 1]));
-            top[1] = max3(top[1], fabsf(x[i + j + 2]), fabsf(x[i + j + 3]));
+    for (int j = 0; j < N; j += 2) top = max3(top, fabsf(x[j]), fabsf(x[j + 1]));
+    if (__all_sync(~0u, top <= 1.0f)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float t = x[j], q = t * t;
+            float p = fmaf(0.0010582648683339357f, q, -0.006259339861571789f);
+            p = fmaf(p, q, 0.020359760150313377f);
+            p = fmaf(p, q, -0.053498707711696625f);
+            p = fmaf(p, q, 0.13326409459114075f);
+            p = fmaf(p, q, -0.33332985639572144f);
+            p = fmaf(p, q, 1.0f);
+            x[j] = t * cap * p;
         }
-        if (__all_sync(~0u, fmaxf(top[0], top[1]) * in <= 1.0f)) {
+    } else {
+        const float k = -2.0f * 1.4426950408889634f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float t = x[i + j] * in, q = t * t;
-                float p = fmaf(0.0010582648683339357f, q, -0.006259339861571789f);
-                p = fmaf(p, q, 0.020359760150313377f);
-                p = fmaf(p, q, -0.053498707711696625f);
-                p = fmaf(p, q, 0.13326409459114075f);
-                p = fmaf(p, q, -0.33332985639572144f);
-                p = fmaf(p, q, 1.0f);
-                x[i + j] = t * cap * p;
-            }
-        } else {
-            const float k = -2.0f * 1.4426950408889634f * in;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const float e = ex2(fabsf(x[i + j]) * k);
-                x[i + j] = copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, x[i + j]);
-            }
+        for (int j = 0; j < N; ++j) {
+            const float e = ex2(fabsf(x[j]) * k);
+            x[j] = copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, x[j]);
         }
     }
 }
