@@ -30,7 +30,8 @@ using paged::View;
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;                   // 11 bits a radix pass
-constexpr int kHeldSlots = 24576;             // weights of so many slots fit beside a second CTA's
+constexpr int kHeldSlots = 32768;             // keys of so many slots fit in a CTA's shared memory,
+constexpr int kHeldHoles = 8192;              // and the holes of such a budget beside them
 
 struct EvictArgs {
     View c;
@@ -39,10 +40,10 @@ struct EvictArgs {
     char* w_out;
     char* kept;
     int* kv_len_out;
-    int* holes;                               // workspace: [batch][head][budget]
-    uint32_t* words;                          // workspace: [batch][head][n_words], a bit a slot that stays
+    int* holes;                               // workspace: [batch][head][budget], for heads of several CTAs
+    uint32_t* words;                          // workspace: [batch][head][n_words], a bit a slot that stays, for long heads
     int n_words;
-    int held;                                 // slots of shared memory for weights (0: read from global memory)
+    int held, held_holes;                     // slots and holes that shared memory has room for
     size_t w_head, w_seq, o_head, o_seq, kept_head, kept_seq;
 };
 
@@ -61,13 +62,15 @@ constexpr int kShare = 4096;                  // slots worth a CTA of a cluster 
 // Shared memory of a selecting CTA.
 struct Sel {
     int4 hist[3][kBins / 4];                  // of each pass
-    int sums[6][kSelWarps];                   // warps' sums, a row a scan
+    int coarse[3][kSelWarps];                 // the same in blocks of 64 digits
+    int sums[3][kSelWarps];                   // warps' sums, a row a scan
     int found[3][3];                          // the digit, how many keys lie above it, how many have it
     int count[3];                             // this CTA's equals, holes, movers
     int listed;
     uint32_t list[2048];                      // keys with the first digit found, where they are few
 };
 constexpr int kList = 2048;
+constexpr uint32_t kForced = 0xFFFFFFFFu;     // key of a slot that stays anyway: above every weight's
 
 __device__ __forceinline__ int warp_sum(int x) { return __reduce_add_sync(~0u, x); }
 
@@ -76,25 +79,48 @@ __device__ __forceinline__ int warps_before(int mine, int* total, int* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane == 0) sh[warp] = mine;
     __syncthreads();
-    const int x = lane < kSelWarps ? sh[lane] : 0;
+    const int x = sh[lane];
     *total = warp_sum(x);
     return warp_sum(lane < warp ? x : 0);
 }
 
+// Of 32 x K counts, K a lane in ascending order, the place of the need-th from the top: its index
+// (warp-wide), the counts above it, its own.
+template <int K>
+__device__ __forceinline__ int3 find_from_top(const int (&c)[K], int need) {
+    const int lane = threadIdx.x & 31;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) mine += c[i];
+    int upto = mine;                          // of this lane and those above
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_down_sync(~0u, upto, o);
+        if (lane + o < 32) upto += y;
+    }
+    const int at = 31 - __clz(__ballot_sync(~0u, upto >= need));
+    int above = upto - mine, k = K - 1, have = c[K - 1];
+#pragma unroll
+    for (int i = K - 2; i >= 0; --i)
+        if (above + have < need) { above += have; have = c[i]; k = i; }
+    return make_int3(__shfl_sync(~0u, lane * K + k, at), __shfl_sync(~0u, above, at), __shfl_sync(~0u, have, at));
+}
+
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ EvictArgs a) {
     __shared__ Sel sel;
-    extern __shared__ float held[];
+    extern __shared__ uint32_t held[];        // keys, bits of the slots that stay, holes
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int n = paged::load_seq(a.c, b, false).kv;
+    for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) sel.hist[0][i] = make_int4(0, 0, 0, 0);
+    if (tid == 0) sel.listed = 0;
     const int size = min(n, a.budget);
     const float* w = reinterpret_cast<const float*>(a.w + (size_t)b * a.w_seq + (size_t)h * a.w_head);
     float* wo = reinterpret_cast<float*>(a.w_out + (size_t)b * a.o_seq + (size_t)h * a.o_head);
     int* kept = reinterpret_cast<int*>(a.kept + (size_t)b * a.kept_seq + (size_t)h * a.kept_head);
-    int* holes = a.holes + ((size_t)b * a.c.n_head_kv + h) * a.budget;
     auto sync = [&]() {
         if (ranks == 1) __syncthreads();
         else cluster.sync();
@@ -112,91 +138,85 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     // every 32nd slot, so that loads and stores are whole lines and a slot's rank is a count of
     // ballot bits.  Short loops on purpose: each phase runs once a launch, and with 16 slots a
     // lane unrolled the selection of 8 heads of 32768 slots took 35 us.
-    const int lane = tid & 31, warp = tid >> 5;
-    const int share = ((n + ranks - 1) / ranks + 31) / 32 * 32, s0 = min(n, rank * share), s1 = min(n, s0 + share);
-    const int run = ((share + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, w0 = min(s1, s0 + warp * run), w1 = min(s1, w0 + run);
+    const int lane = tid & 31, warp = tid >> 5, log_ranks = 31 - __clz(ranks);
+    const int share = (((n + ranks - 1) >> log_ranks) + 31) & ~31, s0 = min(n, rank * share), s1 = min(n, s0 + share);
+    const int run = (share / kSelWarps + 31) & ~31, w0 = min(s1, s0 + warp * run), w1 = min(s1, w0 + run);
     const bool hold = share <= a.held;
     const uint32_t below = (1u << lane) - 1;
-    uint32_t* words = a.words + ((size_t)b * a.c.n_head_kv + h) * a.n_words;
+    const int lo = a.sink, hi = n - a.recent;          // candidates
+    int need = a.budget;                               // with the forced ones; fewer than n
+    const size_t head = (size_t)b * a.c.n_head_kv + h;
+    uint32_t* words = hold ? held + a.held : a.words + head * a.n_words + (s0 >> 5);
+    int* holes = ranks == 1 && a.budget <= a.held_holes ? reinterpret_cast<int*>(held + a.held + a.held / 32) : a.holes + head * a.budget;
+    auto key_of = [&](int i) { return i < lo || i >= hi ? kForced : order_key(ptx::ld_act(w + i)); };
     if (hold) {
 #pragma unroll 4
-        for (int i = w0 + lane; i < w1; i += 32) held[i - s0] = ptx::ld_act(w + i);   // read by the same lane alone
+        for (int i = w0 + lane; i < w1; i += 32) held[i - s0] = key_of(i);   // read by the same lane alone
     }
-    // f(slot, weight) for this lane's slots; every lane of the warp comes along (slots at or past
-    // w1 are none of its)
+    // f(slot, key) for this lane's slots; every lane of the warp comes along (slots at or past w1
+    // are none of its)
     auto each = [&](auto f) {
 #pragma unroll 2
-        for (int i = w0 + lane; i - lane < w1; i += 32) f(i, i < w1 ? (hold ? held[i - s0] : ptx::ld_act(w + i)) : 0.0f);
+        for (int i = w0 + lane; i - lane < w1; i += 32) f(i, i < w1 ? (hold ? held[i - s0] : key_of(i)) : 0u);
     };
-    // the same with the bits of the 32 slots that stay
-    auto each_word = [&](auto f) {
-#pragma unroll 2
-        for (int i = w0 + lane; i - lane < w1; i += 32) f(i, *reinterpret_cast<volatile uint32_t*>(words + (i >> 5)));
-    };
-    auto weight = [&](int i) { return hold ? held[i - s0] : ptx::ld_act(w + i); };
-    const int lo = a.sink, hi = n - a.recent;          // candidates
-    int need = a.budget - a.sink - a.recent;           // of which so many stay (fewer than hi - lo)
-    const bool choose = need > 0;
+    __syncthreads();
     uint32_t prefix = 0, mask = 0;
-    if (choose) {
-        for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) sel.hist[0][i] = make_int4(0, 0, 0, 0);
-        if (tid == 0) sel.listed = 0;
-        __syncthreads();
 #pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
-            int* hist = reinterpret_cast<int*>(sel.hist[pass]);
-            const bool few = pass > 0 && sel.found[0][2] <= kList;
-            if (few && pass == 2) {
-                for (int i = tid; i < sel.listed; i += kSelThreads)
-                    if ((sel.list[i] & mask) == prefix) atomicAdd(&hist[sel.list[i] & (bins - 1)], 1);
-            } else {
-                each([&](int i, float v) {
-                    const uint32_t k = order_key(v);
-                    const bool in = i < w1 && i >= lo && i < hi && (k & mask) == prefix;
-                    if (in) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
-                    if (few && in) sel.list[atomicAdd(&sel.listed, 1)] = k;
-                });
-            }
-            sync();
-            // from the top: the digit whose keys hold the need-th largest; each thread owns four
-            const int p = tid < kBins / 4 ? bins / 4 - 1 - tid : -1;
-            int c[4] = {0, 0, 0, 0};
-            if (p >= 0) {
-                if (ranks == 1) {
-                    const int4 v = sel.hist[pass][p];
-                    c[0] = v.w; c[1] = v.z; c[2] = v.y; c[3] = v.x;
-                } else {
-                    int4 v[kRanks];
-#pragma unroll
-                    for (int r = 0; r < kRanks; ++r) v[r] = r < ranks ? cluster.map_shared_rank(sel.hist[pass], r)[p] : make_int4(0, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < kRanks; ++r) { c[0] += v[r].w; c[1] += v[r].z; c[2] += v[r].y; c[3] += v[r].x; }
-                }
-            }
-            const int mine = c[0] + c[1] + c[2] + c[3];
-            int upto = mine, total;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(~0u, upto, o);
-                if (lane >= o) upto += y;
-            }
-            int before = warps_before(__shfl_sync(~0u, upto, 31), &total, sel.sums[pass]) + upto - mine;
-            if (before < need && need <= before + mine) {
-                int k = 0;
-                while (need > before + c[k]) before += c[k++];
-                sel.found[pass][0] = 4 * p + 3 - k;
-                sel.found[pass][1] = before;
-                sel.found[pass][2] = c[k];
-            }
-            __syncthreads();
-            prefix |= (uint32_t)sel.found[pass][0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            need -= sel.found[pass][1];
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), digits = pass == 2 ? 1023 : 2047;
+        int* hist = reinterpret_cast<int*>(sel.hist[pass]);
+        const bool few = pass > 0 && sel.found[0][2] <= kList;
+        if (few && pass == 2) {
+            for (int i = tid; i < sel.listed; i += kSelThreads)
+                if ((sel.list[i] & mask) == prefix) atomicAdd(&hist[sel.list[i] & digits], 1);
+        } else {
+            each([&](int i, uint32_t k) {
+                const bool in = i < w1 && (k & mask) == prefix;
+                if (in) atomicAdd(&hist[(k >> shift) & digits], 1);
+                if (few && in) sel.list[atomicAdd(&sel.listed, 1)] = k;
+            });
         }
+        // the digit whose keys hold the need-th largest: its block of 64 first, then the digit, so
+        // that a cluster's CTAs read little of one another's
+        __syncthreads();
+        const int2 mine = reinterpret_cast<const int2*>(hist)[tid];
+        const int sum = warp_sum(mine.x + mine.y);
+        if (lane == 0) sel.coarse[pass][warp] = sum;
+        sync();
+        if (warp == 0) {
+            int c[1] = {0}, d[2] = {0, 0};
+            if (ranks == 1) {
+                c[0] = sel.coarse[pass][lane];
+            } else {
+#pragma unroll
+                for (int r = 0; r < kRanks; ++r) c[0] += r < ranks ? *cluster.map_shared_rank(&sel.coarse[pass][lane], r) : 0;
+            }
+            const int3 block = find_from_top(c, need);
+            const int2* fine = reinterpret_cast<const int2*>(hist) + block.x * 32 + lane;
+            if (ranks == 1) {
+                d[0] = fine->x;
+                d[1] = fine->y;
+            } else {
+                int2 v[kRanks];
+#pragma unroll
+                for (int r = 0; r < kRanks; ++r) v[r] = r < ranks ? *cluster.map_shared_rank(fine, r) : make_int2(0, 0);
+#pragma unroll
+                for (int r = 0; r < kRanks; ++r) { d[0] += v[r].x; d[1] += v[r].y; }
+            }
+            const int3 digit = find_from_top(d, need - block.y);
+            if (lane == 0) {
+                sel.found[pass][0] = block.x * 64 + digit.x;
+                sel.found[pass][1] = block.y + digit.y;
+                sel.found[pass][2] = digit.z;
+            }
+        }
+        __syncthreads();
+        prefix |= (uint32_t)sel.found[pass][0] << shift;
+        mask |= (uint32_t)digits << shift;
+        need -= sel.found[pass][1];
     }
-    // Candidates above `prefix` stay, and the first `need` equal to it.  Counts of the CTAs before
-    // this one come from their shared memory.
+    // Keys above `prefix` stay, and the first `need` equal to it.  Counts of the CTAs before this
+    // one come from their shared memory.
     auto from_others = [&](int which) {
         int sum = 0;
         if (ranks > 1) {
@@ -205,40 +225,35 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
         }
         return sum;
     };
-    auto equal = [&](int i, float v) { return i < w1 && i >= lo && i < hi && order_key(v) == prefix; };
     // equal keys need counting in order only where not all of them stay
-    const bool ties = choose && sel.found[2][2] > need;
+    const bool ties = sel.found[2][2] > need;
     int equals = 0, total;
     if (ties) {
         int mine = 0;
-        each([&](int i, float v) { mine += __popc(__ballot_sync(~0u, equal(i, v))); });
-        equals = warps_before(mine, &total, sel.sums[3]);
+        each([&](int i, uint32_t k) { mine += i < w1 && k == prefix; });
+        equals = warps_before(warp_sum(mine), &total, sel.sums[0]);
         if (tid == 0) sel.count[0] = total;
         sync();
         equals += from_others(0);
     }
     // which slots stay, and how many are holes and movers
     int nh = 0, nm = 0;
-    each([&](int i, float v) {
-        const uint32_t k = order_key(v);
-        const bool inside = i >= lo && i < hi;
-        bool s = !inside || (choose && k >= prefix);
+    each([&](int i, uint32_t k) {
+        bool s = i < w1 && k >= prefix;
         if (ties) {
-            const bool eq = i < w1 && inside && k == prefix;
+            const bool eq = i < w1 && k == prefix;
             const uint32_t bits = __ballot_sync(~0u, eq);
             if (eq) s = equals + __popc(bits & below) < need;
             equals += __popc(bits);
         }
-        const uint32_t stay = __ballot_sync(~0u, i < w1 && s);
-        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(words + (i >> 5)) = stay;
-        const int i0 = i - lane;
-        const uint32_t real = w1 - i0 >= 32 ? ~0u : (1u << (w1 - i0)) - 1, front = size - i0 >= 32 ? ~0u : (size > i0 ? (1u << (size - i0)) - 1 : 0);
-        nh += __popc(real & front & ~stay);
-        nm += __popc(stay & ~front);
+        const uint32_t stay = __ballot_sync(~0u, s);
+        if (lane == 0) words[(i - s0) >> 5] = stay;
+        nh += i < min(w1, size) && !s;
+        nm += i >= size && s;
     });
     __syncwarp();
     int th, tm;
-    int rh = warps_before(nh, &th, sel.sums[4]), rm = warps_before(nm, &tm, sel.sums[5]);
+    int rh = warps_before(warp_sum(nh), &th, sel.sums[1]), rm = warps_before(warp_sum(nm), &tm, sel.sums[2]);
     if (tid == 0) {
         sel.count[1] = th;
         sel.count[2] = tm;
@@ -246,30 +261,45 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     sync();
     rh += from_others(1);
     rm += from_others(2);
-    if (w0 < size)
-        each_word([&](int i, uint32_t stay) {
-            const bool mine = i < w1 && i < size, s = stay >> lane & 1, hole = mine && !s;
-            const uint32_t bits = __ballot_sync(~0u, hole);
-            if (hole) holes[rh + __popc(bits & below)] = i;
-            rh += __popc(bits);
-            if (mine && s) {
-                kept[i] = i;
-                if (wo != w) wo[i] = weight(i);
-            }
-        });
+#pragma unroll 1
+    for (int i = w0 + lane; i - lane < min(w1, size); i += 32) {
+        const bool mine = i < min(w1, size), s = words[(i - s0) >> 5] >> lane & 1;
+        const uint32_t bits = __ballot_sync(~0u, mine && !s);
+        if (mine && !s) holes[rh + __popc(bits & below)] = i;
+        rh += __popc(bits);
+        if (mine && s) {
+            kept[i] = i;
+            if (wo != w) wo[i] = ptx::ld_act(w + i);
+        }
+    }
     sync();                                   // every hole is listed, every count read
-    if (w1 > size)
-        each_word([&](int i, uint32_t stay) {
+    // four words at a time, their holes and weights on the way together
+    constexpr int U = 4;
+    const int from = max(w0, size & ~31);
+#pragma unroll 1
+    for (int i0 = from + lane; i0 - lane < w1; i0 += 32 * U) {
+        int to[U];
+        float x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 32 * u;
+            const uint32_t stay = i - lane < w1 ? words[(i - s0) >> 5] : 0;
             const bool mover = i >= size && (stay >> lane & 1);
             const uint32_t bits = __ballot_sync(~0u, mover);
-            if (mover) {
-                const int to = holes[rm + __popc(bits & below)];
-                kept[to] = i;
-                wo[to] = weight(i);
-            }
+            to[u] = mover ? holes[rm + __popc(bits & below)] : -1;
+            x[u] = mover ? ptx::ld_act(w + i) : 0.0f;
             rm += __popc(bits);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 32 * u;
+            if (to[u] >= 0) {
+                kept[to[u]] = i;
+                wo[to[u]] = x[u];
+            }
             if (i >= size && i < w1) wo[i] = 0.0f;
-        });
+        }
+    }
 }
 
 constexpr int kMoveWarps = 8;
@@ -346,11 +376,13 @@ int launch_select(EvictArgs& a, const DeviceCtx* c, cudaStream_t s) {
     int ranks = 1;
     while (ranks < kRanks && (int64_t)a.c.n_head_kv * a.c.batch * 2 * ranks <= c->sm_count && a.c.cap > ranks * kShare) ranks *= 2;
     a.held = std::min(kHeldSlots, ((a.c.cap + ranks - 1) / ranks + 31) / 32 * 32);
-    const size_t smem = (size_t)a.held * 4;
+    a.held_holes = ranks == 1 ? std::min(kHeldHoles, a.budget) : 0;
+    const size_t smem = (size_t)a.held * 4 + a.held / 8 + (size_t)a.held_holes * 4;
     static bool set[64] = {};
     const int dev = c->device < 64 ? c->device : 63;
     if (!set[dev] || c->device >= 64) {
-        MLZC_CUDA_TRY(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldSlots * 4));
+        MLZC_CUDA_TRY(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kHeldSlots * 4 + kHeldSlots / 8 + kHeldHoles * 4));
         set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
