@@ -148,10 +148,19 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     const size_t head = (size_t)b * a.c.n_head_kv + h;
     uint32_t* words = hold ? held + a.held : a.words + head * a.n_words + (s0 >> 5);
     int* holes = ranks == 1 && a.budget <= a.held_holes ? reinterpret_cast<int*>(held + a.held + a.held / 32) : a.holes + head * a.budget;
-    auto key_of = [&](int i) { return i < lo || i >= hi ? kForced : order_key(ptx::ld_act(w + i)); };
+    auto key_of = [&](int i) {
+        const uint32_t k = order_key(ptx::ld_act(w + i));
+        return i < lo || i >= hi ? kForced : k;
+    };
     if (hold) {
-#pragma unroll 4
-        for (int i = w0 + lane; i < w1; i += 32) held[i - s0] = key_of(i);   // read by the same lane alone
+        for (int i = w0 + lane; i < w1; i += 128) {    // read by the same lane alone
+            uint32_t k[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) k[u] = key_of(min(i + 32 * u, w1 - 1));
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + 32 * u < w1) held[i + 32 * u - s0] = k[u];
+        }
     }
     // f(slot, key) for this lane's slots; every lane of the warp comes along (slots at or past w1
     // are none of its)
