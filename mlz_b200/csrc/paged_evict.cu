@@ -12,10 +12,11 @@
 //           and every target before it, so rows move in place, in any order, and only those
 //           that have to (order-keeping compaction would move nearly all of them).
 // The move is bound by HBM: 16 sequences of 512 to 8192 slots x 8 heads x 128 dims cut to 1000 take
-// 16 us for 90 MB.  The selection is bound by latency, by passes that depend on one another and
-// cost a dozen instructions a slot on the one SM that has the head: 20 us for 8192 slots.  Where
-// heads are few, a cluster of up to 8 CTAs shares one, its histograms and counts read over
-// distributed shared memory: 24 us for 32768 slots (41 with one CTA), 33 for 131072.
+// 15 us for 90 MB.  The selection is bound by latency, by passes that depend on one another and
+// cost some twenty instructions a slot and pass on the one SM that has the head: 15 us for 8192
+// slots (20 before its keys, bits and holes lay in shared memory).  Where heads are few, a cluster
+// of up to 8 CTAs shares one, its counts read over distributed shared memory: 18 us for 32768
+// slots (41 with one CTA).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     // every 32nd slot, so that loads and stores are whole lines and a slot's rank is a count of
     // ballot bits.  Short loops on purpose: each phase runs once a launch, and with 16 slots a
     // lane unrolled the selection of 8 heads of 32768 slots took 35 us.
-    const int lane = tid & 31, warp = tid >> 5, log_ranks = 31 - __clz(ranks);
+    const int lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0), log_ranks = 31 - __clz(ranks);
     const int share = (((n + ranks - 1) >> log_ranks) + 31) & ~31, s0 = min(n, rank * share), s1 = min(n, s0 + share);
     const int run = (share / kSelWarps + 31) & ~31, w0 = min(s1, s0 + warp * run), w1 = min(s1, w0 + run);
     const bool hold = share <= a.held;
