@@ -22,6 +22,9 @@
 // the exponential unit idled half of the time: 205 us for 2048 tokens of 8192).  f32 queries come
 // as f16 hi + lo from a small preparing launch, low products summed first.
 //
+// Measured (device times): 2048 tokens of 8192 slots, 8 heads of 4, 128 dims: f16 175 us, f32 239 (twice
+// the products); decode of 16 sequences of 512 to 8192: 39 us (152 MB), of one of 32768: 18 us.
+//
 // lse2 is rounded to f32 once a row (4e-7 of a weight at lse 10).  Carrying what that drops as a
 // factor a column made no weight better (the products' own sums are as far off) and cost 12 %.
 //
