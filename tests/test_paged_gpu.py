@@ -315,6 +315,25 @@ def test_evict_sizes(dev, n, budget, sink, recent):
     _check_evict(c, _weights_of(c, "spread", n), budget, sink, recent)
 
 
+@pytest.mark.parametrize("hkv,n,budget", [
+    (75, 33000, 500),      # a CTA a head, keys past its shared memory
+    (75, 9500, 9000),      # a CTA a head, holes past its shared memory
+    (2, 300000, 3000)])    # a cluster a head, keys past its CTAs' shared memory
+def test_evict_long_heads(dev, hkv, n, budget):
+    c = ref.make(dev, [0], [n], hkv=hkv, D=64, page=128, seed=n)
+    w = _weights_of(c, "spread", n)
+    k0 = c.k.clone()
+    kept, wout = ref.evict(c, w, budget, 4, 64)
+    got, gw, gl = mlz_b200.paged_evict(ref.handle(c), w, budget, n_sink=4, n_recent=64, kv_len_out=c.lens.clone())
+    assert gl.tolist() == [budget]
+    assert torch.equal(got.cpu(), torch.tensor(kept, dtype=torch.int32).view(1, hkv, budget))
+    assert torch.equal(gw[0, :, :n].cpu(), torch.tensor(wout).view(hkv, n))
+    fr, to = got[0].long(), torch.arange(budget, device=dev)
+    page = lambda x: c.table[0].long()[x // c.page]  # noqa: E731
+    h = torch.arange(hkv, device=dev)[:, None]
+    assert torch.equal(c.k[page(to), h, to % c.page], k0[page(fr), h, fr % c.page])
+
+
 def test_evict_into_other_weights_and_layout(dev):
     c = ref.make(dev, [0, 0], [500, 900], hkv=2, page=16, layout="phd", seed=15)
     w = _weights_of(c, "ties")
@@ -509,3 +528,48 @@ def test_calls_on_a_side_stream_and_captured(dev):
     w_out, _, e_out, _ = ref.attn(c)
     for o in outs:
         _within(o, w_out, e_out, "replayed")
+
+
+def test_attn_without_tokens(dev):
+    c = ref.make(dev, [0, 0], [40, 9], seed=43)
+    out, lse = mlz_b200.paged_attn(ref.handle(c), c.q[:0], c.scale, return_lse=True)
+    assert out.shape == (0,) + c.q.shape[1:] and lse.shape[0] == 0
+
+
+def test_two_streams_at_once(dev):
+    """Attention, weights and eviction of two caches on two streams, again and again with nothing
+    between them: the same bits as one after the other."""
+    cs = [ref.make(dev, [1, 90, 3], [900, 300, 2000], hkv=2, page=16, dtype=t, seed=51 + i) for i, t in enumerate((F32, F16))]
+    streams = [torch.cuda.Stream() for _ in cs]
+
+    def step(c, stream):
+        h = ref.handle(c)
+        out, lse = mlz_b200.paged_attn(h, c.q, c.scale, return_lse=True, stream=stream)
+        w = mlz_b200.paged_weights(h, c.q, lse, c.scale, stream=stream)
+        kept, wo, _ = mlz_b200.paged_evict(h, w, 500, n_sink=2, n_recent=9, weights_out=acc[id(c)], kv_len_out=spare[id(c)], stream=stream)
+        return out[:c.T], lse[:c.T], w, kept
+
+    acc = {id(c): torch.zeros((3, 2, c.cap), device=dev) for c in cs}
+    spare = {id(c): c.lens.clone() for c in cs}
+    pools = [(c.k.clone(), c.v.clone()) for c in cs]
+
+    def restore(c, p):
+        c.k.copy_(p[0])
+        c.v.copy_(p[1])
+
+    want = []
+    for c, p in zip(cs, pools):
+        want.append(step(c, None))
+        torch.cuda.synchronize()
+        restore(c, p)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for c, p, st in zip(cs, pools, streams):
+            got.append(step(c, st))
+            with torch.cuda.stream(st):
+                restore(c, p)
+        for st in streams:
+            st.synchronize()
+        for g, x in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, x))
