@@ -80,7 +80,7 @@ constexpr float kRescale = 8.0f;
 
 struct AttnArgs {
     View c;
-    CUtensorMap mk, mv, mq;
+    CUtensorMap mk, mv, mq, mkp, mvp;   // pools in boxes of `box` rows, of a page (where `whole`)
     const char* q;
     char* dst;
     char* lse;
@@ -88,6 +88,7 @@ struct AttnArgs {
     int G, tq;                 // query heads a KV head; tokens a tile (tq * G <= 128)
     paged::Div by_g;
     int box;                   // rows of a K / V box
+    int whole;                 // pages that lie whole in a tile come as one box
     float scale, softcap;      // softcap 0: none
     int n_ctas, rec_rows;
     float* rec;                // [cta][2][rec_rows][D]: 0 continues a cut tile, 1 begins one
@@ -749,9 +750,15 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t r
         const int j = i * BN + lane * a.box;
         return lane < boxes && lane * a.box < tile_rows(a, w, i) ? paged::load_page(a.c, w.b, a.c.by_page.quot(j)) : -1;
     };
-    auto load = [&](const Walk<C>& w, int i, int page, const CUtensorMap* map) {
+    auto load = [&](const Walk<C>& w, int i, int page, const CUtensorMap* map, const CUtensorMap* map_whole) {
         const int n = (tile_rows(a, w, i) + a.box - 1) / a.box;
         const int row = a.c.by_page.rem(i * BN + lane * a.box);
+        // a page whose rows all lie in the tile: its first box's lane fetches them
+        const int start = lane * a.box - row;
+        const bool inside = a.whole && start >= 0 && start + a.c.page <= BN, first = inside && row == 0;
+        const bool copies = lane < n && (first || !inside);
+        const int rows = __popc(__ballot_sync(~0u, copies && first)) * a.c.page + __popc(__ballot_sync(~0u, copies && !first)) * a.box;
+        if (first) map = map_whole;
         // a page outside the pools is a coordinate outside the map, which reads as zeros
         const int pg = page < 0 ? a.c.n_pages : page;
 #pragma unroll
@@ -760,11 +767,11 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t r
             if (!mbar_wait(smem_u32(&B->empty[st]), ((at / C::ST) & 1) ^ 1, abort, a.c.err)) return false;
             const uint32_t bar = smem_u32(&B->full[st]);
             if (lane == 0) {
-                if (n) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
+                if (n) mbar_expect_tx(bar, (uint32_t)rows * 128 * C::SUBS);
                 else mbar_arrive(bar);
             }
             __syncwarp();
-            if (lane < n) {
+            if (copies) {
 #pragma unroll
                 for (int u = 0; u < C::SUBS; ++u)
                     tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, map, bar, (unit * C::SUBS + u) * 64, row, w.h, pg);
@@ -775,15 +782,15 @@ __device__ __forceinline__ void load_role(const AttnArgs& a, Bars* B, uint32_t r
     Walk<C> w(B);
     while (ok && w.next(a)) {
         int cur = page_of(w, w.tile), nxt = -1;
-        ok = load(w, w.tile, cur, &a.mk);
+        ok = load(w, w.tile, cur, &a.mk, &a.mkp);
         for (int it = 0; ok && it < w.n; ++it) {
             const int i = w.tile + it;
             const bool more = it + 1 < w.n;
             if (more) nxt = page_of(w, i + 1);
             // the order in which the MMA warp takes them
-            if (C::NS == 1 && more) ok = load(w, i + 1, nxt, &a.mk);
-            if (ok) ok = load(w, i, cur, &a.mv);
-            if (C::NS == 2 && more && ok) ok = load(w, i + 1, nxt, &a.mk);
+            if (C::NS == 1 && more) ok = load(w, i + 1, nxt, &a.mk, &a.mkp);
+            if (ok) ok = load(w, i, cur, &a.mv, &a.mvp);
+            if (C::NS == 2 && more && ok) ok = load(w, i + 1, nxt, &a.mk, &a.mkp);
             cur = nxt;
         }
     }
@@ -1299,6 +1306,10 @@ extern "C" int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_pag
     a.box = std::gcd(cache->page_size, BN);
     if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
     if ((st = paged::encode_pool(&a.mv, cache, true, a.box)) != MLZC_OK) return st;
+    // a page of 24 rows is three boxes of 8 where a tile cuts it, one of 24 elsewhere
+    a.whole = cache->page_size < BN && a.box < cache->page_size;
+    if (a.whole && (st = paged::encode_pool(&a.mkp, cache, false, cache->page_size)) != MLZC_OK) return st;
+    if (a.whole && (st = paged::encode_pool(&a.mvp, cache, true, cache->page_size)) != MLZC_OK) return st;
     if (!f32 && (st = paged::encode_rows(&a.mq, d->q, cache->head_dim, d->n_head_q, cache->n_tokens, d->q_nb[1], d->q_nb[2],
                                          a.G, a.tq)) != MLZC_OK)
         return st;
