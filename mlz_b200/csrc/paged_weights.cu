@@ -66,12 +66,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct WeightArgs {
     View c;
-    CUtensorMap mk, mq, mql;           // K pool; q rows (hi), lo
+    CUtensorMap mk, mkp, mq, mql;      // K pool in boxes of `box` rows, of a page (where `whole`); q rows (hi), lo
     const char* lse;
     const char* acc;
     char* out;
     size_t lse_head, lse_tok, a_head, a_seq, o_head, o_seq;
-    int G, tq, box, n_ctas;
+    int G, tq, box, whole, n_ctas;
     paged::Div by_tq, by_g;
     float scale, softcap;
     float* rec;                        // [cta][2][128]: 0 continues a cut slot tile, 1 begins one
@@ -362,18 +362,24 @@ __device__ __forceinline__ void load_role(const WeightArgs& a, Bars* B, uint32_t
     auto load_k = [&](const Walk& w, int t, int page, uint32_t& taken) {
         const int n = (min(kBN, w.s.kv - t * kBN) + a.box - 1) / a.box;
         const int row = a.c.by_page.rem(t * kBN + lane * a.box);
+        // a page whose rows all lie in the tile: its first box's lane fetches them
+        const int start = lane * a.box - row;
+        const bool inside = a.whole && start >= 0 && start + a.c.page <= kBN, first = inside && row == 0;
+        const bool copies = lane < n && (first || !inside);
+        const int rows = __popc(__ballot_sync(~0u, copies && first)) * a.c.page + __popc(__ballot_sync(~0u, copies && !first)) * a.box;
+        const CUtensorMap* map = first ? &a.mkp : &a.mk;
         const int pg = page < 0 ? a.c.n_pages : page;   // outside the map: zeros
 #pragma unroll
         for (int unit = 0; unit < C::UN; ++unit) {
             uint32_t st;
             if (!slot(st)) return false;
             const uint32_t bar = MLZC_BAR(full, st);
-            if (lane == 0) mbar_expect_tx(bar, (uint32_t)n * a.box * 128 * C::SUBS);
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)rows * 128 * C::SUBS);
             __syncwarp();
-            if (lane < n) {
+            if (copies) {
 #pragma unroll
                 for (int u = 0; u < C::SUBS; ++u)
-                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, &a.mk, bar, (unit * C::SUBS + u) * 64, row, w.h, pg);
+                    tma_load_4d(ring + st * C::kUnit + u * C::kSub + lane * a.box * 128, map, bar, (unit * C::SUBS + u) * 64, row, w.h, pg);
             }
             taken |= 1u << st;
         }
@@ -770,6 +776,8 @@ extern "C" int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_
     a.by_g.set((uint32_t)a.G);
     a.box = std::gcd(cache->page_size, kBN);
     if ((st = paged::encode_pool(&a.mk, cache, false, a.box)) != MLZC_OK) return st;
+    a.whole = cache->page_size < kBN && a.box < cache->page_size;
+    if (a.whole && (st = paged::encode_pool(&a.mkp, cache, false, cache->page_size)) != MLZC_OK) return st;
     if (T > 0) {
         // checked after every argument: from here on work is issued
         if (f32) {
