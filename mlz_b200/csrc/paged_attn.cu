@@ -10,8 +10,9 @@
 //
 // A CTA walks BN-slot tiles of K and V:
 //   loader warp    K and V tiles by TMA into a ring, one box per page piece (box height
-//                  gcd(page, BN), so a box never crosses a page); each lane looks up its own
-//                  box's page in the block table and issues its own copies;
+//                  gcd(page, BN), so a box never crosses a page, or the page where it lies whole in
+//                  the tile: 24 mixed sequences with pages of 24 rows 75 us, 88 without); each lane
+//                  looks up its own box's page in the block table and issues its own copies;
 //   Q warp         the next piece's Q tile (f16: TMA; f32: split into f16 hi + lo);
 //   MMA warp       S = Q K^T (operands in shared memory) and O += P V (P in TMEM, V as an
 //                  N-contiguous B operand) with tcgen05.mma, accumulators in TMEM;
@@ -164,7 +165,8 @@ __device__ __forceinline__ int tiles_of(const Seq& s, int t, int tokens) {
 
 // What a query tile costs beside its slot tiles (its Q, filling and draining the pipeline), in slot
 // tiles.  The list counts it in front of the tiles, so that CTAs with many short query tiles get
-// fewer slot tiles (24 mixed sequences, 64 dims f32: 127 us with 0, 90 with 2 to 4, 101 with 8).
+// fewer slot tiles (24 mixed sequences, 64 dims f32, before later steps: 127 us with 0, 90 with 2 to
+// 4, 101 with 8).
 constexpr int kStart = 3;
 
 // A walk over this CTA's share: piece after piece (the tiles of one query tile).
