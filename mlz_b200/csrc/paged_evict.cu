@@ -11,8 +11,9 @@
 //   move:   rows of K and V from movers to holes.  Every source lies at or behind the budget
 //           and every target before it, so rows move in place, in any order, and only those
 //           that have to (order-keeping compaction would move nearly all of them).
-// The move is bound by HBM: 16 sequences of 512 to 8192 slots x 8 heads x 128 dims cut to 1000 take
-// 15 us for 90 MB.  The selection is bound by latency, by passes that depend on one another and
+// Measured: 16 sequences of 512 to 8192 slots x 8 heads x 128 dims cut to 1000 take 29.6 us, half of it
+// the move of 43 MB (and as much back, most of it to L2), bound by HBM and its own three dependent
+// loads.  The selection is bound by latency, by passes that depend on one another and
 // cost some twenty instructions a slot and pass on the one SM that has the head: 15 us for 8192
 // slots (20 before its keys, bits and holes lay in shared memory).  Where heads are few, a cluster
 // of up to 8 CTAs shares one, its counts read over distributed shared memory: 18 us for 32768
@@ -313,7 +314,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
 }
 
 constexpr int kMoveWarps = 8;
-constexpr int kMoveSlots = kMoveWarps * 32;
+// Slots a warp looks after: with 32 a warp's rows come in four dependent steps (16 sequences to 1000
+// 30.5 us for 29.6, 32768 slots 24.0 for 22.6), with 8 large batches pay for the blocks' starts (64
+// sequences of 2000 to 4000 to 1500: 104 us for 92).
+constexpr int kWarpSlots = 16;
+constexpr int kMoveSlots = kMoveWarps * kWarpSlots;
 
 template <int D>
 __global__ void __launch_bounds__(kMoveWarps * 32) move_kernel(const __grid_constant__ EvictArgs a) {
@@ -327,9 +332,9 @@ __global__ void __launch_bounds__(kMoveWarps * 32) move_kernel(const __grid_cons
         const int kv = paged::ld_int(c.kv_len + b);
         a.kv_len_out[b] = min(min(max(kv, 0), c.cap), a.budget);
     }
-    const int slot = blockIdx.x * kMoveSlots + warp * 32 + lane;
+    const int slot = blockIdx.x * kMoveSlots + warp * kWarpSlots + lane;
     const int* kept = reinterpret_cast<const int*>(a.kept + (size_t)b * a.kept_seq + (size_t)h * a.kept_head);
-    const int from = slot < a.budget ? paged::ld_int(kept + slot) : -1;
+    const int from = lane < kWarpSlots && slot < a.budget ? paged::ld_int(kept + slot) : -1;
     const bool moves = from >= 0 && from != slot;
     int pf = -1, pt = -1;
     if (moves) {
