@@ -55,6 +55,7 @@
 #include <type_traits>
 
 #include "paged.h"
+#include "paged_records.h"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
 
@@ -92,7 +93,7 @@ struct AttnArgs {
     int whole;                 // pages that lie whole in a tile come as one box
     float scale, softcap;      // softcap 0: none
     int n_ctas, rec_rows;
-    float* rec;                // [cta][2][rec_rows][D]: 0 continues a cut tile, 1 begins one
+    float* rec;                // [cta][2][rec_rows][D]: 0 continues a cut tile, 1 begins one (paged_records.h)
     float2* ml;                // [cta][2][rec_rows]: exponent of the record's scale, sum
     int4* head;                // [cta]: of the query tile begun in record 1, packed row, tokens, kv head, last CTA (-1: none)
 };
@@ -311,7 +312,7 @@ struct Sink {
         whole = w.tile == 0 && w.ends();
         t = w.s.row0 + q.tok(a, w, slot);
         h = w.h * a.G + q.head_of;
-        r = ((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * a.rec_rows + slot * 128 + q.row;
+        r = ((size_t)blockIdx.x * 2 + (w.tile == 0 ? 1 : 0)) * a.rec_rows + paged::record_row(slot, q.row, a.tq, a.G);
     }
     // the row's sum: of 2^(...) = 2^e2 * l
     __device__ void sums(const AttnArgs& a, float e2, float l) const {
@@ -1184,8 +1185,8 @@ __global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_con
     const int row0 = (int)hd.x, tokens = (int)hd.y, h = (int)hd.z, last = (int)hd.w;
     if (last < 0) return;
     const int row = blockIdx.y * kMergeRows + (threadIdx.x >> 5);
-    const int in = row % 128, tok = row / 128 * a.tq + a.by_g.quot(in);
-    if (row >= a.rec_rows || in >= a.tq * a.G || tok >= tokens) return;
+    const int tok = a.by_g.quot(row);
+    if (row >= a.rec_rows || tok >= tokens) return;
     auto rec = [&](int i) { return ((size_t)i * 2 + (i == c ? 1 : 0)) * a.rec_rows + row; };
     // four records at a time, their loads under way together
     float top = -INFINITY, l = 0.0f, acc[D / 32] = {};
@@ -1222,7 +1223,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) merge_kernel(const __grid_con
             }
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int q = row0 + tok, head = h * a.G + a.by_g.rem(in);
+    const int q = row0 + tok, head = h * a.G + a.by_g.rem(row);
     char* dst = a.dst + (size_t)q * a.d_tok + (size_t)head * a.d_head;
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) {
@@ -1246,7 +1247,7 @@ Plan make_plan(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* d, int
     const int64_t G = d->n_head_q / cache->n_head_kv, rows = cache->n_tokens * G;
     // two query tiles a CTA when the sequences fill more than one on average
     p.ns = d->type == MLZC_TYPE_F16 && cache->head_dim < 256 && rows > 128 * cache->batch_size ? 2 : 1;
-    p.rec_rows = (int)std::min<int64_t>(128 * p.ns, (rows + 3) / 4 * 4);
+    p.rec_rows = paged::record_rows(cache->n_tokens, (int)G, 128 / (int)G, p.ns);
     p.rec = (size_t)ctas * 2 * p.rec_rows * cache->head_dim * 4;
     p.ml = (size_t)ctas * 2 * p.rec_rows * 8;
     p.total = p.rec + p.ml + (size_t)ctas * 16;
