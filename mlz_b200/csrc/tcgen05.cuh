@@ -218,10 +218,28 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& r0, float& r1) {
     r1 = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
-// N scores to cap * tanh(s * in), in = scale / cap.  Where no lane of the warp has |s * in| above 1,
-// by the odd minimax polynomial of tanh there (degree 13, Remez; 1.7e-7 relative with f32 rounding)
-// on the FMA pipe; else cap (1 - e) / (1 + e), e = exp(-2 |s in|), whose two more uses of the
-// exponential unit a score would be the bound.
+// cap * tanh(t) for |t| <= 1: the odd minimax polynomial of tanh there (degree 13, Remez; 1.7e-7
+// relative with f32 rounding).
+__device__ __forceinline__ float cap_near(float t, float cap) {
+    const float q = t * t;
+    float p = fmaf(0.0010582648683339357f, q, -0.006259339861571789f);
+    p = fmaf(p, q, 0.020359760150313377f);
+    p = fmaf(p, q, -0.053498707711696625f);
+    p = fmaf(p, q, 0.13326409459114075f);
+    p = fmaf(p, q, -0.33332985639572144f);
+    p = fmaf(p, q, 1.0f);
+    return t * cap * p;
+}
+// cap * tanh(t) for |t| > 1: cap (1 - e) / (1 + e), e = exp(-2 |t|) < 0.14, so that 1 - e loses nothing.
+__device__ __forceinline__ float cap_far(float t, float cap) {
+    const float e = ex2(fabsf(t) * (-2.0f * 1.4426950408889634f));
+    return copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, t);
+}
+
+// N scores to cap * tanh(s * in), in = scale / cap, each by the form for its own size: a score's
+// bits depend on nothing beside it.  The far form's two more uses of the exponential unit a score
+// would be the bound, so a warp passes it over where none of its lanes has a score for it (lanes
+// and columns that do not count may decide that: it changes the time alone).
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&x)[N], float in, float cap) {
     float top = 0.0f;
@@ -231,23 +249,10 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], float in, float cap) {
     for (int j = 0; j < N; j += 2) top = max3(top, fabsf(x[j]), fabsf(x[j + 1]));
     if (__all_sync(~0u, top <= 1.0f)) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float t = x[j], q = t * t;
-            float p = fmaf(0.0010582648683339357f, q, -0.006259339861571789f);
-            p = fmaf(p, q, 0.020359760150313377f);
-            p = fmaf(p, q, -0.053498707711696625f);
-            p = fmaf(p, q, 0.13326409459114075f);
-            p = fmaf(p, q, -0.33332985639572144f);
-            p = fmaf(p, q, 1.0f);
-            x[j] = t * cap * p;
-        }
+        for (int j = 0; j < N; ++j) x[j] = cap_near(x[j], cap);
     } else {
-        const float k = -2.0f * 1.4426950408889634f;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const float e = ex2(fabsf(x[j]) * k);
-            x[j] = copysignf(__fdividef(1.0f - e, 1.0f + e) * cap, x[j]);
-        }
+        for (int j = 0; j < N; ++j) x[j] = fabsf(x[j]) <= 1.0f ? cap_near(x[j], cap) : cap_far(x[j], cap);
     }
 }
 

@@ -1,8 +1,11 @@
 """GPU: calls of the paged KV cache at the edges of what its contract allows, against the plain
 64-bit forms."""
+import math
+
 import pytest
 import torch
 
+import mlz_b200
 from tests import paged_ref as ref
 from tests.test_paged_gpu import _check_attn
 
@@ -21,3 +24,77 @@ def test_attn_one_sequence_with_groups_that_do_not_divide_a_tile(dev, group, tok
     out to many CTAs: every row of both tiles comes back from the records."""
     for T in tokens:
         _check_attn(ref.make(dev, [T], [T + behind], hkv=2, group=group, D=D, page=64, dtype=F16, seed=T))
+
+
+# ------------------------------------------------------------------ capped scores
+
+def _unused_rows(c):
+    """Rows of the pools that lie past every sequence's length."""
+    u = torch.ones((c.k.shape[0], c.page), dtype=torch.bool)
+    table = c.table.cpu()
+    for b, n in enumerate(c.kv_len):
+        for j in range(n):
+            u[table[b, j // c.page], j % c.page] = False
+    return u[:, None, :, None].expand_as(c.k).to(c.k.device)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 9.0])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_len,kv_len", [([5, 1], [100, 333]), ([1, 1, 1], [40, 200, 1001]), ([200], [500])])
+def test_what_does_not_count_changes_no_bit(dev, q_len, kv_len, D, dtype, softcap):
+    """Attention and weights with other contents of the pages' unused rows, of the rows behind the
+    last sequence and, left by other calls, of shared and tensor memory."""
+    c = ref.make(dev, q_len, kv_len, D=D, dtype=dtype, seed=7, tail=5, junk=False)
+    unused, cache, first = _unused_rows(c), ref.handle(c), None
+    for junk in (0.0, 3.0e4, -7.0, math.nan):
+        c.k[unused] = c.v[unused] = junk
+        c.q[c.T:] = junk
+        o = ref.make(dev, [130, 64], [700, 400], D=D, dtype=dtype, seed=3, q_scale=0.1 if junk == 0 else 300.0)
+        other = ref.handle(o)
+        _, lse = mlz_b200.paged_attn(other, o.q, o.scale, return_lse=True)
+        mlz_b200.paged_weights(other, o.q, lse, o.scale)
+        out, lse = mlz_b200.paged_attn(cache, c.q, c.scale, softcap=softcap, return_lse=True)
+        w = mlz_b200.paged_weights(cache, c.q, lse, c.scale, softcap=softcap)
+        got = out[:c.T].clone(), lse[:c.T].clone(), w
+        first = first or got
+        for a, b, what in zip(first, got, ("out", "lse", "weights")):
+            assert torch.equal(a, b), f"{what} with {junk} in what does not count"
+
+
+@pytest.mark.parametrize("cap", [50.0, 1000.0, 2.0 ** 14])
+@pytest.mark.parametrize("q_len,kv_len", [([4], [40]), ([1, 1], [300, 77]), ([150], [150])])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_small_capped_scores_beside_large_ones(dev, D, q_len, kv_len, cap):
+    """f32: one head's scores reach past the cap, the others' stay below 1.  q and k have one dim,
+    so the products are exact and the bound is that of the capping alone."""
+    c = ref.make(dev, q_len, kv_len, hkv=1, group=4, D=D, seed=1, junk=False)
+    g = torch.Generator(device=dev).manual_seed(5)
+    c.q.zero_()
+    c.k.zero_()
+    c.q[:, :, 3] = torch.rand(c.q.shape[:2], generator=g, device=dev) - 0.5
+    c.q[::2, 1, 3] = 3 * cap
+    c.k[..., 3] = (torch.rand(c.k.shape[:3], generator=g, device=dev) * 2 - 1).half()
+    c.scale = 1.1
+    cache = ref.handle(c)
+    _, lse = mlz_b200.paged_attn(cache, c.q, c.scale, softcap=cap, return_lse=True)
+    _, want, _, _ = ref.attn(c, cap)
+    # q as hi + lo (2^-22), scale / cap and its product with the score (2^-24 each), tanh (1.7e-7),
+    # two products with the cap's (2^-24 each): below 2^-20 of a score, which is below 1 in heads 0, 2 and 3
+    # and below cap in head 1; then the exponentials (2^-22) and their sum, in f32, and the lse from the
+    # maximum less an offset of 6 and the logarithm of a sum below 2^20, each rounded twice
+    n = max(kv_len)
+    for h in range(4):
+        most = cap if h == 1 else 1.0
+        bound = 2.0 ** -20 * most + (8 + n ** 0.5) * 2.0 ** -24 + 4 * 2.0 ** -24 * (most + 6 + 20)
+        worst = float((lse[:, h].double() - want[:, h]).abs().max())
+        assert worst <= bound, f"head {h}: lse off by {worst:.2e}, bound {bound:.2e}"
+    # weights of the small heads with lse = 0: exp(score), its relative error that of the score, of the
+    # exponential and of the sums of T x 4 terms
+    zero = torch.zeros_like(lse)
+    zero[:, 1] = -math.inf
+    got = mlz_b200.paged_weights(cache, c.q, zero, c.scale, softcap=cap)
+    want, _ = ref.weights(c, zero, cap)
+    real = ~torch.isnan(want)
+    bound = 2.0 ** -20 + 2.0 ** -22 + (8 + (4 * c.T) ** 0.5) * 2.0 ** -24
+    assert float(((got.double() - want) / want)[real].abs().max()) <= bound
