@@ -27,10 +27,10 @@ __all__ = [
     "last_error", "launch_count", "lib", "Comm", "Weight", "device_errors", "flash_attn_dispatch", "flash_attn_dispatch_quant",
     "flash_attn_workspace_bytes", "ggml_simd_try_flash_attn", "ggml_simd_try_mul_mat", "init",
     "make_fa_desc", "mul_mat", "mul_mat_workspace_bytes", "quantize_q8k", "selftest_wait_timeout", "shutdown", "tensor_view",
-    "weight_type_of", "PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store",
-    "paged_weights", "DEVERR_BAD_INDEX", "ROPE_ADJACENT", "ROPE_HALVES",
+    "weight_type_of", "DEVERR_BAD_INDEX", "ROPE_ADJACENT", "ROPE_HALVES",
 ]
 
+# Not in __all__: a star import would load them, and torch with them.
 _PAGED = ("PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store", "paged_weights")
 
 
@@ -41,3 +41,7 @@ def __getattr__(name):
     from . import paged
     globals().update({n: getattr(paged, n) for n in _PAGED})
     return globals()[name]
+
+
+def __dir__():
+    return sorted({*globals(), *_PAGED})
