@@ -31,7 +31,8 @@ __all__ = [
 ]
 
 # Not in __all__: a star import would load them, and torch with them.
-_PAGED = ("PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_store", "paged_weights")
+_PAGED = ("PagedCache", "paged_attn", "paged_attn_workspace_bytes", "paged_evict", "paged_evict_workspace_bytes", "paged_store",
+          "paged_weights", "paged_weights_workspace_bytes")
 
 
 def __getattr__(name):

@@ -272,6 +272,15 @@ def paged_attn(cache, q, scale, *, softcap=0.0, out=None, lse=None, return_lse=F
     return (out, lse) if lse is not None else out
 
 
+def paged_weights_workspace_bytes(cache, q, scale=1.0, *, softcap=0.0):
+    """Bytes of workspace that :func:`paged_weights` needs for these tensors."""
+    L = _Launch(cache.device, None)
+    d = _attn_desc(cache, q, scale, softcap)
+    d.lse, d.lse_nb[:] = q.data_ptr(), (4, 4 * q.shape[1])   # any lse: its place does not change the size
+    return cache._workspace(L, lib().mlzc_paged_weights_workspace_bytes, ("weights", q.shape[0], q.shape[1], q.dtype),
+                            C.byref(cache._with(q.shape[0])), C.byref(d))
+
+
 def paged_weights(cache, q, lse, scale, *, softcap=0.0, acc=None, out=None, workspace=None, stream=None):
     """Attention weight that each slot received from the new tokens, summed over them and the
     query heads of each kv head, added to acc (batch, n_head_kv, capacity) float32 (None: from
@@ -295,6 +304,14 @@ def paged_weights(cache, q, lse, scale, *, softcap=0.0, acc=None, out=None, work
     ws, n, owner = _given(workspace, need, L, q)
     L.run(lib().mlzc_paged_weights_dev, cd, d, acc.data_ptr() if acc is not None else None, anb, out.data_ptr(), onb, ws, n, L.handle)
     return out
+
+
+def paged_evict_workspace_bytes(cache, budget):
+    """Bytes of workspace that :func:`paged_evict` needs for this cache and budget."""
+    d = PagedEvictDesc()
+    d.budget = budget
+    return cache._workspace(_Launch(cache.device, None), lib().mlzc_paged_evict_workspace_bytes, ("evict", budget),
+                            C.byref(cache._desc), C.byref(d))
 
 
 def paged_evict(cache, weights, budget, *, n_sink=0, n_recent=0, weights_out=None, kept=None, kv_len_out=None,
@@ -324,4 +341,5 @@ def paged_evict(cache, weights, budget, *, n_sink=0, n_recent=0, weights_out=Non
     return kept, weights_out, kv_len_out
 
 
-__all__ = ["PagedCache", "paged_store", "paged_attn", "paged_attn_workspace_bytes", "paged_weights", "paged_evict"]
+__all__ = ["PagedCache", "paged_store", "paged_attn", "paged_attn_workspace_bytes", "paged_weights",
+           "paged_weights_workspace_bytes", "paged_evict", "paged_evict_workspace_bytes"]

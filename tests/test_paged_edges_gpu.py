@@ -98,3 +98,33 @@ def test_small_capped_scores_beside_large_ones(dev, D, q_len, kv_len, cap):
     real = ~torch.isnan(want)
     bound = 2.0 ** -20 + 2.0 ** -22 + (8 + (4 * c.T) ** 0.5) * 2.0 ** -24
     assert float(((got.double() - want) / want)[real].abs().max()) <= bound
+
+
+# ------------------------------------------------------------------ workspaces
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("q_len", [[1, 1], [150, 1], [0, 0]])
+def test_workspaces_of_the_stated_sizes(dev, q_len, dtype):
+    """The stated sizes are enough and needed, asked for before the first call or after it."""
+    for before in (True, False):
+        c = ref.make(dev, q_len, [400, 90], hkv=3, dtype=dtype, seed=61)
+        cache, q = ref.handle(c), c.q[:c.T]
+        if not before:
+            _, lse = mlz_b200.paged_attn(cache, q, c.scale, return_lse=True)
+            w = mlz_b200.paged_weights(cache, q, lse, c.scale)
+            mlz_b200.paged_evict(cache, w, 100, kv_len_out=c.lens.clone())
+        sizes = (mlz_b200.paged_attn_workspace_bytes(cache, q), mlz_b200.paged_weights_workspace_bytes(cache, q),
+                 mlz_b200.paged_evict_workspace_bytes(cache, 100))
+        assert (sizes[0] > 0) == (c.T > 0) and sizes[1] > 0 and sizes[2] > 0
+        room = [torch.empty(max(16, n), dtype=torch.uint8, device=dev) for n in sizes]
+        attn = lambda ws: mlz_b200.paged_attn(cache, q, c.scale, return_lse=True, workspace=ws)  # noqa: E731
+        _, lse = attn(room[0])
+        weigh = lambda ws: mlz_b200.paged_weights(cache, q, lse, c.scale, workspace=ws)  # noqa: E731
+        w = weigh(room[1])
+        evict = lambda ws: mlz_b200.paged_evict(cache, w.clone(), 100, kv_len_out=c.lens.clone(), workspace=ws)  # noqa: E731
+        evict(room[2])
+        torch.cuda.synchronize()
+        for call, ws, n in zip((attn, weigh, evict), room, sizes):
+            if n:
+                with pytest.raises(mlz_b200.MlzcError, match="workspace"):
+                    call(ws[:n - 1])
