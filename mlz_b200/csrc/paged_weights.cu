@@ -225,11 +225,6 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
     const float cap_in = C::CAP ? a.scale / a.softcap : 0.0f;
     const uint32_t bars = smem_u32(B);
     volatile int* abort = &B->abort;
-    // weights of columns i, i + 1 where they count: outside [from, cols) a score may hold anything
-    auto some = [&](const float* x, const float* lt, int i, int from, int cols) {
-        const float y0 = ex2(fmaf(x[0], c2, lt[i])), y1 = ex2(fmaf(x[1], c2, lt[i + 1]));
-        return pair(i >= from && i < cols ? y0 : 0.0f, i + 1 >= from && i + 1 < cols ? y1 : 0.0f);
-    };
     uint32_t g = 0, item = 0;
     Walk w(B);
     while (w.next(a)) {
@@ -254,9 +249,10 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
             tc_fence_after();
             const int cols = w.cols(a, it);
             if ((warp & 3) * 32 < slots && cols > 0) {
-                // columns [from, cols) see this thread's slot
+                // columns [from, cols) see this thread's slot; outside them a score may hold anything
                 const int gap = j - past - w.tok0(a, it);
                 const int from = gap > 0 ? min(gap, a.tq) * a.G : 0;
+                auto counts = [&](int i) { return (uint32_t)(i - from) < (uint32_t)max(0, cols - from); };
                 const float* lt = lse2 + buf * 128;
                 const uint32_t s_col = lanes + buf * 128;
                 uint64_t sum[2] = {0, 0};
@@ -270,23 +266,41 @@ __device__ __forceinline__ void sum_role(const WeightArgs& a, Bars* B, const flo
                     if (C::CAP) cap_scores(x, cap_in, a.softcap);
                     if (some_cols || i + 32 > cols) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 2)
-                            if (i + k < cols) sum[0] = add2(sum[0], some(x + k, lt, i + k, from, cols));
-                    } else {
+                        for (int k = 0; k < 32; ++k) x[k] = counts(i + k) ? x[k] : -INFINITY;
+                    }
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            const float4 L = *reinterpret_cast<const float4*>(lt + i + k);
-                            float y0, y1, y2, y3;
-                            unpair(fma2(pair(x[k], x[k + 1]), c22, pair(L.x, L.y)), y0, y1);
-                            unpair(fma2(pair(x[k + 2], x[k + 3]), c22, pair(L.z, L.w)), y2, y3);
-                            sum[0] = add2(sum[0], pair(ex2(y0), ex2(y1)));
-                            sum[1] = add2(sum[1], pair(ex2(y2), ex2(y3)));
-                        }
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 L = *reinterpret_cast<const float4*>(lt + i + k);
+                        float y0, y1, y2, y3;
+                        unpair(fma2(pair(x[k], x[k + 1]), c22, pair(L.x, L.y)), y0, y1);
+                        unpair(fma2(pair(x[k + 2], x[k + 3]), c22, pair(L.z, L.w)), y2, y3);
+                        sum[0] = add2(sum[0], pair(ex2(y0), ex2(y1)));
+                        sum[1] = add2(sum[1], pair(ex2(y2), ex2(y3)));
                     }
                 }
                 float s0, s1;
                 unpair(add2(sum[0], sum[1]), s0, s1);
-                total += s0 + s1;
+                float s = s0 + s1;
+                // A sum that is not a number is taken again, in the same order, from the rows that add
+                // something alone: one with lse = -inf (lt = -inf) does not, whatever its q, nor one that does
+                // not see the slot, whatever its lse.
+                if (__any_sync(~0u, s != s && slot < slots)) {
+                    sum[0] = sum[1] = 0;
+#pragma unroll 1
+                    for (int i = 0; i < cols; i += 32) {
+                        float x[32];
+                        tmem_ld32(s_col + i, *reinterpret_cast<uint32_t(*)[32]>(x));
+                        tmem_ld_wait();
+                        if (C::CAP) cap_scores(x, cap_in, a.softcap);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) x[k] = counts(i + k) && lt[i + k] != -INFINITY ? ex2(fmaf(x[k], c2, lt[i + k])) : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) sum[k >> 1 & 1] = add2(sum[k >> 1 & 1], pair(x[k], x[k + 1]));
+                    }
+                    unpair(add2(sum[0], sum[1]), s0, s1);
+                    s = s0 + s1;
+                }
+                total += s;
             }
             tc_fence_before();
             __syncwarp();

@@ -128,3 +128,26 @@ def test_workspaces_of_the_stated_sizes(dev, q_len, dtype):
             if n:
                 with pytest.raises(mlz_b200.MlzcError, match="workspace"):
                     call(ws[:n - 1])
+
+
+# ------------------------------------------------------------------ tokens that are to add nothing
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("softcap", [0.0, 8.0])
+def test_weights_of_tokens_without_lse_add_nothing_whatever_their_q(dev, dtype, softcap):
+    c = ref.make(dev, [3, 150, 1, 1], [20, 400, 30, 300], dtype=dtype, seed=9)
+    _, lse, _, _ = ref.attn(c, softcap)
+    lse = lse.float().contiguous()
+    dead = torch.zeros(c.T, dtype=torch.bool, device=dev)
+    dead[[1, 77, 130, 153]] = True
+    lse[dead] = -math.inf
+    c.q[dead] = 0.0
+    want, bound = ref.weights(c, lse, softcap)
+    real = ~torch.isnan(want)
+    for x in (0.0, math.nan, math.inf, -math.inf):
+        c.q[dead] = x
+        got = mlz_b200.paged_weights(ref.handle(c), c.q, lse, c.scale, softcap=softcap)
+        assert ((got.double() - want).abs() <= bound)[real].all(), f"q = {x}"
+        first = got if x == 0.0 else first
+        assert torch.equal(got, first), f"q = {x}"
+        assert (got[2, :, :30] == 0).all()   # a sequence whose only token adds nothing
