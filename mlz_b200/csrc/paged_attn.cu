@@ -382,6 +382,30 @@ __device__ __forceinline__ void each32(uint32_t s_col, F f) {
     }
 }
 
+// A row's scores s go into P = 2^(c2 s + off), off = kPOffset - c2 m with their maximum m: one rounding
+// a row and one a score.  The first is half a last place of c2 m: far from 0 it would move P by more
+// than a few powers of two, until P and its sum leave their types.  There m is taken from the scores first.
+constexpr float kFar = 0x1p22f;
+__device__ __forceinline__ float offset(float m, float c2) { return m == -INFINITY ? 0.0f : kPOffset - m * c2; }
+__device__ __forceinline__ bool is_far(float off) { return fabsf(off) > kFar; }
+
+// N scores at s_col less the maximum m of a far row, back in place; the row's offset then.
+template <int N>
+__device__ __forceinline__ float shift_row(uint32_t s_col, float m, float off) {
+    const float shift = is_far(off) ? m : 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < N; i += 16) {
+        float v[16];
+        tmem_ld16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] -= shift;
+        tmem_st16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(v));
+    }
+    tmem_st_wait();
+    return is_far(off) ? kPOffset : off;
+}
+
 // N scores at s_col capped, those past `limit` masked where `cut`, back in place; the largest.
 template <int N>
 __device__ __forceinline__ float cap_row(uint32_t s_col, float cap_in, float cap, bool cut, int limit) {
@@ -419,6 +443,7 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
         const bool real = q.real(a, w, slot), busy = __any_sync(~0u, real);
         const int own = w.s.kv - w.s.rows + q.tok(a, w, slot);   // last slot this row sees
         float m = -INFINITY, l = 0.0f;
+        float off = 0.0f;                                // of m
         for (int it = 0; it < w.n * H; ++it, ++g) {
             // barriers 2 * query tile + half, or the buffer; either way one phase in two steps
             const int buf = C::NS == 1 ? (int)(g & 1) : (H == 2 ? 2 * slot + (int)(g & 1) : slot);
@@ -428,15 +453,21 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                 const uint32_t s_col = lanes + C::kSCol + buf * N;
                 const int limit = own - w.tile * BN - it * N;
                 const bool cut = __any_sync(~0u, limit < N - 1);
-                // the running maximum with a step's; O follows where it rises far
+                bool far = false;                        // some row of the warp is
+                // the running maximum with a step's; O follows where it rises far (far rows come
+                // by every time: a vote of their own cost 64 dims 3 %)
                 auto raise = [&](float top) {
                     if (it == 0) {
                         m = top;
-                    } else if (__any_sync(~0u, top > m + rise)) {
-                        const float to = top > m + rise ? top : m;
+                        off = offset(m, c2);
+                        far = __any_sync(~0u, is_far(off));
+                    } else if (__any_sync(~0u, top - m > rise || is_far(off))) {
+                        const float to = top - m > rise ? top : m;
                         const float al = m == -INFINITY ? 0.0f : ex2((m - to) * c2);
                         m = to;
                         l *= al;
+                        off = offset(m, c2);
+                        far = __any_sync(~0u, is_far(off));
                         // O has the products of the steps before the last (this S came after
                         // them); wait for the last's
                         if (!mbar_wait(smem_u32(&B->o_step[slot]), (g - 1) & 1, abort, a.c.err)) return false;
@@ -456,8 +487,8 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                 if constexpr (C::CAP) {
                     const float top = cap_row<N>(s_col, cap_in, a.softcap, cut, limit);
                     if (!raise(top)) return;
-                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
-                    each32<N>(s_col, [&](int i, float (&v)[32]) { l += weigh<C::kPoly>(v, c2, off, s_col + i); });
+                    const float add = far ? shift_row<N>(s_col, m, off) : off;
+                    each32<N>(s_col, [&](int i, float (&v)[32]) { l += weigh<C::kPoly>(v, c2, add, s_col + i); });
                 } else {
                     float x[N];
 #pragma unroll
@@ -469,7 +500,15 @@ __device__ __forceinline__ void softmax_role(const AttnArgs& a, Bars* B, uint32_
                         for (int i = 0; i < N; ++i) x[i] = i > limit ? -INFINITY : x[i];
                     }
                     if (!raise(row_max(x))) return;
-                    l += weigh<C::kPoly>(x, c2, m == -INFINITY ? 0.0f : kPOffset - m * c2, s_col);
+                    float add = off;
+                    if (far) {
+                        const float shift = is_far(off) ? m : 0.0f;
+                        const uint64_t sh = pair(-shift, -shift);
+#pragma unroll
+                        for (int i = 0; i < N; i += 2) unpair(add2(pair(x[i], x[i + 1]), sh), x[i], x[i + 1]);
+                        add = is_far(off) ? kPOffset : off;
+                    }
+                    l += weigh<C::kPoly>(x, c2, add, s_col);
                 }
                 tmem_st_wait();
             }
@@ -544,7 +583,13 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                         for (int i = 0; i < 32; ++i) x[i] = clip(x[i], c0 + i);
                     }
                     m = row_max(x);
-                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                    float off = offset(m, c2);
+                    if (__any_sync(~0u, is_far(off))) {
+                        const float shift = is_far(off) ? m : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] -= shift;
+                        off = is_far(off) ? kPOffset : off;
+                    }
                     uint32_t p[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
@@ -582,7 +627,8 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                         }
                         if (cut) tmem_st_wait();
                     }
-                    const float off = m == -INFINITY ? 0.0f : kPOffset - m * c2;
+                    float off = offset(m, c2);
+                    if (__any_sync(~0u, is_far(off))) off = shift_row<BN>(s_col, m, off);
                     float x[16];
                     tmem_ld16(s_col, *reinterpret_cast<uint32_t(*)[16]>(x));
                     tmem_ld_wait();

@@ -151,3 +151,63 @@ def test_weights_of_tokens_without_lse_add_nothing_whatever_their_q(dev, dtype, 
         first = got if x == 0.0 else first
         assert torch.equal(got, first), f"q = {x}"
         assert (got[2, :, :30] == 0).all()   # a sequence whose only token adds nothing
+
+
+# ------------------------------------------------------------------ scores of any size
+
+def _check_far_scores(c, softcap, scales):
+    """q and k of c have one dim of a few bits, so products and differences of scores are exact; no
+    two different scores are within 2^-11 of one another."""
+    vmax = float(c.v.abs().max())
+    for e in scales:
+        c.scale = 1.37 * 2.0 ** e
+        # (softmax by differences of scores: at 2^44 the lse's own 64-bit rounding is 2^-10)
+        want, want_lse = torch.zeros(c.q.shape, dtype=torch.float64, device=c.q.device), torch.zeros(c.q.shape[:2], dtype=torch.float64, device=c.q.device)
+        for r in range(c.group):
+            x, _ = ref.score_rows(c, 0, 0, r, softcap)
+            want[:, r], want_lse[:, r] = torch.softmax(x, dim=-1) @ ref.rows(c, c.v, 0, 0), torch.logsumexp(x, dim=-1)
+        top = float(want_lse.abs().max())
+        if softcap and top > 2.0 ** 36:   # of cap 2^40: nearer to it, f32 does not hold the scores apart
+            continue
+        out, lse = mlz_b200.paged_attn(ref.handle(c), c.q, c.scale, softcap=softcap, return_lse=True)
+        # a weight is off by its score's rounded difference from the largest, d: 2^-24 of the scale, its
+        # product with log2 e and the difference's, below 2^-20 of d, and d exp(-d) < 0.37; then as in every
+        # call.  With a cap also by each score's own 2^-20, which past 2^15 moves no weight off 0 or 1
+        own = 2.0 ** -20 * top if softcap and top < 2.0 ** 15 else 0.0
+        worst = float((out.double() - want).abs().nan_to_num(math.inf).max())
+        bound = vmax * (2.0 ** -18 + 4 * own + (0.0 if c.q.dtype == F32 else 2.0 ** -10))
+        assert worst <= bound, f"scale 2^{e}: out off by {worst:.2e}, bound {bound:.2e}"
+        worst = float(((lse.double() - want_lse) / want_lse.abs().clamp(min=8)).abs().nan_to_num(math.inf).max())
+        assert worst <= 2.0 ** -19, f"scale 2^{e}: lse off by {worst:.2e}"
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("softcap", [0.0, 2.0 ** 40])
+@pytest.mark.parametrize("q", [1.3125, -1.3125, 20000.0])
+@pytest.mark.parametrize("T", [1, 140])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attn_of_scores_past_f32s_fractions(dev, D, T, q, softcap, dtype):
+    """Scores of 2^26 to 2^56 are weights of 1 for the largest and 0 for the others."""
+    c = ref.make(dev, [T], [300], hkv=1, group=2, D=D, seed=1, junk=False, dtype=dtype)
+    rank = torch.randperm(300, generator=torch.Generator().manual_seed(2)).to(dev)
+    slot = torch.arange(300, device=dev)
+    c.q.zero_()
+    c.k.zero_()
+    c.q[:, :, 3] = q
+    c.k[c.table[0].long()[slot // c.page], 0, slot % c.page, 3] = ((rank + 100) / 32).half()
+    _check_far_scores(c, softcap, (0, 9, 16, 19, 20, 21, 22, 24, 26, 28, 32, 38))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("softcap", [0.0, 2.0 ** 40])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attn_of_far_scores_that_rise_from_tile_to_tile(dev, D, softcap, dtype):
+    """Several slot tiles a CTA, each with larger scores than the one before."""
+    n = 60000
+    c = ref.make(dev, [1], [n], hkv=1, group=2, D=D, page=128, seed=1, junk=False, dtype=dtype)
+    slot = torch.arange(n, device=dev)
+    c.q.zero_()
+    c.k.zero_()
+    c.q[:, :, 3] = 1.3125
+    c.k[c.table[0].long()[slot // c.page], 0, slot % c.page, 3] = ((slot // 64 + 100) / 32).half()
+    _check_far_scores(c, softcap, (9, 18, 20, 22, 24, 28, 31, 38))
