@@ -211,3 +211,31 @@ def test_attn_of_far_scores_that_rise_from_tile_to_tile(dev, D, softcap, dtype):
     c.q[:, :, 3] = 1.3125
     c.k[c.table[0].long()[slot // c.page], 0, slot % c.page, 3] = ((slot // 64 + 100) / 32).half()
     _check_far_scores(c, softcap, (9, 18, 20, 22, 24, 28, 31, 38))
+
+
+# ------------------------------------------------------------------ the exponentials
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lse_has_the_precision_of_f32_exponentials(dev, D, dtype):
+    """Row r: one slot with score 0 and eight, in places where any form of the exponential may be
+    used, with score -q_r; everything else counts for nothing.  q and k have one dim of few bits."""
+    T = 150
+    c = ref.make(dev, [T], [300], hkv=1, group=1, D=D, page=64, seed=1, junk=False, dtype=dtype)
+    q = (1.0 + torch.arange(T, device=dev) / 512).to(dtype)
+    k = torch.full((300,), -60000.0, device=dev)
+    k[0], k[[6, 7, 14, 15, 22, 23, 30, 31]] = 0.0, -1.0
+    slot = torch.arange(300, device=dev)
+    c.q.zero_()
+    c.k.zero_()
+    c.q[:, 0, 3] = q
+    c.k[c.table[0].long()[slot // c.page], 0, slot % c.page, 3] = k.half()
+    _, lse = mlz_b200.paged_attn(ref.handle(c), c.q, 1.0, return_lse=True)
+    want = torch.log1p(8 * torch.exp(-q.double()))
+    # an exponent below 8 rounded (2^-22 ln 2) with log2 e's own rounding (2^-24 of 1.3), the
+    # exponential (2^-22), nine additions (2^-24 each), log2 of a sum below 2^8 to one last place
+    # (2^-21 ln 2), its sum with the offset and the product with ln 2 (values below 2: 2^-23 in all)
+    ln2 = math.log(2.0)
+    bound = 2.0 ** -22 * ln2 + 1.3 * 2.0 ** -24 + 2.0 ** -22 + 9 * 2.0 ** -24 + 2.0 ** -21 * ln2 + 2.0 ** -23
+    worst = float((lse[:, 0].double() - want).abs().max())
+    assert worst <= bound, f"lse off by {worst:.2e}, bound {bound:.2e}"
