@@ -627,10 +627,16 @@ __device__ __forceinline__ void softmax_tile_role(const AttnArgs& a, Bars* B, fl
                         }
                         if (cut) tmem_st_wait();
                     }
-                    float off = offset(m, c2);
-                    if (__any_sync(~0u, is_far(off))) off = shift_row<BN>(s_col, m, off);
-                    float x[16];
+                    float x[16];                         // (under way during the vote: 256 dims 775 us for 800)
                     tmem_ld16(s_col, *reinterpret_cast<uint32_t(*)[16]>(x));
+                    float off = offset(m, c2);
+                    if (__any_sync(~0u, is_far(off))) {
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) asm volatile("" ::"f"(x[j]));   // until here the load's
+                        off = shift_row<BN>(s_col, m, off);
+                        tmem_ld16(s_col, *reinterpret_cast<uint32_t(*)[16]>(x));
+                    }
                     tmem_ld_wait();
 #pragma unroll 1
                     for (int i = 0; i < BN; i += 16) {
