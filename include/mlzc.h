@@ -274,7 +274,8 @@ typedef struct {
 } mlzc_paged_store_desc;
 
 /* Writes the new tokens' rotated k and their v into the cache (rounded to f16 once) and the
- * rotated q to q_dst, on `stream`.  Angles are exact to 2^-29 of a turn at any position (2^-32 below 2^24).
+ * rotated q to q_dst, on `stream`.  Angles are exact to 2^-27 of a turn at any position (where
+ * freq_base is at least 1 and |freq_scale| at most 1; a larger scale costs far positions its bits).
  * Two tokens with one slot, or sequences sharing a page that is written, race. */
 int mlzc_paged_store_dev(const mlzc_paged_cache* cache, const mlzc_paged_store_desc* desc, void* stream);
 

@@ -7,7 +7,8 @@
 // F_j = freq_j / 2 pi * 2^64 (computed once on the host in extended precision and passed as a
 // kernel argument), pos * F_j modulo 2^64 IS the fraction: the integer product drops whole
 // turns exactly, so a position of two million is nearly as exact as position two (f32 angles of far
-// positions lose all their bits).  The top 32 bits go to sincospi.
+// positions lose all their bits).  What lies beyond the nearest quarter turn goes to sincospi: within
+// an eighth of a turn f32 holds it to 2^-28 of one (2^-26 over the whole turn).
 //
 // Bound by HBM (each row read once, written once; in f32 6 bytes a k or v value, 8 a q value)
 // and, for a decode step, by launch latency.  One block handles one token and a range of its
@@ -90,9 +91,11 @@ __global__ void __launch_bounds__(kThreads) store_kernel(const __grid_constant__
     for (int j = threadIdx.x; j < a.half; j += kThreads) {
         const int64_t pos = paged::ld_int(reinterpret_cast<const int*>(reinterpret_cast<const char*>(a.pos) + a.axis[j] * a.pos_nb) + t);
         const uint64_t turns = (uint64_t)pos * a.turn[j];
+        const uint32_t quarter = (uint32_t)((turns + (1ull << 61)) >> 62);
         float sn, cn;
-        sincospif((float)(int32_t)(turns >> 32) * 0x1p-31f, &sn, &cn);
-        cs[j] = make_float2(cn, sn);
+        sincospif((float)(int64_t)(turns - ((uint64_t)quarter << 62)) * 0x1p-63f, &sn, &cn);
+        const float2 at = quarter & 1 ? make_float2(-sn, cn) : make_float2(cn, sn);
+        cs[j] = quarter & 2 ? make_float2(-at.x, -at.y) : at;
     }
     __syncthreads();
     const int heads = a.n_head_q + 2 * c.n_head_kv;

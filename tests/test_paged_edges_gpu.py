@@ -239,3 +239,37 @@ def test_lse_has_the_precision_of_f32_exponentials(dev, D, dtype):
     bound = 2.0 ** -22 * ln2 + 1.3 * 2.0 ** -24 + 2.0 ** -22 + 9 * 2.0 ** -24 + 2.0 ** -21 * ln2 + 2.0 ** -23
     worst = float((lse[:, 0].double() - want).abs().max())
     assert worst <= bound, f"lse off by {worst:.2e}, bound {bound:.2e}"
+
+
+# ------------------------------------------------------------------ angles
+
+@pytest.mark.parametrize("pairs", ["halves", "adjacent"])
+@pytest.mark.parametrize("first,base", [(0, 10000.0), (10 ** 6, 500000.0), (2 ** 31 - 5000, 10000.0), (-2 ** 31, 500000.0)])
+def test_store_angles(dev, first, base, pairs):
+    """Pairs (1, 0) become (cos, sin) themselves."""
+    from fractions import Fraction
+    T, D, half = 600, 128, 64
+    c = ref.make(dev, [T], [T], hkv=1, group=1, D=D, page=64, seed=71, junk=False)
+    g = torch.Generator().manual_seed(3)
+    pos = (first + torch.randint(0, 4000, (T,), generator=g)).to(torch.int32)
+    one = torch.zeros((T, 1, D), device=dev)
+    one[..., slice(0, half) if pairs == "halves" else slice(0, D, 2)] = 1.0
+    got = mlz_b200.paged_store(ref.handle(c), one, one, q=one, positions=pos.to(dev), n_rot=D, pairs=pairs, freq_base=base)
+    got = got[:, 0].double().cpu()
+    co, si = (got[:, :half], got[:, half:]) if pairs == "halves" else (got[:, ::2], got[:, 1::2])
+    # turns of a position, rounded to 2^-100 (the powers of base by square roots of rationals)
+    one100 = 1 << 100
+    two_pi = Fraction(6283185307179586476925286766559005768394, 10 ** 39)
+    step, x = Fraction(int(base)), []
+    for _ in range(6):   # base ^ (1 / 64)
+        step = Fraction(math.isqrt(int(step * one100 * one100)), one100)
+    freq = Fraction(1)
+    for _ in range(half):
+        x.append(round(freq / two_pi * one100))
+        freq = Fraction(int(freq / step * one100), one100)
+    # 2^-27 of a turn; the functions to one last place of values below 1
+    bound = 2 * math.pi * 2.0 ** -27 + 2.0 ** -24
+    for j in range(half):
+        turn = torch.tensor([((int(p) * x[j]) % one100) / one100 for p in pos], dtype=torch.float64) * (2 * math.pi)
+        worst = max(float((co[:, j] - torch.cos(turn)).abs().max()), float((si[:, j] - torch.sin(turn)).abs().max()))
+        assert worst <= bound, f"pair {j}: off by {worst:.2e}, bound {bound:.2e}"
