@@ -305,7 +305,8 @@ int mlzc_paged_attn_workspace_bytes(const mlzc_paged_cache* cache, const mlzc_pa
  * type F32: q, the weights and the sums keep f32 precision (q and the softmax weights go
  * through the tensor cores as f16 hi + lo pairs, so |q| <= 65504, and parts of q below
  * 2^-25 are lost); type F16: q is f16 as given, the softmax
- * weights are rounded to f16 once, sums are f32, dst is rounded once.
+ * weights are rounded to f16 once (in out; lse is that of the weights before), sums are f32, dst
+ * is rounded once.
  * K and V of the slots below kv_len are finite. */
 int mlzc_paged_attn_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, void* workspace,
                         size_t workspace_bytes, void* stream);
@@ -318,7 +319,8 @@ int mlzc_paged_weights_workspace_bytes(const mlzc_paged_cache* cache, const mlzc
  * acc NULL starts from 0, acc == out accumulates in place (with the same strides).  f32,
  * byte strides nb = slot (4), head, sequence.  desc: q, scale, mode, softcap and lse as given
  * to and returned by mlzc_paged_attn_dev; dst is not used.  A token with lse = -inf adds
- * nothing.  The result repeats bit for bit. */
+ * nothing, whatever its q.  What is subtracted is f32, so a weight is off by up to 2^-23 |lse| of
+ * itself.  The result repeats bit for bit. */
 int mlzc_paged_weights_dev(const mlzc_paged_cache* cache, const mlzc_paged_attn_desc* desc, const float* acc,
                            const size_t acc_nb[3], float* out, const size_t out_nb[3], void* workspace,
                            size_t workspace_bytes, void* stream);

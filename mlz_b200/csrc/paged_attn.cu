@@ -36,9 +36,9 @@
 // quarter of the slots (P is 0 in the others); the correction warps add the copies up at the end
 // of a piece.
 //
-// Measured (device times): 4096 new of 16384 slots, 8 KV heads of 4, 128 dims: f16 870-940 us (1030-1110
-// TFLOP/s, by the clock), f32 1650 (570, each product twice); 4096 of 8192, 4 KV heads of 4, 256 dims:
-// f16 352 us, f32 810.  Decode of 64 sequences of 4096 slots: 173 us, 6.2 TB/s, f16 and f32 alike; of 16
+// Measured (device times): 4096 new of 16384 slots, 8 KV heads of 4, 128 dims: f16 840-980 us (980-1140
+// TFLOP/s, by the clock), f32 1510-1780 (540-640, each product twice); 4096 of 8192, 4 KV heads of 4, 256
+// dims: f16 353 us, f32 775-850.  Decode of 64 sequences of 4096 slots: 173 us, 6.2 TB/s, f16 and f32 alike; of 16
 // of 512 to 8192: 55 and 57 us (5.3 TB/s); of one: 10 us of latency.
 //
 // All (sequence, KV head, query tile, slot tile) of a call form one list, of which every CTA

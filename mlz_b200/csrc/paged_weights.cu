@@ -8,10 +8,12 @@
 // The scores are recomputed (storing them would cost 4 bytes a score) as S^T = K Q^T: slots on
 // the lanes, rows on the columns.  A slot's sum then stays in one thread, so nothing is added
 // across threads and nothing atomically, and the softmax's statistics, known from the
-// attention, enter as one constant a column: one FMA, one exponential and one add a score.  The
-// exponential unit (1024 clocks a 128 x 128 tile; the products take 512) is the bound for long
-// chunks, reading K that for decode.  Moving a share of the exponentials to the FMA pipe gains
-// nothing (175 us with and without one in four, for 2048 tokens of 8192, 8 heads of 4).
+// attention, enter as one constant a column: one FMA, one exponential and one add a score.  Of a
+// long chunk's time the exponential unit (1024 clocks a 128 x 128 tile; the products take 512) is
+// busy 72 %, the tensor cores 36 % (counters, 2048 tokens of 8192, 8 heads of 4).  The unit is the
+// nearest bound, but not alone what takes the time: moving one exponential in four to the FMA pipe
+// gained nothing (175 us either way); each step waits for its 32 columns before it computes.  Decode
+// reads K at 4 TB/s with no unit busy (HBM 46 %, tensor cores 7 %, exponentials 15 %).
 //
 // A piece of work is what one operand is held for: a slot tile (K) and its query tiles, or,
 // where a sequence's rows fill one query tile at most (decode), that tile (Q) and a run of slot
@@ -22,8 +24,9 @@
 // the exponential unit idled half of the time: 205 us for 2048 tokens of 8192).  f32 queries come
 // as f16 hi + lo from a small preparing launch, low products summed first.
 //
-// Measured (device times): 2048 tokens of 8192 slots, 8 heads of 4, 128 dims: f16 175 us, f32 239 (twice
-// the products); decode of 16 sequences of 512 to 8192: 39 us (152 MB), of one of 32768: 18 us.
+// Measured (device times): 2048 tokens of 8192 slots, 8 heads of 4, 128 dims: f16 172 us, f32 231 (twice
+// the products); masked columns become -inf before the common code (selected after the exponentials
+// instead: 175 and 235); decode of 16 sequences of 512 to 8192: 38 us (152 MB), of one of 32768: 18 us.
 //
 // lse2 is rounded to f32 once a row (4e-7 of a weight at lse 10).  Carrying what that drops as a
 // factor a column made no weight better (the products' own sums are as far off) and cost 12 %.
