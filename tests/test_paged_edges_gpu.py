@@ -200,11 +200,12 @@ def test_attn_of_scores_past_f32s_fractions(dev, D, T, q, softcap, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("softcap", [0.0, 2.0 ** 40])
+@pytest.mark.parametrize("T", [1, 150])
 @pytest.mark.parametrize("D", [64, 128, 256])
-def test_attn_of_far_scores_that_rise_from_tile_to_tile(dev, D, softcap, dtype):
+def test_attn_of_far_scores_that_rise_from_tile_to_tile(dev, D, T, softcap, dtype):
     """Several slot tiles a CTA, each with larger scores than the one before."""
     n = 60000
-    c = ref.make(dev, [1], [n], hkv=1, group=2, D=D, page=128, seed=1, junk=False, dtype=dtype)
+    c = ref.make(dev, [T], [n], hkv=1, group=2, D=D, page=128, seed=1, junk=False, dtype=dtype)
     slot = torch.arange(n, device=dev)
     c.q.zero_()
     c.k.zero_()
